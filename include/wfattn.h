@@ -249,6 +249,133 @@ WFATTN_API wfattn_status_t wfattn_decode_noalloc(int64_t batch, int64_t heads, i
                                                  void *stream);
 
 /*
+ * Key/value caches -- no counterpart in the reference, which has no KV cache
+ * (demo/README.md:45).  A wfattn_cache_t describes a cache that the caller
+ * owns: rows of one token and one head, head_dim values each, of K and of V,
+ * [batch, heads, max_len] rows of each.
+ *
+ * Row formats (head_dim = D):
+ *  WFATTN_CACHE_F32, WFATTN_CACHE_BF16: D values; no scales.
+ *  WFATTN_CACHE_E4M3: D e4m3 codes, and one f32 scale a row in k_scale /
+ *    v_scale.  A value is code * scale.  wfattn_cache_write takes as scale the
+ *    smallest power of two s >= 2^-126 with max|x| <= 448 s, so x / s is exact
+ *    and each value is rounded once (to nearest even).
+ *  WFATTN_CACHE_INT4: D 4-bit codes u (value 2i in the low half of byte i), and
+ *    two bf16 numbers (s, m) a row in k_scale / v_scale.  A value is m + s u.
+ *    wfattn_cache_write takes as m the largest bf16 <= min(x), as s the
+ *    smallest bf16 >= (max(x) - m) / 15 (in f32), and as u (x - m) / s in f32
+ *    rounded to nearest even, in 0..15 (0 where s = 0).
+ * A row that holds a NaN or an infinity (or, for INT4, spans more than f32
+ * does) is stored by the last two with a NaN scale and codes 0: it reads back
+ * as NaN in every value.
+ *
+ * Row (b, h, t) of K, of V and of their scales is number
+ * b * batch_stride + h * head_stride + t of its array; rows do not overlap
+ * (head_stride >= max_len and batch_stride >= the rows of a batch entry, or
+ * the other way round; a stride over a size of 1 is not looked at).  k and v
+ * are 16-byte aligned, the scales 4-byte aligned.  head_dim is 64 or 128;
+ * batch * heads * max_len is at most 2^31 - 1 rows.
+ *
+ * Lengths and positions are DEVICE int32 arrays.  An entry that points outside
+ * the cache reads and writes nothing there, and wfattn_device_status() then
+ * returns WFATTN_INVALID_ARG; each call says what it does with it.
+ */
+typedef enum {
+  WFATTN_CACHE_F32 = 0,
+  WFATTN_CACHE_BF16 = 1,
+  WFATTN_CACHE_E4M3 = 2,
+  WFATTN_CACHE_INT4 = 3
+} wfattn_cache_format_t;
+
+typedef struct wfattn_cache {
+  int32_t format; /* wfattn_cache_format_t */
+  int32_t head_dim;
+  int64_t batch, heads, max_len;
+  int64_t batch_stride, head_stride; /* in rows */
+  void *k, *v;
+  void *k_scale, *v_scale; /* NULL for F32 and BF16 */
+} wfattn_cache_t;
+
+/*
+ * Writes new rows: for every b and h, rows starts[b] .. starts[b]+counts[b]-1
+ * of K and V take the first counts[b] of the n_rows rows of k and v
+ * ([batch, heads, n_rows, head_dim] of `dtype`, f32 or bf16, with strides
+ * {batch, head, row}; any alignment of the element).  counts NULL: n_rows for
+ * every b.  Other rows are left as they are.  Row positions below 0 or past
+ * max_len are not written; a count outside 0..n_rows is clamped (both are
+ * recorded, see above).  n_rows 0 does nothing.
+ */
+WFATTN_API wfattn_status_t wfattn_cache_write(const wfattn_cache_t *cache, int dtype,
+                                              int64_t n_rows, const void *k,
+                                              const int64_t *k_strides, const void *v,
+                                              const int64_t *v_strides, const int32_t *starts,
+                                              const int32_t *counts, void *stream);
+
+/*
+ * Reads rows back: for every b and h, the first counts[b] of the n_rows rows
+ * of k and v ([batch, heads, n_rows, head_dim] of `dtype`) take the values of
+ * rows starts[b] .. starts[b]+counts[b]-1, computed in f32 and rounded once.
+ * The other rows of k and v, and those whose position is outside the cache,
+ * are left as they are, or set to zero where zero_rest is not 0.
+ */
+WFATTN_API wfattn_status_t wfattn_cache_read(const wfattn_cache_t *cache, int dtype,
+                                             int64_t n_rows, void *k, const int64_t *k_strides,
+                                             void *v, const int64_t *v_strides,
+                                             const int32_t *starts, const int32_t *counts,
+                                             int zero_rest, void *stream);
+
+/*
+ * Keeps the accepted nodes of a drafted tree: for every b and h and every i <
+ * counts[b], row lens[b] + i of K and V becomes what row lens[b] + path[b][i]
+ * was before the call (rows as stored, scales with them; any order of the
+ * path, repeated entries too), and new_lens[b] = lens[b] + counts[b].  path is
+ * [batch, depth] with rows path_stride entries apart, depth at most 64; counts
+ * NULL: depth for every b.  new_lens is another array than lens
+ * (WFATTN_INVALID_ARG): every head reads lens.
+ * A sequence with a negative length, a count outside 0..depth, or a source or
+ * destination row outside the cache moves nothing and keeps its length.
+ */
+WFATTN_API wfattn_status_t wfattn_cache_keep(const wfattn_cache_t *cache, const int32_t *lens,
+                                             int64_t depth, const int32_t *path,
+                                             int64_t path_stride, const int32_t *counts,
+                                             int32_t *new_lens, void *stream);
+
+/*
+ * Attention of a tree of drafted tokens over a cache (one token: decode).
+ *
+ * q, o:   [batch, heads_q, nodes, head_dim] of `dtype`, strides {batch, head,
+ *         node} in elements; query head h reads cache head h / (heads_q /
+ *         heads).  BF16 queries take a BF16, E4M3 or INT4 cache, F32 queries an
+ *         F32, E4M3 or INT4 one.  Scores, softmax and sums are held in f32; F32
+ *         outputs keep the f32 path's accuracy (~1e-6 of the values).
+ * lens:   rows before the tree, lens[b] >= 0: every node sees them all.
+ * nodes:  1..64 nodes; node j of sequence b is row lens[b] + j of the cache
+ *         (written by wfattn_cache_write before this call).
+ * tree:   64-bit words [batch, nodes], tree_stride words from one sequence to
+ *         the next (0: one tree for all): node i sees node j when bit j of its
+ *         word is set.  NULL: node i sees nodes 0..i.
+ * counts: nodes of each sequence, 0..nodes (NULL: all); the rest is padding.
+ *         Padding nodes, and nodes that see nothing, give zeros.
+ * Rows that a node does not see do not reach its output, whatever they hold.
+ * A negative length counts as 0, a count is clamped to 0..nodes, and rows past
+ * max_len are not read (recorded, see above).
+ * scale <= 0 selects 1/sqrt(head_dim).  workspace: at least
+ * wfattn_tree_decode_workspace_size() bytes (0 for a bad cache or size),
+ * 16-byte aligned; calls that share one must be ordered on one stream.
+ */
+WFATTN_API size_t wfattn_tree_decode_workspace_size(const wfattn_cache_t *cache, int dtype,
+                                                    int64_t heads_q, int64_t nodes);
+
+WFATTN_API wfattn_status_t wfattn_tree_decode(const wfattn_cache_t *cache, int dtype,
+                                              int64_t heads_q, int64_t nodes, const void *q,
+                                              const int64_t *q_strides, const int32_t *lens,
+                                              const uint64_t *tree, int64_t tree_stride,
+                                              const int32_t *counts, void *o,
+                                              const int64_t *o_strides, float scale,
+                                              void *workspace, size_t workspace_bytes,
+                                              void *stream);
+
+/*
  * Peer buffers -- no counterpart in the reference, which runs on one GPU.
  *
  * Device memory that other processes on the node can map, for the outputs of
@@ -281,7 +408,8 @@ WFATTN_API wfattn_status_t wfattn_peer_free(void *ptr, int device);
 /*
  * Reads (and optionally clears) the device-side status word of the current
  * device: WFATTN_OK, or WFATTN_TIMEOUT when a bounded wait inside a kernel
- * (TMA/MMA pipeline barrier) gave up and the kernel returned early.
+ * (TMA/MMA pipeline barrier) gave up and the kernel returned early, or
+ * WFATTN_INVALID_ARG when a device-side length or position was out of range.
  * Synchronizes `stream` first.
  */
 WFATTN_API wfattn_status_t wfattn_device_status(void *stream, int clear);

@@ -16,13 +16,16 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libwfattn.so"
 OK, INVALID_ARG, UNSUPPORTED, CUDA_ERROR, TIMEOUT = range(5)
 # wfattn_dtype_t
 DTYPE_F32, DTYPE_BF16 = 0, 1
+# wfattn_cache_format_t
+CACHE_F32, CACHE_BF16, CACHE_E4M3, CACHE_INT4 = range(4)
 
 EXPORTED_SYMBOLS = (
     "wfattn_version", "wfattn_status_string", "wfattn_last_error", "wfattn_attention",
     "wfattn_prefill", "wfattn_prefill_gather", "wfattn_prefill_multicast",
     "wfattn_decode_workspace_size", "wfattn_decode",
     "wfattn_decode_f32_workspace_size", "wfattn_decode_f32", "wfattn_decode_noalloc", "wfattn_device_status", "wfattn_peer_alloc", "wfattn_peer_open",
-    "wfattn_peer_close", "wfattn_peer_free",
+    "wfattn_peer_close", "wfattn_peer_free", "wfattn_cache_write", "wfattn_cache_read",
+    "wfattn_cache_keep", "wfattn_tree_decode_workspace_size", "wfattn_tree_decode",
 )
 
 
@@ -42,6 +45,16 @@ class PeerHandle(ctypes.Structure):
     """wfattn_peer_handle_t: 64 opaque bytes naming a device buffer across processes."""
 
     _fields_ = [("bytes", ctypes.c_ubyte * 64)]
+
+
+class Cache(ctypes.Structure):
+    """wfattn_cache_t: a key/value cache that the caller owns."""
+
+    _fields_ = [("format", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("batch", ctypes.c_int64), ("heads", ctypes.c_int64),
+                ("max_len", ctypes.c_int64), ("batch_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
 
 
 _lib = None
@@ -98,6 +111,21 @@ def load() -> ctypes.CDLL:
     lib.wfattn_peer_close.argtypes = [_vp, ctypes.c_int]
     lib.wfattn_peer_free.restype = ctypes.c_int
     lib.wfattn_peer_free.argtypes = [_vp, ctypes.c_int]
+    _cache = ctypes.POINTER(Cache)
+    lib.wfattn_cache_write.restype = ctypes.c_int
+    lib.wfattn_cache_write.argtypes = [_cache, ctypes.c_int, _i64, _vp, _i64p, _vp, _i64p, _vp,
+                                       _vp, _vp]
+    lib.wfattn_cache_read.restype = ctypes.c_int
+    lib.wfattn_cache_read.argtypes = [_cache, ctypes.c_int, _i64, _vp, _i64p, _vp, _i64p, _vp,
+                                      _vp, ctypes.c_int, _vp]
+    lib.wfattn_cache_keep.restype = ctypes.c_int
+    lib.wfattn_cache_keep.argtypes = [_cache, _vp, _i64, _vp, _i64, _vp, _vp, _vp]
+    lib.wfattn_tree_decode_workspace_size.restype = ctypes.c_size_t
+    lib.wfattn_tree_decode_workspace_size.argtypes = [_cache, ctypes.c_int, _i64, _i64]
+    lib.wfattn_tree_decode.restype = ctypes.c_int
+    lib.wfattn_tree_decode.argtypes = [_cache, ctypes.c_int, _i64, _i64, _vp, _i64p, _vp, _vp,
+                                       _i64, _vp, _vp, _i64p, ctypes.c_float, _vp,
+                                       ctypes.c_size_t, _vp]
     _lib = lib
     return lib
 
@@ -113,6 +141,11 @@ def check(status: int) -> None:
     if status != OK:
         msg = load().wfattn_last_error().decode(errors="replace")
         raise WfattnError(status, msg)
+
+
+def check_last(lib: ctypes.CDLL) -> None:
+    """Raise for a size query that returned 0: its arguments were refused."""
+    raise WfattnError(INVALID_ARG, lib.wfattn_last_error().decode(errors="replace"))
 
 
 def strides_arg(strides) -> ctypes.Array | None:

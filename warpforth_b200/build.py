@@ -36,8 +36,10 @@ NVCC_FLAGS = [
     "-I", str(ROOT / "include"),
 ]
 SOURCES = ["wfattn_api.cu", "attn_f32.cu", "attn_f32_tc_sm100.cu", "attn_bf16_sm100.cu",
-           "attn_bf16_2q_sm100.cu", "decode_sm100.cu", "tma_map.cu"]
-HEADERS = ["wfattn_internal.h", "sm100_ptx.cuh", "tma_map.h", "exp2_poly.cuh"]
+           "attn_bf16_2q_sm100.cu", "decode_sm100.cu", "cache_sm100.cu",
+           "tree_decode_sm100.cu", "tma_map.cu"]
+HEADERS = ["wfattn_internal.h", "sm100_ptx.cuh", "tma_map.h", "exp2_poly.cuh",
+           "cache_format.cuh"]
 
 
 def nvcc() -> str:

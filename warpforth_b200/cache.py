@@ -1,0 +1,299 @@
+"""Key/value caches: writing and reading rows, attention of drafted trees, keeping accepted rows.
+
+A ``KVCache`` holds the keys and values of a batch of sequences in one of four row formats
+(``fmt``): ``"f32"``, ``"bf16"``, ``"e4m3"`` (8 bits a value and a power-of-two f32 scale a row) or
+``"int4"`` (4 bits a value and a bf16 scale and minimum a row); include/wfattn.h defines them.
+The reference has no cache (demo/README.md:45); GPT-2's generation with drafted tokens
+(``gpt2.generate_drafted``) runs on these calls:
+
+* ``cache_write`` puts new rows at given positions, quantising them;
+* ``tree_decode`` attends from a tree of up to 64 drafted tokens (one token: a decode step) to the
+  rows before it and to the nodes each one follows;
+* ``cache_keep`` moves the accepted nodes' rows to the end of the sequence;
+* ``cache_read`` returns rows as f32 or bf16, e.g. as keys and values of ``attention``.
+
+Lengths and positions are int32 CUDA tensors, read on the device; an entry that points outside the
+cache reads and writes nothing there, and ``device_status`` raises.  Every call runs on the current
+stream of the cache's device.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .warpforth import _DTYPES, DecodeWorkspace, _ptr, _require_cuda, _stream_handle
+
+_FORMATS = {"f32": (_lib.CACHE_F32, torch.float32), "bf16": (_lib.CACHE_BF16, torch.bfloat16),
+            "e4m3": (_lib.CACHE_E4M3, torch.float8_e4m3fn), "int4": (_lib.CACHE_INT4, torch.uint8)}
+_BY_DTYPE = {dtype: fmt for fmt, (_, dtype) in _FORMATS.items()}
+
+MAX_NODES = 64  # of a drafted tree
+
+
+class KVCache:
+    """Keys and values of ``batch`` sequences, ``heads`` heads and up to ``max_len`` tokens.
+
+    ``k`` and ``v`` are ``[batch, heads, max_len, head_dim]`` (``"int4"``: uint8, head_dim / 2, two
+    values a byte, the even one low); ``k_scale`` and ``v_scale`` are None (``"f32"``, ``"bf16"``),
+    f32 ``[batch, heads, max_len]`` (``"e4m3"``) or bf16 ``[batch, heads, max_len, 2]`` (``"int4"``:
+    scale, minimum).  head_dim is 64 or 128.  The tensors start at zero; they belong to the object
+    and are not to be replaced.
+    """
+
+    def __init__(self, batch: int, heads: int, max_len: int, head_dim: int = 64, *,
+                 fmt: str = "bf16", device: torch.device | str = "cuda") -> None:
+        if fmt not in _FORMATS:
+            raise ValueError(f"fmt must be one of {sorted(_FORMATS)}, got {fmt!r}")
+        if min(batch, heads, max_len) < 1 or head_dim not in (64, 128):
+            raise ValueError("sizes must be >= 1 and head_dim 64 or 128")
+        rows = (batch, heads, max_len)
+        width = head_dim // 2 if fmt == "int4" else head_dim
+
+        def scale():
+            if fmt == "e4m3":
+                return torch.zeros(rows, dtype=torch.float32, device=device)
+            if fmt == "int4":
+                return torch.zeros((*rows, 2), dtype=torch.bfloat16, device=device)
+            return None
+
+        k, v = (torch.zeros((*rows, width), dtype=_FORMATS[fmt][1], device=device)
+                for _ in range(2))
+        self._set(k, v, scale(), scale())
+
+    @classmethod
+    def wrap(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
+             v_scale: torch.Tensor | None = None) -> KVCache:
+        """A cache over existing tensors, without a copy (e.g. some of a larger cache's sequences).
+
+        Their format is told by ``k``'s dtype.  A head's rows are contiguous, and all the tensors
+        have the same batch and head strides, counted in rows.
+        """
+        cache = cls.__new__(cls)
+        cache._set(k, v, k_scale, v_scale)
+        return cache
+
+    def _set(self, k, v, k_scale, v_scale) -> None:
+        for name, t in (("k", k), ("v", v)):
+            _require_cuda(name, t)
+            if t.dim() != 4 or t.dtype not in _BY_DTYPE:
+                raise ValueError(f"{name} must be [batch, heads, max_len, row] of float32, bfloat16, "
+                                 "float8_e4m3fn or uint8")
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("k and v must have one shape and dtype")
+        fmt = _BY_DTYPE[k.dtype]
+        batch, heads, max_len, width = k.shape
+        rows = (batch, heads, max_len)
+        scaled = fmt in ("e4m3", "int4")
+        parts = [("k", k, width), ("v", v, width)]
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if not scaled:
+                if t is not None:
+                    raise ValueError(f"an {fmt} cache has no {name}")
+                continue
+            _require_cuda(name, t)
+            shape = rows if fmt == "e4m3" else (*rows, 2)
+            dtype = torch.float32 if fmt == "e4m3" else torch.bfloat16
+            if t.shape != shape or t.dtype != dtype:
+                raise ValueError(f"{name} must be {dtype} of shape {shape}")
+            parts.append((name, t, 1 if fmt == "e4m3" else 2))
+        strides = set()
+        for name, t, unit in parts:
+            if t.device != k.device:
+                raise ValueError("the cache's tensors must be on one device")
+            st = t.stride()
+            if (t.dim() == 4 and st[3] != 1 and t.shape[3] > 1) or \
+                    (max_len > 1 and st[2] != unit):
+                raise ValueError(f"{name}: the rows of a head must be contiguous")
+            if (batch > 1 and st[0] % unit) or (heads > 1 and st[1] % unit):
+                raise ValueError(f"{name}: batch and head strides must be whole rows")
+            strides.add((st[0] // unit if batch > 1 else 0, st[1] // unit if heads > 1 else 0))
+        if len(strides) != 1:
+            raise ValueError("the cache's tensors must have the same strides, counted in rows")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.fmt, self.device = fmt, k.device
+        self.batch, self.heads, self.max_len = rows
+        self.head_dim = 2 * width if fmt == "int4" else width
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {self.head_dim}")
+        sb, sh = strides.pop()
+        self._c = _lib.Cache(_FORMATS[fmt][0], self.head_dim, batch, heads, max_len, sb, sh,
+                             _ptr(k), _ptr(v), _ptr(k_scale) if scaled else None,
+                             _ptr(v_scale) if scaled else None)
+        self._ref = ctypes.byref(self._c)
+
+
+def _call(cache: KVCache, fn, *args) -> None:
+    """fn(cache, *args, stream) with the cache's device current."""
+    index = cache.device.index
+    if index == torch.cuda.current_device():
+        _lib.check(fn(cache._ref, *args, _stream_handle(cache.device)))
+        return
+    with torch.cuda.device(index):
+        _lib.check(fn(cache._ref, *args, _stream_handle(cache.device)))
+
+
+def _check_ints(name: str, t: torch.Tensor, shape: tuple[int, ...], cache: KVCache,
+                dtype: torch.dtype = torch.int32) -> int:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != cache.device or \
+            t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} of shape {shape} on {cache.device}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have a unit last stride")
+    return t.data_ptr()
+
+
+def _counts(counts, cache: KVCache) -> int | None:
+    return None if counts is None else _check_ints("counts", counts, (cache.batch,), cache)
+
+
+def _check_rows(name: str, t: torch.Tensor, shape: tuple[int, ...], dtype, cache: KVCache) -> None:
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.device != cache.device:
+        raise ValueError(f"{name} must be of shape {tuple(shape)} on {cache.device}")
+    if t.dtype != dtype or dtype not in _DTYPES:
+        raise ValueError(f"{name} must be float32 or bfloat16, as its companions (got {t.dtype})")
+    if t.stride(-1) != 1:
+        raise ValueError(f"{name} must have a unit head_dim stride")
+
+
+def _strides(t: torch.Tensor) -> ctypes.Array:
+    st = t.stride()
+    return (ctypes.c_int64 * 3)(st[0], st[1], st[2])
+
+
+def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, *,
+                counts: torch.Tensor | None = None) -> None:
+    """Writes rows ``starts[b] .. starts[b] + counts[b] - 1`` of every sequence and head.
+
+    k, v: [batch, heads, n, head_dim] f32 or bf16, any batch/head/row strides; the first
+    ``counts[b]`` rows of sequence b are taken (all n without ``counts``).  The other rows of the
+    cache stay as they are.
+    """
+    _require_cuda("k", k)
+    if k.dim() != 4:
+        raise ValueError(f"k must be [batch, heads, n, head_dim], got {tuple(k.shape)}")
+    n = k.shape[2]
+    shape = (cache.batch, cache.heads, n, cache.head_dim)
+    _check_rows("k", k, shape, k.dtype, cache)
+    _check_rows("v", v, shape, k.dtype, cache)
+    at = _check_ints("starts", starts, (cache.batch,), cache)
+    _call(cache, _lib.load().wfattn_cache_write, _DTYPES[k.dtype], n, k.data_ptr(), _strides(k),
+          v.data_ptr(), _strides(v), at, _counts(counts, cache))
+
+
+def cache_read(cache: KVCache, starts: torch.Tensor, rows: int, *,
+               counts: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+               out: tuple[torch.Tensor, torch.Tensor] | None = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``starts[b] .. starts[b] + counts[b] - 1`` of every sequence and head, as values.
+
+    Returns (k, v), each [batch, heads, rows, head_dim] of ``dtype`` (float32 for an f32 cache,
+    else bfloat16, by default).  Rows from ``counts[b]`` on are zero in new tensors, and left as
+    they are in ``out``, whose strides may be any with a unit last one.
+    """
+    shape = (cache.batch, cache.heads, int(rows), cache.head_dim)
+    if out is None:
+        dtype = dtype or (torch.float32 if cache.fmt == "f32" else torch.bfloat16)
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
+        k, v = (torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
+    else:
+        k, v = out
+        for name, t in (("out[0]", k), ("out[1]", v)):
+            _check_rows(name, t, shape, dtype or k.dtype, cache)
+    at = _check_ints("starts", starts, (cache.batch,), cache)
+    _call(cache, _lib.load().wfattn_cache_read, _DTYPES[k.dtype], shape[2], k.data_ptr(),
+          _strides(k), v.data_ptr(), _strides(v), at, _counts(counts, cache),
+          1 if out is None else 0)
+    return k, v
+
+
+def cache_keep(cache: KVCache, lens: torch.Tensor, path: torch.Tensor, *,
+               counts: torch.Tensor | None = None, out: torch.Tensor | None = None
+               ) -> torch.Tensor:
+    """Keeps the accepted nodes of a drafted tree and returns the new lengths.
+
+    Row ``lens[b] + i`` becomes what row ``lens[b] + path[b, i]`` was, for i < ``counts[b]`` (the
+    whole path without ``counts``); path is int32 [batch, depth], depth <= 64, in any order.
+    Returns ``out`` (a new int32 [batch] tensor when not given, never ``lens`` itself):
+    ``lens + counts``.
+    """
+    at = _check_ints("lens", lens, (cache.batch,), cache)
+    if not isinstance(path, torch.Tensor) or path.dim() != 2:
+        raise ValueError("path must be int32 [batch, depth]")
+    to = _check_ints("path", path, (cache.batch, path.shape[1]), cache)
+    if out is None:
+        out = torch.empty_like(lens, memory_format=torch.contiguous_format)
+    _call(cache, _lib.load().wfattn_cache_keep, at, path.shape[1], to, path.stride(0),
+          _counts(counts, cache), _check_ints("out", out, (cache.batch,), cache))
+    return out
+
+
+def tree_decode(q: torch.Tensor, cache: KVCache, kv_lens: torch.Tensor, *,
+                tree: torch.Tensor | None = None, nodes: torch.Tensor | None = None,
+                scale: float | None = None, out: torch.Tensor | None = None,
+                workspace: DecodeWorkspace | None = None) -> torch.Tensor:
+    """Attention of a tree of drafted tokens over the cache; one token is a decode step.
+
+    q: [batch, heads_q, n, head_dim], n <= 64, heads_q a multiple of the cache's heads (query head
+    h reads cache head h // (heads_q // heads)); bf16 over a bf16, e4m3 or int4 cache, f32 over an
+    f32, e4m3 or int4 one.  Node j of sequence b is row ``kv_lens[b] + j`` of the cache.  Every node
+    sees the ``kv_lens[b]`` rows before the tree, and node i sees node j when bit j of
+    ``tree[b, i]`` is set (``tree_words``; int64 [batch, n], or [n] for one tree of all; without
+    it, nodes 0..i).  ``nodes`` (int32 [batch]) is how many of the n nodes each sequence has; the
+    rest is padding, and gives zeros like a node that sees nothing.  What a node does not see does
+    not reach its output, whatever it holds.
+
+    Returns [batch, heads_q, n, head_dim] of q's dtype (``out`` where given).
+    """
+    _require_cuda("q", q)
+    if q.dim() != 4:
+        raise ValueError(f"q must be [batch, heads_q, nodes, head_dim], got {tuple(q.shape)}")
+    b, hq, n, d = q.shape
+    _check_rows("q", q, (cache.batch, hq, n, cache.head_dim), q.dtype, cache)
+    if out is None:
+        out = torch.empty((b, hq, n, d), dtype=q.dtype, device=q.device)
+    else:
+        _check_rows("out", out, q.shape, q.dtype, cache)
+    at = _check_ints("kv_lens", kv_lens, (b,), cache)
+    words, words_stride = None, 0
+    if tree is not None:
+        shape = (n,) if isinstance(tree, torch.Tensor) and tree.dim() == 1 else (b, n)
+        words = _check_ints("tree", tree, shape, cache, torch.int64)
+        words_stride = 0 if tree.dim() == 1 else tree.stride(0)
+    lib = _lib.load()
+    dtype = _DTYPES[q.dtype]
+    nbytes = int(lib.wfattn_tree_decode_workspace_size(cache._ref, dtype, hq, n))
+    if nbytes == 0:
+        _lib.check_last(lib)
+    ws = (workspace or DecodeWorkspace()).get(nbytes, q.device)
+    count = None if nodes is None else _check_ints("nodes", nodes, (b,), cache)
+    _call(cache, lib.wfattn_tree_decode, dtype, hq, n, q.data_ptr(), _strides(q), at, words,
+          words_stride, count, out.data_ptr(), _strides(out), float(scale) if scale else 0.0,
+          ws.data_ptr(), ws.numel())
+    return out
+
+
+def tree_words(parents) -> torch.Tensor:
+    """The words of ``tree_decode`` for a tree given by each node's parent.
+
+    parents: [..., n] integers (a list or a tensor), n <= 64, the parent of node i an earlier node
+    or -1 where it follows the rows before the tree alone.  Every node sees itself and its
+    ancestors.  Returns int64 [..., n] on the CPU or the tensor's device.
+    """
+    parents = torch.as_tensor(parents, dtype=torch.int64)
+    n = parents.shape[-1] if parents.dim() else 0
+    if not 1 <= n <= MAX_NODES:
+        raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {n}")
+    index = torch.arange(n, device=parents.device)
+    if bool(((parents >= index) | (parents < -1)).any()):
+        raise ValueError("a node's parent is an earlier node, or -1")
+    bit = torch.ones((), dtype=torch.int64, device=parents.device) << index
+    words = torch.zeros_like(parents)
+    for i in range(n):
+        up = parents[..., i:i + 1]
+        above = words.gather(-1, up.clamp_min(0)).masked_fill(up < 0, 0)
+        words[..., i:i + 1] = above | bit[i]
+    return words

@@ -1,0 +1,85 @@
+// cache_format.cuh -- the row formats of a key/value cache (include/wfattn.h)
+// as the kernels see them.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/wfattn.h"
+#include "sm100_ptx.cuh"
+#include "wfattn_internal.h"
+
+namespace wfattn {
+
+// Bytes of a row of D values.
+template <int kFmt, int D>
+struct CacheRow {
+  static constexpr int kBytes = kFmt == WFATTN_CACHE_F32    ? 4 * D
+                                : kFmt == WFATTN_CACHE_BF16 ? 2 * D
+                                : kFmt == WFATTN_CACHE_E4M3 ? D
+                                                            : D / 2;
+  static constexpr bool kScaled = kFmt == WFATTN_CACHE_E4M3 || kFmt == WFATTN_CACHE_INT4;
+};
+
+namespace ptx {
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Two e4m3 codes (the low 16 bits of w) as f16x2: exact, NaN codes stay NaN.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)w));
+  return r;
+}
+
+// Two f32 as e4m3 codes (nearest even; |x| <= 448 here), lo in the low byte.
+__device__ __forceinline__ uint32_t pack_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ float2 f16x2_to_f32(uint32_t w) {
+  float2 f;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+      : "=f"(f.x), "=f"(f.y)
+      : "r"(w));
+  return f;
+}
+
+}  // namespace ptx
+
+// Eight consecutive values of a row as f32, from the row's eight codes at
+// `codes` (8 f32, 8 bf16, 8 bytes or 4 bytes) and its scale word.
+template <int kFmt>
+__device__ __forceinline__ void cache_load8(const uint8_t *codes, uint32_t scale, float (&f)[8]) {
+  if constexpr (kFmt == WFATTN_CACHE_F32) {
+    const float4 a = *reinterpret_cast<const float4 *>(codes);
+    const float4 b = *reinterpret_cast<const float4 *>(codes + 16);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
+    f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  } else if constexpr (kFmt == WFATTN_CACHE_BF16) {
+    const uint4 w = *reinterpret_cast<const uint4 *>(codes);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = ptx::bf16_lo(u[i]), f[2 * i + 1] = ptx::bf16_hi(u[i]);
+  } else if constexpr (kFmt == WFATTN_CACHE_E4M3) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(codes);
+    const float s = __uint_as_float(scale);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = ptx::f16x2_to_f32(ptx::e4m3x2_to_f16x2((i < 2 ? w.x : w.y) >> (16 * (i & 1))));
+      f[2 * i] = x.x * s, f[2 * i + 1] = x.y * s;
+    }
+  } else {
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(codes);
+    const float s = ptx::bf16_lo(scale), m = ptx::bf16_hi(scale);
+    // s u is exact in f32 (8 and 4 bits), so one rounding is left either way
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = fmaf(s, (float)((w >> (4 * i)) & 15u), m);
+  }
+}
+
+}  // namespace wfattn

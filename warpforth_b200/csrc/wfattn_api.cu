@@ -515,7 +515,254 @@ wfattn_status_t wfattn_device_status(void *stream, int clear) {
   if (word & kDevBadLengthMask)
     return fail(WFATTN_INVALID_ARG, "a kv_lens entry was outside [1, max_kv_len] (status 0x%x)",
                 word);
+  if (word & kDevBadRowMask)
+    return fail(WFATTN_INVALID_ARG,
+                "a cache call's length, count or row position was out of range (status 0x%x)",
+                word);
   return WFATTN_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Checks a cache description and turns it into the kernels' view of it.
+wfattn_status_t check_cache(const wfattn_cache_t *c, CacheView *out) {
+  if (!c) return fail(WFATTN_INVALID_ARG, "null cache");
+  if (c->format < WFATTN_CACHE_F32 || c->format > WFATTN_CACHE_INT4)
+    return fail(WFATTN_INVALID_ARG, "unknown cache format %d", (int)c->format);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(WFATTN_UNSUPPORTED, "caches support head_dim 64 and 128 (got %d)",
+                (int)c->head_dim);
+  if (c->batch < 1 || c->heads < 1 || c->max_len < 1)
+    return fail(WFATTN_INVALID_ARG, "cache sizes must be >= 1");
+  int64_t bh = 0, rows = 0;
+  if (__builtin_mul_overflow(c->batch, c->heads, &bh) ||
+      __builtin_mul_overflow(bh, c->max_len, &rows) || rows > INT32_MAX)
+    return fail(WFATTN_INVALID_ARG, "a cache holds at most 2^31-1 rows");
+  const bool scaled = c->format == WFATTN_CACHE_E4M3 || c->format == WFATTN_CACHE_INT4;
+  if (!c->k || !c->v || (scaled && (!c->k_scale || !c->v_scale)))
+    return fail(WFATTN_INVALID_ARG, "null cache pointer");
+  if (!aligned(c->k, 16) || !aligned(c->v, 16))
+    return fail(WFATTN_INVALID_ARG, "cache rows must be 16-byte aligned");
+  if (scaled && (!aligned(c->k_scale, 4) || !aligned(c->v_scale, 4)))
+    return fail(WFATTN_INVALID_ARG, "cache scales must be 4-byte aligned");
+  const int64_t sb = c->batch == 1 ? 0 : c->batch_stride, sh = c->heads == 1 ? 0 : c->head_stride;
+  constexpr int64_t kMaxStride = int64_t(1) << 40;  // keeps byte offsets inside 64 bits
+  if (sb < 0 || sh < 0 || sb > kMaxStride || sh > kMaxStride)
+    return fail(WFATTN_INVALID_ARG, "cache strides must be in [0, 2^40] rows");
+  // the rows of one head, then of the inner of batch and head, then of the outer
+  const bool head_inner = (c->heads == 1 || sh >= c->max_len) &&
+                          (c->batch == 1 || sb >= (c->heads - 1) * sh + c->max_len);
+  const bool batch_inner = (c->batch == 1 || sb >= c->max_len) &&
+                           (c->heads == 1 || sh >= (c->batch - 1) * sb + c->max_len);
+  if (!head_inner && !batch_inner) return fail(WFATTN_INVALID_ARG, "cache rows overlap");
+  out->format = c->format;
+  out->D = c->head_dim;
+  out->B = c->batch;
+  out->H = c->heads;
+  out->L = c->max_len;
+  out->sb = sb;
+  out->sh = sh;
+  out->k = static_cast<uint8_t *>(c->k);
+  out->v = static_cast<uint8_t *>(c->v);
+  out->k_scale = scaled ? static_cast<uint8_t *>(c->k_scale) : nullptr;
+  out->v_scale = scaled ? static_cast<uint8_t *>(c->v_scale) : nullptr;
+  return WFATTN_OK;
+}
+
+wfattn_status_t sm100_device(DeviceInfo *dev) {
+  const wfattn_status_t st = current_device(dev);
+  if (st != WFATTN_OK) return st;
+  if (!is_sm100(*dev))
+    return fail(WFATTN_UNSUPPORTED, "libwfattn is built for sm_100a; device %d is sm_%d%d",
+                dev->device, dev->cc_major, dev->cc_minor);
+  return WFATTN_OK;
+}
+
+wfattn_status_t check_dtype(int dtype, const void *a, const void *b) {
+  if (dtype != WFATTN_DTYPE_F32 && dtype != WFATTN_DTYPE_BF16)
+    return fail(WFATTN_INVALID_ARG, "unknown dtype %d", dtype);
+  const uintptr_t size = dtype == WFATTN_DTYPE_F32 ? 4 : 2;
+  if (!aligned(a, size) || !aligned(b, size))
+    return fail(WFATTN_INVALID_ARG, "tensors must be aligned to their elements");
+  return WFATTN_OK;
+}
+
+// Checks shared by cache_write and cache_read; n_rows 0 leaves *a unset.
+wfattn_status_t prepare_rows(const wfattn_cache_t *cache, int dtype, int64_t n_rows, void *k,
+                             const int64_t *k_strides, void *v, const int64_t *v_strides,
+                             const int32_t *starts, const int32_t *counts, CacheRowsArgs *a) {
+  wfattn_status_t st = check_cache(cache, &a->c);
+  if (st != WFATTN_OK) return st;
+  if (n_rows < 0 || n_rows > a->c.L)
+    return fail(WFATTN_INVALID_ARG, "n_rows must be in [0, max_len = %lld] (got %lld)",
+                (long long)a->c.L, (long long)n_rows);
+  if (n_rows > 0 && (!k || !v || !starts)) return fail(WFATTN_INVALID_ARG, "null tensor pointer");
+  st = check_dtype(dtype, k, v);
+  if (st != WFATTN_OK) return st;
+  a->f32 = dtype == WFATTN_DTYPE_F32;
+  a->n = n_rows;
+  a->k = k;
+  a->v = v;
+  a->ks = resolve_strides(k_strides, a->c.H, n_rows, a->c.D);
+  a->vs = resolve_strides(v_strides, a->c.H, n_rows, a->c.D);
+  if (!strides_ok(a->ks) || !strides_ok(a->vs)) return fail(WFATTN_INVALID_ARG, "negative stride");
+  a->starts = starts;
+  a->counts = counts;
+  return WFATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+wfattn_status_t wfattn_cache_write(const wfattn_cache_t *cache, int dtype, int64_t n_rows,
+                                   const void *k, const int64_t *k_strides, const void *v,
+                                   const int64_t *v_strides, const int32_t *starts,
+                                   const int32_t *counts, void *stream) {
+  t_last_error.clear();
+  CacheRowsArgs a;
+  wfattn_status_t st = prepare_rows(cache, dtype, n_rows, const_cast<void *>(k), k_strides,
+                                    const_cast<void *>(v), v_strides, starts, counts, &a);
+  if (st != WFATTN_OK || n_rows == 0) return st;
+  DeviceInfo dev;
+  st = sm100_device(&dev);
+  if (st != WFATTN_OK) return st;
+  const cudaError_t err = launch_cache_write(a, dev, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? WFATTN_OK : cuda_fail(err, "cache_write launch");
+}
+
+wfattn_status_t wfattn_cache_read(const wfattn_cache_t *cache, int dtype, int64_t n_rows, void *k,
+                                  const int64_t *k_strides, void *v, const int64_t *v_strides,
+                                  const int32_t *starts, const int32_t *counts, int zero_rest,
+                                  void *stream) {
+  t_last_error.clear();
+  CacheRowsArgs a;
+  wfattn_status_t st = prepare_rows(cache, dtype, n_rows, k, k_strides, v, v_strides, starts,
+                                    counts, &a);
+  if (st != WFATTN_OK || n_rows == 0) return st;
+  a.zero_rest = zero_rest != 0;
+  const int64_t ext[3] = {a.c.B, a.c.H, n_rows}, sk[3] = {a.ks.b, a.ks.h, a.ks.s},
+                sv[3] = {a.vs.b, a.vs.h, a.vs.s};
+  for (int i = 0; i < 3; ++i)
+    if (ext[i] > 1 && (sk[i] == 0 || sv[i] == 0))
+      return fail(WFATTN_INVALID_ARG, "cache_read does not write broadcast (zero) strides");
+  DeviceInfo dev;
+  st = sm100_device(&dev);
+  if (st != WFATTN_OK) return st;
+  const cudaError_t err = launch_cache_read(a, dev, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? WFATTN_OK : cuda_fail(err, "cache_read launch");
+}
+
+wfattn_status_t wfattn_cache_keep(const wfattn_cache_t *cache, const int32_t *lens, int64_t depth,
+                                  const int32_t *path, int64_t path_stride, const int32_t *counts,
+                                  int32_t *new_lens, void *stream) {
+  t_last_error.clear();
+  CacheKeepArgs a;
+  wfattn_status_t st = check_cache(cache, &a.c);
+  if (st != WFATTN_OK) return st;
+  if (!lens || !path || !new_lens) return fail(WFATTN_INVALID_ARG, "null tensor pointer");
+  const char *from = reinterpret_cast<const char *>(lens), *to = reinterpret_cast<char *>(new_lens);
+  if (from < to + 4 * a.c.B && to < from + 4 * a.c.B)
+    return fail(WFATTN_INVALID_ARG, "new_lens must be another array than lens");
+  if (depth < 1 || depth > kMaxTreeNodes)
+    return fail(WFATTN_INVALID_ARG, "depth must be in [1, %d] (got %lld)", kMaxTreeNodes,
+                (long long)depth);
+  if (path_stride < 0) return fail(WFATTN_INVALID_ARG, "negative stride");
+  a.lens = lens;
+  a.path = path;
+  a.counts = counts;
+  a.depth = (int)depth;
+  a.path_stride = path_stride;
+  a.new_lens = new_lens;
+  DeviceInfo dev;
+  st = sm100_device(&dev);
+  if (st != WFATTN_OK) return st;
+  const cudaError_t err = launch_cache_keep(a, dev, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? WFATTN_OK : cuda_fail(err, "cache_keep launch");
+}
+
+}  // extern "C"
+
+namespace {
+
+wfattn_status_t check_tree(const wfattn_cache_t *cache, int dtype, int64_t heads_q, int64_t nodes,
+                           TreeDecodeArgs *a) {
+  wfattn_status_t st = check_cache(cache, &a->c);
+  if (st != WFATTN_OK) return st;
+  st = check_dtype(dtype, nullptr, nullptr);
+  if (st != WFATTN_OK) return st;
+  a->f32 = dtype == WFATTN_DTYPE_F32;
+  if (a->c.format == (a->f32 ? WFATTN_CACHE_BF16 : WFATTN_CACHE_F32))
+    return fail(WFATTN_UNSUPPORTED, "tree_decode takes a plain cache with queries of its own type");
+  if (nodes < 1 || nodes > kMaxTreeNodes)
+    return fail(WFATTN_INVALID_ARG, "nodes must be in [1, %d] (got %lld)", kMaxTreeNodes,
+                (long long)nodes);
+  int64_t rows = 0;
+  if (heads_q < 1 || heads_q % a->c.H || __builtin_mul_overflow(heads_q, a->c.B * nodes, &rows) ||
+      rows > INT32_MAX)
+    return fail(WFATTN_INVALID_ARG,
+                "heads_q must be a multiple of the cache's %lld heads, with at most 2^31-1 rows "
+                "of queries (got %lld heads)", (long long)a->c.H, (long long)heads_q);
+  a->Hq = heads_q;
+  a->T = (int)nodes;
+  return WFATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t wfattn_tree_decode_workspace_size(const wfattn_cache_t *cache, int dtype, int64_t heads_q,
+                                         int64_t nodes) {
+  t_last_error.clear();
+  TreeDecodeArgs a;
+  if (check_tree(cache, dtype, heads_q, nodes, &a) != WFATTN_OK) return 0;
+  return tree_decode_workspace_bytes(a.c, a.f32, a.Hq, a.T);
+}
+
+wfattn_status_t wfattn_tree_decode(const wfattn_cache_t *cache, int dtype, int64_t heads_q,
+                                   int64_t nodes, const void *q, const int64_t *q_strides,
+                                   const int32_t *lens, const uint64_t *tree, int64_t tree_stride,
+                                   const int32_t *counts, void *o, const int64_t *o_strides,
+                                   float scale, void *workspace, size_t workspace_bytes,
+                                   void *stream) {
+  t_last_error.clear();
+  TreeDecodeArgs a;
+  wfattn_status_t st = check_tree(cache, dtype, heads_q, nodes, &a);
+  if (st != WFATTN_OK) return st;
+  if (!q || !o || !lens) return fail(WFATTN_INVALID_ARG, "null tensor pointer");
+  st = check_dtype(dtype, q, o);
+  if (st != WFATTN_OK) return st;
+  if (!aligned(lens, 4) || !aligned(counts, 4) || !aligned(tree, 8))
+    return fail(WFATTN_INVALID_ARG, "lens, counts and tree must be aligned to their elements");
+  if (tree_stride < 0) return fail(WFATTN_INVALID_ARG, "negative stride");
+  if (!(scale == scale)) return fail(WFATTN_INVALID_ARG, "scale is NaN");
+  a.q = q;
+  a.o = o;
+  a.qs = resolve_strides(q_strides, heads_q, nodes, a.c.D);
+  a.os = resolve_strides(o_strides, heads_q, nodes, a.c.D);
+  if (!strides_ok(a.qs) || !strides_ok(a.os)) return fail(WFATTN_INVALID_ARG, "negative stride");
+  if ((a.c.B > 1 && a.os.b == 0) || (heads_q > 1 && a.os.h == 0) || (nodes > 1 && a.os.s == 0))
+    return fail(WFATTN_INVALID_ARG, "the output does not take zero (broadcast) strides");
+  a.lens = lens;
+  a.counts = counts;
+  a.tree = tree;
+  a.tree_stride = tree_stride;
+  a.scale = resolve_scale(scale, a.c.D);
+  const size_t need = tree_decode_workspace_bytes(a.c, a.f32, a.Hq, a.T);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(WFATTN_INVALID_ARG, "a 16-byte aligned workspace of %zu bytes needed, %zu given",
+                need, workspace ? workspace_bytes : (size_t)0);
+  a.workspace = workspace;
+  DeviceInfo dev;
+  st = sm100_device(&dev);
+  if (st != WFATTN_OK) return st;
+  const cudaError_t err = launch_tree_decode(a, dev, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? WFATTN_OK : cuda_fail(err, "tree_decode launch");
 }
 
 // Peer buffers: plain cudaMalloc memory exported and imported with CUDA IPC

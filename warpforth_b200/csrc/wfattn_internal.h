@@ -12,6 +12,7 @@ namespace wfattn {
 enum DeviceStatusBits : unsigned int {
   kDevTimeoutMask = 1u,
   kDevBadLengthMask = 2u,  // a device-side length (decode kv_lens) was out of range
+  kDevBadRowMask = 4u,     // a cache call's length, count or row position was out of range
 };
 
 __host__ __device__ __forceinline__ int64_t imin64(int64_t a, int64_t b) { return a < b ? a : b; }
@@ -94,5 +95,58 @@ cudaError_t launch_decode(const DecodeArgs &a, const DeviceInfo &dev, cudaStream
 constexpr size_t kDecodeNoAllocScratchBytes = size_t(8) << 20;
 // Device address of that scratch on the current device (looked up on first use).
 cudaError_t decode_noalloc_scratch(void **ptr);
+
+// ---- key/value caches (row formats: include/wfattn.h)
+
+struct CacheView {
+  int format;  // wfattn_cache_format_t
+  int D;       // 64 or 128
+  int64_t B, H, L;
+  int64_t sb, sh;  // strides in rows
+  uint8_t *k, *v;
+  uint8_t *k_scale, *v_scale;
+};
+
+// Rows of new keys and values, or room for read ones.
+struct CacheRowsArgs {
+  CacheView c;
+  bool f32;  // the rows are f32 (else bf16)
+  int64_t n;
+  void *k, *v;
+  Strides3 ks, vs;
+  const int32_t *starts, *counts;
+  bool zero_rest = false;  // reading: the other rows become zeros
+};
+cudaError_t launch_cache_write(const CacheRowsArgs &a, const DeviceInfo &dev, cudaStream_t stream);
+cudaError_t launch_cache_read(const CacheRowsArgs &a, const DeviceInfo &dev, cudaStream_t stream);
+
+constexpr int kMaxTreeNodes = 64;
+
+struct CacheKeepArgs {
+  CacheView c;
+  const int32_t *lens, *path, *counts;
+  int depth;  // 1..kMaxTreeNodes
+  int64_t path_stride;
+  int32_t *new_lens;
+};
+cudaError_t launch_cache_keep(const CacheKeepArgs &a, const DeviceInfo &dev, cudaStream_t stream);
+
+struct TreeDecodeArgs {
+  CacheView c;
+  bool f32;    // q and o are f32 (else bf16)
+  int64_t Hq;  // a multiple of c.H
+  int T;       // 1..kMaxTreeNodes
+  const void *q;
+  void *o;
+  Strides3 qs, os;  // s: node stride
+  const int32_t *lens, *counts;
+  const uint64_t *tree;
+  int64_t tree_stride;
+  float scale;
+  void *workspace;
+};
+size_t tree_decode_workspace_bytes(const CacheView &c, bool f32, int64_t Hq, int T);
+cudaError_t launch_tree_decode(const TreeDecodeArgs &a, const DeviceInfo &dev,
+                               cudaStream_t stream);
 
 }  // namespace wfattn
