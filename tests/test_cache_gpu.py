@@ -9,6 +9,11 @@ p |v| over the keys, S = scale * max over the keys of sum |q k|, n keys:
 * weights are exp2 of at most a few units of 2^-22, kept in f32 for the total and, for the products
   with bf16 queries, in 16 bits: 2^-11 (f16 beside quantised rows; bf16 rows take two bf16 terms),
   with f32 queries in two terms: 2^-21;
+* f16 weights (beside quantised rows) are p s / s_top 2^7 or more, s_top being the largest row scale,
+  and below 2^-14 they are held in steps of 2^-24: off by 2^-25 each, with a total of weights >= 1
+  and codes c (e4m3 codes; u - 8) of |c| s_top <= 2.2 max |v| (e4m3: 448 s < 2 * 2 * 224 s / 2 and
+  max |x| > 224 s; int4: 8 s <= 8/15 (1 + 2^-7) times a span of at most 2 max |v|).  The sum is off
+  by at most n 2^-25 2^-7 2.2 max |v| < n 2^-30 max |v|;
 * the sum over n keys adds n / 16 matrix products in f32: 2^-23 each;
 * the output is rounded once: 2^-8 |o| in bf16, 2^-24 |o| in f32.
 
@@ -144,6 +149,8 @@ def attend(fmt, cache, q, lens, words, nodes, scale=None):
                 e = 2 * (d + 3) * 2.0 ** -23 * big + (len(sees) / 16 + 64) * 2.0 ** -23
                 e += 2.0 ** -21 if f32 else 2.0 ** -11
                 tol[i, h, t] = e * (p @ size[i, h // g, sees])
+                if fmt not in TYPES:
+                    tol[i, h, t] += len(sees) * 2.0 ** -30 * np.abs(vv).max()
     return out, tol + np.abs(out) * (2.0 ** -24 if f32 else 2.0 ** -8)
 
 

@@ -37,9 +37,11 @@ NVCC_FLAGS = [
 ]
 SOURCES = ["wfattn_api.cu", "attn_f32.cu", "attn_f32_tc_sm100.cu", "attn_bf16_sm100.cu",
            "attn_bf16_2q_sm100.cu", "decode_sm100.cu", "cache_sm100.cu",
-           "tree_decode_sm100.cu", "tma_map.cu"]
+           "tree_decode_sm100.cu", "tree_decode_f32_f32.cu", "tree_decode_bf16_bf16.cu",
+           "tree_decode_e4m3_bf16.cu", "tree_decode_e4m3_f32.cu", "tree_decode_int4_bf16.cu",
+           "tree_decode_int4_f32.cu", "tma_map.cu"]
 HEADERS = ["wfattn_internal.h", "sm100_ptx.cuh", "tma_map.h", "exp2_poly.cuh",
-           "cache_format.cuh"]
+           "cache_format.cuh", "tree_decode.cuh"]
 
 
 def nvcc() -> str:

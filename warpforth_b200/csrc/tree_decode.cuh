@@ -1,0 +1,1181 @@
+// tree_decode.cuh -- the split kernel of tree_decode (include/wfattn.h), one
+// instantiation a row format, head size, query type and number of query rows.
+//
+// The rows of queries that share one cache head, R = heads_q / heads * nodes,
+// are attended together, so every cache row is read once for all of them.  The
+// kernel works on transposed products, whose narrow side (8) holds queries:
+//
+//   S^T [16 keys x 8 queries] = K [16 x D] Q^T [D x 8]
+//   O^T [D x 8 queries]      += V^T [D x 16 keys] P^T [16 x 8]
+//
+// with mma.sync: rows of K and V go from shared memory through a conversion in
+// registers (codes to f16; nothing is written back), which tcgen05 operands in
+// shared or tensor memory would need a round trip for, and a step has 8 to 64
+// query rows where a tcgen05 tile has 128.  Products:
+//  * e4m3 / int4 rows: the codes (int4: u - 8) are exact in f16; scale and
+//    minimum of a row are applied to the f32 score and to the f32 weight;
+//  * bf16 rows: bf16 products, the weights as two bf16 terms (16 bits);
+//  * f32 rows: tf32 products of two-term splits (hi hi, hi lo, lo hi), and
+//    with f32 queries over quantised rows Q and P as two f16 terms: ~2^-21.
+// Queries are scaled by a power of two into f16's upper range, weights are
+// taken as p <= 2^4 times the row's scale over the running largest scale, also
+// in f16's range; sums, maxima and all other arithmetic are f32.
+//
+// Softmax is online with a lazy maximum: weights are 2^(s - m) for a reference
+// m that is raised (and the sums rescaled) only when a score passes m + 4, so
+// most tiles pay one vote instead of the maximum's shuffles.
+//
+// Work: a unit is kKeys keys of one (sequence, cache head, tile of query
+// rows); the units of all sequences in order are dealt in equal contiguous
+// shares to a grid of kCtas CTAs an SM, whatever the lengths.  A CTA streams
+// its units through a ring of cp.async stages without regard to where a
+// segment (one sequence, head and tile) ends; a segment that lies in one CTA
+// is written out directly, the others as partials (maximum, sum, unnormalised
+// output) that a second kernel joins in order: no atomics, the same bits every
+// time.  Four warps split the keys of a unit or, with more rows, the rows.
+#pragma once
+
+#include <float.h>
+#include <math.h>
+
+#include "cache_format.cuh"
+
+namespace wfattn {
+namespace tree {
+
+constexpr int kThreads = 128, kWarps = 4;
+constexpr int kMaxSms = 148;  // CTAs are dealt for at most this many SMs
+
+// Per CTA, written by every launch before the joining kernel reads it.
+struct Desc {
+  int64_t seg;  // segment that begins in this CTA and goes on in later ones, or -1
+  int32_t last;  // its last CTA
+  int32_t head;  // 1: the CTA's first piece is a partial (slot 0)
+};
+
+struct Params {
+  CacheView c;
+  int64_t HR;    // segments a sequence: heads * row tiles
+  int RT;        // row tiles a head
+  int R, G, T;   // query rows a head = G heads x T nodes
+  int ctas;      // of the grid
+  const uint8_t *q;
+  uint8_t *o;
+  Strides3 qs, os;
+  const int32_t *lens, *counts;
+  const uint64_t *tree;
+  int64_t tree_stride;
+  float scale_log2;
+  Desc *desc;
+  float *part;   // [ctas][2][rows][D], then [ctas][2][rows][2]
+  unsigned int *status;
+};
+
+enum Kind { kF16, kBf16, kTf32 };
+
+template <int kFmt_, int D_, bool kF32_, int kNT_, int kRW_>
+struct Cfg {
+  static constexpr int kFmt = kFmt_, D = D_, kNT = kNT_, kRW = kRW_, kKW = kWarps / kRW_;
+  static constexpr bool kF32 = kF32_;  // queries and output
+  static constexpr Kind kKind = kFmt == WFATTN_CACHE_F32    ? kTf32
+                                : kFmt == WFATTN_CACHE_BF16 ? kBf16
+                                                            : kF16;
+  static constexpr bool kScaled = CacheRow<kFmt, D>::kScaled;
+  static constexpr int kRowBytes = CacheRow<kFmt, D>::kBytes;
+  static constexpr int kRows = 8 * kNT * kRW;               // query rows of a CTA
+  static constexpr int kKeys = kRowBytes <= 64 ? 128 : 64;  // keys of a unit
+  static constexpr int kKBytes = kKeys * kRowBytes;
+  static constexpr int kStage = 2 * kKBytes + (kScaled ? 8 * kKeys : 0);
+  static constexpr int kOStride = D + 2;  // floats a row of the merge buffer
+  static constexpr int kMerge = kKW > 1 ? kWarps * 8 * kNT * kOStride * 4 : 0;
+  static constexpr int kStats = kWarps * 8 * kNT * 2 * 4;
+  static constexpr int kCtas = kRowBytes >= 512 ? 1 : kRowBytes == 256 ? 2 : kNT * D <= 64 ? 4 : 3;
+  static constexpr int kBudget = 227 * 1024 / kCtas - 2048;
+  static constexpr int kFit = (kBudget - kMerge - kStats) / kStage;
+  static constexpr int kStages = kFit > 6 ? 6 : kFit;
+  static_assert(kStages >= 2, "shared memory budget");
+  static constexpr int kSmem = kStages * kStage + kMerge + kStats;
+  static constexpr int kTiles = kKeys / 16 / kKW;  // 16-key tiles of a warp in a unit
+  static constexpr int kMt = D / 16;               // row tiles of O^T
+};
+
+// ------------------------------------------------------------- instructions
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(live ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+               "r"(live ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+template <bool kTrans>
+__device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&r)[4]) {
+  if constexpr (kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a));
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a));
+}
+// The 8x8 matrix of 16-bit elements held by the warp, transposed.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+template <Kind kKind>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                    uint32_t b1) {
+  if constexpr (kKind == kF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else if constexpr (kKind == kBf16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// (x & kMask) | kBits in one operation
+template <uint32_t kMask, uint32_t kBits>
+__device__ __forceinline__ uint32_t and_or(uint32_t x) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "n"(kMask), "n"(kBits));
+  return r;
+}
+// 4-bit codes number 0 and 4 (kOdd: 1 and 5) of w as the f16x2 u - 8: a code
+// put below f16's 1024 (above 64's sixteenths) reads 1024 + u (64 + u), exactly.
+template <bool kOdd>
+__device__ __forceinline__ uint32_t int4_f16x2(uint32_t w) {
+  return kOdd ? hsub2(and_or<0x00f000f0u, 0x54005400u>(w), 0x54805480u)
+              : hsub2(and_or<0x000f000fu, 0x64006400u>(w), 0x64086408u);
+}
+// f32 as tf32 terms: the upper 10 fraction bits, and what is left (exact; the
+// product unit takes its upper bits)
+__device__ __forceinline__ uint32_t tf32_hi(uint32_t x) { return x & 0xffffe000u; }
+__device__ __forceinline__ uint32_t tf32_lo(uint32_t x) {
+  return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u));
+}
+
+// ----------------------------------------------------------------- layouts
+
+// Byte offset `o` of row `r` in a stage's K or V: 16-byte pieces are permuted
+// inside 128-byte lines so that the loads of a fragment (8 rows, or 4 row
+// pairs, at one offset) fall into different banks.
+template <class C>
+__device__ __forceinline__ uint32_t swizzle(uint32_t r, uint32_t o) {
+  const uint32_t x = C::kKind == kBf16    ? r & 7
+                     : C::kRowBytes >= 128 ? (r & 6) ^ ((r & 1) << 2)
+                     : C::kRowBytes == 64  ? r & 6
+                                           : (r >> 1) & 2;
+  return (r * C::kRowBytes + o) ^ (x << 4);
+}
+
+// Which value of the row the element e of product step s, lane column t, is:
+// steps are 16 values (4 elements a lane) or, for tf32, 8 (2 elements).
+template <class C>
+__device__ __forceinline__ int q_index(int s, int t, int e) {
+  if constexpr (C::kKind == kBf16) return 16 * s + 2 * t + (e & 1) + 8 * (e >> 1);
+  if constexpr (C::kKind == kTf32) return 4 * (4 * (s >> 1) + t) + 2 * (s & 1) + e;
+  if constexpr (C::kFmt == WFATTN_CACHE_E4M3)
+    return 16 * (t + 4 * (s >> 2)) + 4 * (s & 3) + e;
+  // int4: codes n and n + 4 of a word make a pair
+  const int n = 2 * (s & 1) + (e >> 1);
+  return (C::D / 4) * t + 8 * (s >> 1) + n + 4 * (e & 1);
+}
+
+// Which value the row g (r = 0) or g + 8 (r = 1) of O^T's tile mt is.
+template <class C>
+__device__ __forceinline__ int o_index(int mt, int g, int r) {
+  if constexpr (C::kKind == kBf16) return 16 * mt + g + 8 * r;
+  if constexpr (C::kKind == kTf32) return 4 * (g + 8 * (mt >> 1)) + 2 * (mt & 1) + r;
+  return (C::D / 8) * g + 2 * mt + r;
+}
+
+// One value of a V row in a stage, unscaled (used where a row is not finite).
+template <class C>
+__device__ __forceinline__ float v_value(uint32_t v, int row, int d) {
+  if constexpr (C::kFmt == WFATTN_CACHE_F32) {
+    return __uint_as_float(lds32(v + swizzle<C>(row, 4 * d)));
+  } else if constexpr (C::kFmt == WFATTN_CACHE_BF16) {
+    const uint32_t w = lds32(v + swizzle<C>(row, 2 * (d & ~1)));
+    return d & 1 ? ptx::bf16_hi(w) : ptx::bf16_lo(w);
+  } else {
+    const uint32_t w = lds32(v + swizzle<C>(row, d & ~3)) >> (8 * (d & 3));
+    return ptx::f16x2_to_f32(ptx::e4m3x2_to_f16x2(w & 0xff)).x;
+  }
+}
+
+// -------------------------------------------------------------- work order
+
+struct Seq {
+  int64_t len, total;  // rows before the tree, rows in all
+  int n;               // nodes
+  int64_t units;       // of one segment, at least 1
+};
+
+template <int kKeys>
+__device__ __forceinline__ Seq sequence(const Params &p, int64_t b, bool report) {
+  Seq s;
+  int64_t len = p.lens[b], n = p.counts ? p.counts[b] : p.T;
+  bool bad = len < 0 || n < 0 || n > p.T;
+  len = len < 0 ? 0 : len;
+  n = n < 0 ? 0 : n > p.T ? p.T : n;
+  bad = bad || len + n > p.c.L;
+  len = imin64(len, p.c.L);
+  n = imin64(n, p.c.L - len);
+  if (bad && report) atomicOr(p.status, kDevBadRowMask);
+  s.len = len;
+  s.n = (int)n;
+  s.total = len + n;
+  s.units = imax64(1, (s.total + kKeys - 1) / kKeys);
+  return s;
+}
+
+// A position in the order of units.
+template <int kKeys>
+struct Cursor {
+  int64_t b, hr, u;
+  Seq s;
+  __device__ __forceinline__ void next(const Params &p) {
+    if (++u < s.units) return;
+    u = 0;
+    if (++hr < p.HR) return;
+    hr = 0;
+    if (++b < p.c.B) s = sequence<kKeys>(p, b, false);
+  }
+};
+
+// Finds this CTA's share [begin, end) of the units and where it begins.
+template <int kKeys>
+__device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, int64_t &end,
+                                               int64_t &all) {
+  __shared__ int64_t warp_sum[kWarps], found[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t per = (p.c.B + kThreads - 1) / kThreads;
+  const int64_t b0 = imin64(p.c.B, threadIdx.x * per), b1 = imin64(p.c.B, b0 + per);
+  int64_t mine = 0;
+  for (int64_t b = b0; b < b1; ++b) mine += sequence<kKeys>(p, b, blockIdx.x == 0).units * p.HR;
+  int64_t upto = mine;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, upto, x);
+    if (lane >= x) upto += y;
+  }
+  if (lane == 31) warp_sum[warp] = upto;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) upto += warp_sum[w];
+    all += warp_sum[w];
+  }
+  begin = all * blockIdx.x / p.ctas;
+  end = all * (blockIdx.x + 1) / p.ctas;
+  if (begin >= upto - mine && begin < upto) {
+    int64_t at = upto - mine, b = b0;
+    for (;; ++b) {
+      const int64_t n = sequence<kKeys>(p, b, false).units * p.HR;
+      if (begin < at + n) break;
+      at += n;
+    }
+    found[0] = b;
+    found[1] = begin - at;
+  }
+  __syncthreads();
+  Cursor<kKeys> c;
+  c.b = found[0];
+  c.s = sequence<kKeys>(p, c.b, false);
+  c.hr = found[1] / c.s.units;
+  c.u = found[1] - c.hr * c.s.units;
+  return c;
+}
+
+// ------------------------------------------------------------------ kernel
+
+template <class C>
+struct Warp {
+  // fragments of the queries, and of the output
+  static constexpr int kSteps = C::kKind == kTf32 ? C::D / 8 : C::D / 16;
+  static constexpr int kQTerms = C::kKind == kF16 && C::kF32 ? 2 : 1;
+  uint32_t q[C::kNT][kSteps][2 * kQTerms];
+  float o[C::kNT][C::kMt][4];
+  // per query 2t, 2t + 1 of each n-tile
+  float qf[C::kNT][2], qsum[C::kNT][2];
+  uint64_t word[C::kNT][2];
+  float m[C::kNT][2], l[C::kNT][2], om[C::kNT][2];
+  float vinv;  // weights carry scale * vinv
+
+  // Loads the query rows `row0`.. of cache head h of sequence b.
+  __device__ __forceinline__ void load_q(const Params &p, int64_t b, int64_t h, int row0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < C::kNT; ++nt) {
+      const int r = row0 + 8 * nt + g;
+      float x[kSteps][C::kKind == kTf32 ? 2 : 4];
+      constexpr int kE = C::kKind == kTf32 ? 2 : 4;
+      float top = 0.f, sum = 0.f;
+      if (r < p.R) {
+        const int hg = r / p.T, node = r - hg * p.T;
+        const int64_t at = b * p.qs.b + (h * p.G + hg) * p.qs.h + node * p.qs.s;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int e = 0; e < kE; ++e) {
+            const int64_t i = at + q_index<C>(s, t, e);
+            x[s][e] = C::kF32 ? reinterpret_cast<const float *>(p.q)[i]
+                              : ptx::bf16_lo(reinterpret_cast<const uint16_t *>(p.q)[i]);
+          }
+      } else {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int e = 0; e < kE; ++e) x[s][e] = 0.f;
+      }
+      float mul = 1.f;
+      if constexpr (C::kKind == kF16) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[s][e]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^14 <= top * mul < 2^15
+        const int f = min(max(268 - (int)(__float_as_uint(top) >> 23), 1), 253);
+        mul = __uint_as_float((uint32_t)f << 23);
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if constexpr (C::kKind == kTf32) {
+          q[nt][s][0] = __float_as_uint(x[s][0]);
+          q[nt][s][1] = __float_as_uint(x[s][1]);
+        } else if constexpr (C::kKind == kBf16) {
+          q[nt][s][0] = ptx::pack_bf16x2(x[s][0], x[s][1]);
+          q[nt][s][1] = ptx::pack_bf16x2(x[s][2], x[s][3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[s][e] *= mul;
+            sum += x[s][e];
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            q[nt][s][i] = pack_f16x2(x[s][2 * i], x[s][2 * i + 1]);
+            if constexpr (kQTerms == 2) {
+              const float2 hi = ptx::f16x2_to_f32(q[nt][s][i]);
+              q[nt][s][2 + i] = pack_f16x2(x[s][2 * i] - hi.x, x[s][2 * i + 1] - hi.y);
+            }
+          }
+        }
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const float f = p.scale_log2 / mul;  // a power of two: exact
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // from query g to queries 2t, 2t + 1
+        qf[nt][i] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + i));
+        qsum[nt][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i));
+        const int rr = row0 + 8 * nt + 2 * t + i, node = rr % p.T;
+        word[nt][i] = p.tree ? p.tree[b * p.tree_stride + node] : (2ull << node) - 1;
+        m[nt][i] = -FLT_MAX;
+        l[nt][i] = om[nt][i] = 0.f;
+      }
+#pragma unroll
+      for (int mt = 0; mt < C::kMt; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
+    }
+    vinv = __uint_as_float(253u << 23);  // 2^126
+  }
+
+  // Attends to the 16 keys of rows tr.. of a stage (k, v, scales), key0 their
+  // position.  kTail: some of them are nodes of the tree, or no keys.
+  template <bool kTail>
+  __device__ __forceinline__ void tile(uint32_t k, uint32_t v, uint32_t scales, int tr,
+                                       int64_t key0, const Seq &seq) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float c[C::kNT][4];
+#pragma unroll
+    for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[nt][e] = 0.f;
+
+    // ---- S^T = K Q^T
+    if constexpr (C::kKind == kBf16) {
+      const int row = tr + (lane & 15);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        uint32_t a[4];
+        ldmatrix4<false>(k + swizzle<C>(row, 32 * s + 16 * (lane >> 4)), a);
+#pragma unroll
+        for (int nt = 0; nt < C::kNT; ++nt) mma<kBf16>(c[nt], a, q[nt][s][0], q[nt][s][1]);
+      }
+    } else if constexpr (C::kKind == kTf32) {
+#pragma unroll
+      for (int j = 0; j < C::D / 16; ++j) {
+        const uint4 x0 = lds128(k + swizzle<C>(tr + g, 16 * (4 * j + t)));
+        const uint4 x1 = lds128(k + swizzle<C>(tr + g + 8, 16 * (4 * j + t)));
+        const uint32_t a[2][4] = {{x0.x, x1.x, x0.y, x1.y}, {x0.z, x1.z, x0.w, x1.w}};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) hi[e] = tf32_hi(a[i][e]), lo[e] = tf32_lo(a[i][e]);
+#pragma unroll
+          for (int nt = 0; nt < C::kNT; ++nt) {
+            const uint32_t *qq = q[nt][2 * j + i];
+            mma<kTf32>(c[nt], hi, tf32_lo(qq[0]), tf32_lo(qq[1]));
+            mma<kTf32>(c[nt], lo, tf32_hi(qq[0]), tf32_hi(qq[1]));
+            mma<kTf32>(c[nt], hi, tf32_hi(qq[0]), tf32_hi(qq[1]));
+          }
+        }
+      }
+    } else {
+      auto step = [&](int s, const uint32_t(&a)[4]) {
+#pragma unroll
+        for (int nt = 0; nt < C::kNT; ++nt) {
+          if constexpr (kQTerms == 2) mma<kF16>(c[nt], a, q[nt][s][2], q[nt][s][3]);
+          mma<kF16>(c[nt], a, q[nt][s][0], q[nt][s][1]);
+        }
+      };
+      if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
+#pragma unroll
+        for (int j = 0; j < C::D / 64; ++j) {
+          const uint4 x0 = lds128(k + swizzle<C>(tr + g, 16 * (t + 4 * j)));
+          const uint4 x1 = lds128(k + swizzle<C>(tr + g + 8, 16 * (t + 4 * j)));
+          const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a[4] = {ptx::e4m3x2_to_f16x2(w0[i]), ptx::e4m3x2_to_f16x2(w1[i]),
+                                   ptx::e4m3x2_to_f16x2(w0[i] >> 16),
+                                   ptx::e4m3x2_to_f16x2(w1[i] >> 16)};
+            step(4 * j + i, a);
+          }
+        }
+      } else {
+        constexpr int kWords = C::D / 32;
+        uint32_t w0[kWords], w1[kWords];
+        if constexpr (C::D == 64) {
+          const uint2 x0 = lds64(k + swizzle<C>(tr + g, 8 * t));
+          const uint2 x1 = lds64(k + swizzle<C>(tr + g + 8, 8 * t));
+          w0[0] = x0.x, w0[1] = x0.y, w1[0] = x1.x, w1[1] = x1.y;
+        } else {
+          const uint4 x0 = lds128(k + swizzle<C>(tr + g, 16 * t));
+          const uint4 x1 = lds128(k + swizzle<C>(tr + g + 8, 16 * t));
+          w0[0] = x0.x, w0[1] = x0.y, w0[2] = x0.z, w0[3] = x0.w;
+          w1[0] = x1.x, w1[1] = x1.y, w1[2] = x1.z, w1[3] = x1.w;
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t y0 = w0[i] >> (8 * j), y1 = w1[i] >> (8 * j);
+            const uint32_t a[4] = {int4_f16x2<false>(y0), int4_f16x2<false>(y1),
+                                   int4_f16x2<true>(y0), int4_f16x2<true>(y1)};
+            step(2 * i + j, a);
+          }
+      }
+    }
+
+    // ---- scales of keys g and g + 8
+    float vs[2] = {1.f, 1.f}, vm[2] = {0.f, 0.f};
+    if constexpr (C::kScaled) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t at = scales + 4 * (tr + g + 8 * i);
+        const uint32_t ks = lds32(at), vw = lds32(at + 4 * C::kKeys);
+        if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
+          vs[i] = __uint_as_float(vw);
+#pragma unroll
+          for (int nt = 0; nt < C::kNT; ++nt) {
+            c[nt][2 * i] *= __uint_as_float(ks);
+            c[nt][2 * i + 1] *= __uint_as_float(ks);
+          }
+        } else {
+          const float s = ptx::bf16_lo(ks), mid = fmaf(8.f, s, ptx::bf16_hi(ks));
+          vs[i] = ptx::bf16_lo(vw);
+          vm[i] = fmaf(8.f, vs[i], ptx::bf16_hi(vw));
+#pragma unroll
+          for (int nt = 0; nt < C::kNT; ++nt) {
+            c[nt][2 * i] = fmaf(c[nt][2 * i], s, mid * qsum[nt][0]);
+            c[nt][2 * i + 1] = fmaf(c[nt][2 * i + 1], s, mid * qsum[nt][1]);
+          }
+        }
+      }
+    }
+
+    // ---- weights: 2^(score - m), m raised first where a score is far above it
+    float d[C::kNT][4];
+    bool raise = false;
+#pragma unroll
+    for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d[nt][e] = fmaf(c[nt][e], qf[nt][e & 1], -m[nt][e & 1]);
+        if constexpr (kTail) {
+          const int64_t key = key0 + g + 8 * (e >> 1);
+          const int64_t j = key - seq.len;
+          if (j >= 0 && (j >= seq.n || !(word[nt][e & 1] >> j & 1))) d[nt][e] = -INFINITY;
+        }
+        raise = raise || d[nt][e] > 4.f;
+      }
+    if constexpr (C::kScaled) raise = raise || fmaxf(vs[0], vs[1]) * vinv > 2048.f;
+    if (__any_sync(0xffffffffu, raise)) {
+      float ratio = 1.f;
+      if constexpr (C::kScaled) {
+        float top = fmaxf(vs[0], vs[1]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        if (top * vinv > 2048.f) {  // the same in the whole warp
+          // 2^7 <= top * vinv < 2^8: weights of 2^4 times scales up to 2^11
+          // stay below 2^16, and a weight has all its 11 bits down to 2^-21
+          const int f = min(max(261 - (int)(__float_as_uint(top) >> 23), 1), 253);
+          const float now = __uint_as_float((uint32_t)f << 23);
+          ratio = now / vinv;
+          vinv = now;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float top = m[nt][i];
+#pragma unroll
+          for (int e = i; e < 4; e += 2)
+            if (d[nt][e] != -INFINITY) top = fmaxf(top, c[nt][e] * qf[nt][i]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float f = ptx::ex2_approx(m[nt][i] - top);
+          m[nt][i] = top;
+          l[nt][i] *= f;
+          om[nt][i] *= f;
+#pragma unroll
+          for (int e = i; e < 4; e += 2)
+            if (d[nt][e] != -INFINITY) d[nt][e] = fmaf(c[nt][e], qf[nt][i], -top);
+#pragma unroll
+          for (int mt = 0; mt < C::kMt; ++mt) {
+            o[nt][mt][i] *= f * ratio;
+            o[nt][mt][2 + i] *= f * ratio;
+          }
+        }
+    }
+    // P^T as the narrow operand: [term][keys 0-7, 8-15]
+    constexpr int kPTerms = C::kKind == kBf16 || (C::kKind == kF16 && C::kF32) ? 2 : 1;
+    uint32_t pb[C::kNT][kPTerms][2];
+    float pf[C::kNT][4];  // tf32: weight of query g at keys 2t, 2t+1 of each half
+    float pv[C::kNT][4];
+    const float w[2] = {vs[0] * vinv, vs[1] * vinv};
+#pragma unroll
+    for (int nt = 0; nt < C::kNT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = ptx::ex2_approx(d[nt][e]);
+        l[nt][e & 1] += x;
+        pv[nt][e] = C::kScaled ? x * w[e >> 1] : x;
+        if (kTail && C::kScaled && d[nt][e] == -INFINITY) pv[nt][e] = 0.f;  // scale NaN
+        if constexpr (C::kFmt == WFATTN_CACHE_INT4) {
+          const float y = x * vm[e >> 1];
+          om[nt][e & 1] += kTail && d[nt][e] == -INFINITY ? 0.f : y;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float x = pv[nt][2 * i], y = pv[nt][2 * i + 1];
+        if constexpr (C::kKind == kTf32) {
+          const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+          const uint32_t hi = movmatrix(__byte_perm(a, b, 0x7632));
+          const uint32_t lo = movmatrix(__byte_perm(a, b, 0x5410));
+          pf[nt][2 * i] = __uint_as_float(__byte_perm(lo, hi, 0x5410));
+          pf[nt][2 * i + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
+        } else if constexpr (C::kKind == kBf16) {
+          const uint32_t hi = ptx::pack_bf16x2(x, y);
+          pb[nt][0][i] = movmatrix(hi);
+          pb[nt][1][i] = movmatrix(ptx::pack_bf16x2(x - ptx::bf16_lo(hi), y - ptx::bf16_hi(hi)));
+        } else {
+          const uint32_t hi = pack_f16x2(x, y);
+          pb[nt][0][i] = movmatrix(hi);
+          if constexpr (kPTerms == 2) {
+            const float2 f = ptx::f16x2_to_f32(hi);
+            pb[nt][1][i] = movmatrix(pack_f16x2(x - f.x, y - f.y));
+          }
+        }
+      }
+    }
+
+    // ---- O^T += V^T P^T
+    bool odd = false;  // tail: V holds something that is not finite
+    // f32 results: a tile's product is added in f32 arithmetic, so that cut
+    // bits do not pile up along the keys
+    auto add = [&](int mt, uint32_t(&a)[4]) {
+      if constexpr (kTail && C::kFmt != WFATTN_CACHE_INT4) {
+        constexpr uint32_t kExp = C::kKind == kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((a[e] & kExp) == kExp) a[e] &= 0xffff0000u, odd = true;
+          if ((a[e] >> 16 & kExp) == kExp) a[e] &= 0xffffu, odd = true;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < C::kNT; ++nt) {
+        if constexpr (C::kF32) {
+          float z[4] = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (kPTerms == 2) mma<C::kKind>(z, a, pb[nt][1][0], pb[nt][1][1]);
+          mma<C::kKind>(z, a, pb[nt][0][0], pb[nt][0][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][mt][e] += z[e];
+        } else {
+          if constexpr (kPTerms == 2)
+            mma<C::kKind>(o[nt][mt], a, pb[nt][1][0], pb[nt][1][1]);
+          mma<C::kKind>(o[nt][mt], a, pb[nt][0][0], pb[nt][0][1]);
+        }
+      }
+    };
+    if constexpr (C::kKind == kBf16) {
+      const int row = tr + (lane & 7) + 8 * (lane >> 4);
+#pragma unroll
+      for (int mt = 0; mt < C::kMt; ++mt) {
+        uint32_t a[4];
+        ldmatrix4<true>(v + swizzle<C>(row, 32 * mt + 16 * (lane >> 3 & 1)), a);
+        add(mt, a);
+      }
+    } else if constexpr (C::kKind == kTf32) {
+#pragma unroll
+      for (int h = 0; h < C::D / 32; ++h) {
+        uint4 x[4];  // keys 2t, 2t + 1 of each half
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = lds128(v + swizzle<C>(tr + 2 * t + (i & 1) + 8 * (i >> 1), 16 * (g + 8 * h)));
+          if constexpr (kTail) {
+            uint32_t *y = &x[i].x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if ((y[e] & 0x7f800000u) == 0x7f800000u) y[e] = 0, odd = true;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int mt = 2 * h + j;
+          uint32_t hi[2][4], lo[2][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t a[4] = {j ? x[2 * i].z : x[2 * i].x, j ? x[2 * i].w : x[2 * i].y,
+                                   j ? x[2 * i + 1].z : x[2 * i + 1].x,
+                                   j ? x[2 * i + 1].w : x[2 * i + 1].y};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hi[i][e] = tf32_hi(a[e]), lo[i][e] = tf32_lo(a[e]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < C::kNT; ++nt) {
+            float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t p0 = __float_as_uint(pf[nt][2 * i]);
+              const uint32_t p1 = __float_as_uint(pf[nt][2 * i + 1]);
+              mma<kTf32>(z, hi[i], tf32_lo(p0), tf32_lo(p1));
+              mma<kTf32>(z, lo[i], tf32_hi(p0), tf32_hi(p1));
+              mma<kTf32>(z, hi[i], tf32_hi(p0), tf32_hi(p1));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nt][mt][e] += z[e];
+          }
+        }
+      }
+    } else if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
+      constexpr int kWords = C::D / 32;
+      uint32_t x[4][kWords];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = tr + 2 * t + (i & 1) + 8 * (i >> 1);
+        if constexpr (C::D == 64) {
+          const uint2 y = lds64(v + swizzle<C>(row, 8 * g));
+          x[i][0] = y.x, x[i][1] = y.y;
+        } else {
+          const uint4 y = lds128(v + swizzle<C>(row, 16 * g));
+          x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kWords; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t y0 = __byte_perm(x[0][i], x[1][i], j ? 0x7362 : 0x5140);
+          const uint32_t y1 = __byte_perm(x[2][i], x[3][i], j ? 0x7362 : 0x5140);
+          uint32_t a[4] = {ptx::e4m3x2_to_f16x2(y0), ptx::e4m3x2_to_f16x2(y0 >> 16),
+                           ptx::e4m3x2_to_f16x2(y1), ptx::e4m3x2_to_f16x2(y1 >> 16)};
+          add(2 * i + j, a);
+        }
+    } else {
+      constexpr int kWords = C::D / 64;
+      uint32_t x[4][kWords];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = tr + 2 * t + (i & 1) + 8 * (i >> 1);
+        if constexpr (C::D == 64) {
+          x[i][0] = lds32(v + swizzle<C>(row, 4 * g));
+        } else {
+          const uint2 y = lds64(v + swizzle<C>(row, 8 * g));
+          x[i][0] = y.x, x[i][1] = y.y;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kWords; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t y0 = __byte_perm(x[0][i], x[1][i], h ? 0x7632 : 0x5410);
+          const uint32_t y1 = __byte_perm(x[2][i], x[3][i], h ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t z0 = y0 >> (8 * j), z1 = y1 >> (8 * j);
+            uint32_t a[4] = {int4_f16x2<false>(z0), int4_f16x2<true>(z0), int4_f16x2<false>(z1),
+                             int4_f16x2<true>(z1)};
+            add(4 * i + 2 * h + j, a);
+          }
+        }
+    }
+    if constexpr (kTail && C::kFmt != WFATTN_CACHE_INT4) {
+      // What is not finite was left out of the products, where a weight of 0
+      // would spread it: queries that see its key get it here.
+      if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+          for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float mine = r < 8 ? (d[nt][i] == -INFINITY ? -1.f : pv[nt][i])
+                                       : (d[nt][2 + i] == -INFINITY ? -1.f : pv[nt][2 + i]);
+              const float x = __shfl_sync(0xffffffffu, mine, 4 * (r & 7) + t);
+              if (x < 0.f) continue;
+#pragma unroll
+              for (int mt = 0; mt < C::kMt; ++mt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float y = v_value<C>(v, tr + r, o_index<C>(mt, g, e));
+                  if (!(fabsf(y) <= FLT_MAX)) o[nt][mt][2 * e + i] += x * y;
+                }
+            }
+      }
+    }
+  }
+};
+
+// Where the row r of a segment goes, or null: no such row.  `live`: the node
+// is no padding.
+__device__ __forceinline__ uint8_t *out_row(const Params &p, int64_t b, int64_t h, int r, int n,
+                                            int size, bool &live) {
+  if (r >= p.R) return nullptr;
+  const int hg = r / p.T, node = r - hg * p.T;
+  live = node < n;
+  return p.o + (b * p.os.b + (h * p.G + hg) * p.os.h + node * p.os.s) * size;
+}
+
+template <bool kF32>
+__device__ __forceinline__ void store_out(uint8_t *row, int d, float x) {
+  if constexpr (kF32)
+    reinterpret_cast<float *>(row)[d] = x;
+  else
+    reinterpret_cast<uint16_t *>(row)[d] = (uint16_t)ptx::pack_bf16x2(x, 0.f);
+}
+
+template <class C>
+__global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  float *merge = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
+  float *stats = reinterpret_cast<float *>(smem + C::kStages * C::kStage + C::kMerge);
+  const uint32_t ring = ptx::smem_u32(smem);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rw = warp / C::kKW, kw = warp % C::kKW;
+
+  int64_t begin, end, all;
+  Cursor<C::kKeys> cur = share<C::kKeys>(p, begin, end, all), ahead = cur;
+  const int64_t units = end - begin;
+  if (threadIdx.x == 0) {
+    Desc d;
+    d.seg = -1;
+    d.last = 0;
+    d.head = units > 0 && cur.u > 0;
+    p.desc[blockIdx.x] = d;
+  }
+  if (units <= 0) return;
+
+  auto fetch = [&](int64_t i) {
+    if (i < units) {
+      const int64_t h = ahead.hr / p.RT, at = ahead.u * C::kKeys;
+      const int64_t row = ahead.b * p.c.sb + h * p.c.sh + at;
+      const int live = (int)imin64(C::kKeys, ahead.s.total - at);
+      const uint32_t st = ring + (uint32_t)(i % C::kStages) * C::kStage;
+      const uint8_t *k = p.c.k + row * C::kRowBytes, *v = p.c.v + row * C::kRowBytes;
+      constexpr int kPieces = C::kKBytes / 16;
+#pragma unroll
+      for (int j = 0; j < kPieces / kThreads; ++j) {
+        const int piece = threadIdx.x + j * kThreads;
+        const int r = piece / (C::kRowBytes / 16), o = piece % (C::kRowBytes / 16) * 16;
+        const uint32_t dst = st + swizzle<C>(r, o);
+        const int64_t src = r < live ? piece * 16 : 0;
+        cp_async16(dst, k + src, r < live);
+        cp_async16(dst + C::kKBytes, v + src, r < live);
+      }
+      if constexpr (C::kScaled) {
+        for (int r = threadIdx.x; r < 2 * C::kKeys; r += kThreads) {
+          const int rr = r % C::kKeys;
+          const uint8_t *s = r < C::kKeys ? p.c.k_scale : p.c.v_scale;
+          cp_async4(st + 2 * C::kKBytes + 4 * r, s + (row + (rr < live ? rr : 0)) * 4, rr < live);
+        }
+      }
+      ahead.next(p);
+    }
+    cp_async_commit();
+  };
+  static_assert(C::kKBytes / 16 % kThreads == 0, "pieces per thread");
+
+#pragma unroll 1
+  for (int i = 0; i < C::kStages - 1; ++i) fetch(i);
+  Warp<C> w;
+  bool fresh = true;  // the segment's queries are not loaded yet
+  bool headed = cur.u == 0;  // it begins in this CTA
+#pragma unroll 1
+  for (int64_t i = 0; i < units; ++i) {
+    const int64_t h = cur.hr / p.RT;
+    const int tile = (int)(cur.hr - h * p.RT);
+    if (fresh) w.load_q(p, cur.b, h, tile * C::kRows + rw * 8 * C::kNT);
+    fresh = false;
+    cp_async_wait<C::kStages - 2>();
+    __syncthreads();  // the unit is here, and the stage refilled next is read
+    fetch(i + C::kStages - 1);
+    const uint32_t st = ring + (uint32_t)(i % C::kStages) * C::kStage;
+    const int64_t key0 = cur.u * C::kKeys;
+#pragma unroll 1
+    for (int j = 0; j < C::kTiles; ++j) {
+      const int tr = 16 * (kw + C::kKW * j);
+      if (key0 + tr >= cur.s.total) break;
+      if (key0 + tr + 16 <= cur.s.len)
+        w.template tile<false>(st, st + C::kKBytes, st + 2 * C::kKBytes, tr, key0 + tr, cur.s);
+      else
+        w.template tile<true>(st, st + C::kKBytes, st + 2 * C::kKBytes, tr, key0 + tr, cur.s);
+    }
+
+    const bool done = cur.u + 1 == cur.s.units;
+    if (done || i + 1 == units) {
+      const bool whole = done && headed;
+      const int g = lane >> 2, t = lane & 3;
+      const float back = C::kScaled ? 1.f / w.vinv : 1.f;
+#pragma unroll
+      for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            w.l[nt][e] += __shfl_xor_sync(0xffffffffu, w.l[nt][e], x);
+            if constexpr (C::kFmt == WFATTN_CACHE_INT4)
+              w.om[nt][e] += __shfl_xor_sync(0xffffffffu, w.om[nt][e], x);
+          }
+#pragma unroll
+          for (int mt = 0; mt < C::kMt; ++mt) {
+            w.o[nt][mt][e] = w.o[nt][mt][e] * back + w.om[nt][e];
+            w.o[nt][mt][2 + e] = w.o[nt][mt][2 + e] * back + w.om[nt][e];
+          }
+        }
+      const int slot = headed ? 1 : 0;
+      float *part = p.part + (int64_t)(blockIdx.x * 2 + slot) * C::kRows * C::D;
+      float *part_ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D +
+                       (int64_t)(blockIdx.x * 2 + slot) * C::kRows * 2;
+      constexpr int kSize = C::kF32 ? 4 : 2;
+      if constexpr (C::kKW == 1) {
+        // the warp has all the keys of its rows
+#pragma unroll
+        for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = (rw * C::kNT + nt) * 8 + 2 * t + e;
+            if (whole) {
+              bool live;
+              uint8_t *to = out_row(p, cur.b, h, tile * C::kRows + r, cur.s.n, kSize, live);
+              const float inv = live && w.l[nt][e] != 0.f ? 1.f / w.l[nt][e] : 0.f;
+              if (!to) continue;
+#pragma unroll
+              for (int mt = 0; mt < C::kMt; ++mt)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                  store_out<C::kF32>(to, o_index<C>(mt, g, y),
+                                     inv == 0.f ? 0.f : w.o[nt][mt][2 * y + e] * inv);
+            } else {
+#pragma unroll
+              for (int mt = 0; mt < C::kMt; ++mt)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                  part[r * C::D + o_index<C>(mt, g, y)] = w.o[nt][mt][2 * y + e];
+              if (g == 0) {
+                part_ml[2 * r] = w.m[nt][e];
+                part_ml[2 * r + 1] = w.l[nt][e];
+              }
+            }
+          }
+      } else {
+        // join the warps that have the other keys of the rows
+        float *mine = merge + warp * 8 * C::kNT * C::kOStride;
+#pragma unroll
+        for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = 8 * nt + 2 * t + e;
+#pragma unroll
+            for (int mt = 0; mt < C::kMt; ++mt)
+#pragma unroll
+              for (int y = 0; y < 2; ++y)
+                mine[r * C::kOStride + o_index<C>(mt, g, y)] = w.o[nt][mt][2 * y + e];
+            if (g == 0) {
+              stats[(warp * 8 * C::kNT + r) * 2] = w.m[nt][e];
+              stats[(warp * 8 * C::kNT + r) * 2 + 1] = w.l[nt][e];
+            }
+          }
+        __syncthreads();
+#pragma unroll 1
+        for (int x = threadIdx.x; x < C::kRows * C::D; x += kThreads) {
+          const int r = x / C::D, dd = x % C::D;
+          const int rr = r % (8 * C::kNT), w0 = r / (8 * C::kNT) * C::kKW;
+          float m = -FLT_MAX, l = 0.f, o = 0.f;
+#pragma unroll
+          for (int y = 0; y < C::kKW; ++y)
+            m = fmaxf(m, stats[((w0 + y) * 8 * C::kNT + rr) * 2]);
+#pragma unroll
+          for (int y = 0; y < C::kKW; ++y) {
+            const int at = (w0 + y) * 8 * C::kNT + rr;
+            const float f = ptx::ex2_approx(stats[at * 2] - m);
+            l = fmaf(stats[at * 2 + 1], f, l);
+            o = fmaf(merge[at * C::kOStride + dd], f, o);
+          }
+          if (whole) {
+            bool live;
+            uint8_t *to = out_row(p, cur.b, h, tile * C::kRows + r, cur.s.n, kSize, live);
+            if (to) store_out<C::kF32>(to, dd, live && l != 0.f ? o / l : 0.f);
+          } else {
+            part[x] = o;
+            if (dd == 0) {
+              part_ml[2 * r] = m;
+              part_ml[2 * r + 1] = l;
+            }
+          }
+        }
+      }
+      if (!done && headed && threadIdx.x == 0) {
+        // goes on: unit s lies in CTA ((s + 1) * ctas - 1) / all
+        const int64_t last = begin + i + (cur.s.units - 1 - cur.u);
+        p.desc[blockIdx.x].seg = cur.b * p.HR + cur.hr;
+        p.desc[blockIdx.x].last = (int32_t)(((last + 1) * p.ctas - 1) / all);
+      }
+      fresh = true;
+      headed = true;
+    }
+    cur.next(p);
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the partials of a segment that more than one CTA worked on: block
+// (x, y) the row y of the one that begins in CTA x.  Warps take every fourth
+// partial, eight loads in flight each; then the four sums are joined.
+template <int D, bool kF32, int kRows, int kKeys>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
+  __shared__ float sums[kWarps][D + 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Desc desc = p.desc[blockIdx.x];
+  if (desc.seg < 0) return;
+  const int64_t b = desc.seg / p.HR, hr = desc.seg - b * p.HR, h = hr / p.RT;
+  const Seq s = sequence<kKeys>(p, b, false);
+  const int row = blockIdx.y;
+  bool live = false;
+  uint8_t *to = out_row(p, b, h, (int)(hr - h * p.RT) * kRows + row, s.n, kF32 ? 4 : 2, live);
+  if (!to) return;
+  constexpr int kVals = D / 32;
+  const float *ml = p.part + (int64_t)p.ctas * 2 * kRows * D;
+  const int first = (int)blockIdx.x, n = desc.last - first + 1;
+  float m = -FLT_MAX, l = 0.f, o[kVals];
+#pragma unroll
+  for (int i = 0; i < kVals; ++i) o[i] = 0.f;
+  for (int c0 = warp; c0 < n; c0 += 32 * kWarps) {
+    // lane i: piece c0 + 4 i
+    const int c = c0 + kWarps * lane;
+    float mc = -FLT_MAX, lc = 0.f;
+    if (c < n && (c == 0 || p.desc[first + c].head)) {
+      const float *at = ml + ((int64_t)((first + c) * 2 + (c == 0)) * kRows + row) * 2;
+      mc = at[0];
+      lc = at[1];
+    }
+    float top = fmaxf(m, mc);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float f = ptx::ex2_approx(m - top);
+    const float w = lc == 0.f && mc == -FLT_MAX ? 0.f : ptx::ex2_approx(mc - top);
+    float lw = lc * w;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, x);
+    l = l * f + lw;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < kVals; ++i) o[i] *= f;
+    const int count = min(32, (n - c0 + kWarps - 1) / kWarps);
+    const unsigned some = __ballot_sync(0xffffffffu, w != 0.f);
+    for (int j = 0; j < count; j += 8) {
+      float x[8][kVals];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int cc = c0 + kWarps * (j + k);
+        const bool use = j + k < 32 && (some >> ((j + k) & 31) & 1);
+        const float *at = p.part + ((int64_t)((first + cc) * 2 + (cc == 0)) * kRows + row) * D +
+                          lane * kVals;
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) x[k][i] = use ? at[i] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, w, (j + k) & 31);
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) o[i] = fmaf(x[k][i], wk, o[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kVals; ++i) sums[warp][lane * kVals + i] = o[i];
+  if (lane == 0) {
+    sums[warp][D] = m;
+    sums[warp][D + 1] = l;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x >= D) return;
+  float top = sums[0][D];
+#pragma unroll
+  for (int i = 1; i < kWarps; ++i) top = fmaxf(top, sums[i][D]);
+  float total = 0.f, x = 0.f;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    const float f = ptx::ex2_approx(sums[i][D] - top);
+    total = fmaf(sums[i][D + 1], f, total);
+    x = fmaf(sums[i][threadIdx.x], f, x);
+  }
+  store_out<kF32>(to, threadIdx.x, live && total != 0.f ? x / total : 0.f);
+}
+
+// ------------------------------------------------------------------ launch
+
+template <class C>
+size_t workspace_bytes() {
+  const size_t ctas = (size_t)kMaxSms * C::kCtas;
+  return ctas * (sizeof(Desc) + 2 * C::kRows * (C::D + 2) * sizeof(float));
+}
+
+template <class C>
+cudaError_t launch(Params p, void *workspace, const DeviceInfo &dev, cudaStream_t stream) {
+  p.RT = (p.R + C::kRows - 1) / C::kRows;
+  p.HR = p.c.H * p.RT;
+  const int64_t units = (p.c.L + C::kKeys - 1) / C::kKeys;  // of a segment, at most
+  const int64_t most = (dev.sm_count < kMaxSms ? dev.sm_count : kMaxSms) * C::kCtas;
+  p.ctas = (int)imin64(most, units > most ? most : units * (p.c.B * p.HR > most ? most : p.c.B * p.HR));
+  p.desc = static_cast<Desc *>(workspace);
+  p.part = reinterpret_cast<float *>(p.desc + most);
+  cudaError_t err = ensure_smem_attr(reinterpret_cast<const void *>(split_kernel<C>), C::kSmem,
+                                     dev.device);
+  if (err != cudaSuccess) return err;
+  split_kernel<C><<<p.ctas, kThreads, C::kSmem, stream>>>(p);
+  err = cudaGetLastError();
+  if (err != cudaSuccess || units == 1) return err;  // no segment is split
+  join_kernel<C::D, C::kF32, C::kRows, C::kKeys>
+      <<<dim3(p.ctas, C::kRows < p.R ? C::kRows : p.R), kThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+// Calls f with the configuration for R query rows a cache head: one 8-row tile
+// a warp while the rows fit, then two (not with f32 queries, whose fragments
+// are twice as large), then warps take different rows instead of keys.
+template <int kFmt, bool kF32, int D, class F>
+auto with_rows(int R, F f) {
+  if (R <= 8) return f(Cfg<kFmt, D, kF32, 1, 1>{});
+  if constexpr (kF32) {
+    if (R <= 16) return f(Cfg<kFmt, D, true, 1, 2>{});
+    return f(Cfg<kFmt, D, true, 1, 4>{});
+  } else {
+    if (R <= 16) return f(Cfg<kFmt, D, false, 2, 1>{});
+    if (R <= 32) return f(Cfg<kFmt, D, false, 2, 2>{});
+    return f(Cfg<kFmt, D, false, 2, 4>{});
+  }
+}
+
+template <int kFmt, bool kF32>
+size_t workspace_for(int D, int R) {
+  auto f = [](auto cfg) { return workspace_bytes<decltype(cfg)>(); };
+  return D == 64 ? with_rows<kFmt, kF32, 64>(R, f) : with_rows<kFmt, kF32, 128>(R, f);
+}
+
+template <int kFmt, bool kF32>
+cudaError_t launch_for(const Params &p, void *workspace, const DeviceInfo &dev,
+                       cudaStream_t stream) {
+  auto f = [&](auto cfg) { return launch<decltype(cfg)>(p, workspace, dev, stream); };
+  return p.c.D == 64 ? with_rows<kFmt, kF32, 64>(p.R, f) : with_rows<kFmt, kF32, 128>(p.R, f);
+}
+
+}  // namespace tree
+
+// One translation unit a row format and query type (tree_decode_*.cu).
+#define WFATTN_TREE_KINDS(X)                                                           \
+  X(f32_f32, WFATTN_CACHE_F32, true) X(bf16_bf16, WFATTN_CACHE_BF16, false)            \
+  X(e4m3_bf16, WFATTN_CACHE_E4M3, false) X(e4m3_f32, WFATTN_CACHE_E4M3, true)          \
+  X(int4_bf16, WFATTN_CACHE_INT4, false) X(int4_f32, WFATTN_CACHE_INT4, true)
+#define WFATTN_TREE_DECLARE(name, fmt, f32)                                            \
+  size_t tree_workspace_##name(int D, int R);                                          \
+  cudaError_t tree_launch_##name(const tree::Params &p, void *workspace,               \
+                                 const DeviceInfo &dev, cudaStream_t stream);
+WFATTN_TREE_KINDS(WFATTN_TREE_DECLARE)
+
+#define WFATTN_TREE_DEFINE(name, fmt, f32)                                             \
+  size_t tree_workspace_##name(int D, int R) { return tree::workspace_for<fmt, f32>(D, R); } \
+  cudaError_t tree_launch_##name(const tree::Params &p, void *workspace,               \
+                                 const DeviceInfo &dev, cudaStream_t stream) {         \
+    return tree::launch_for<fmt, f32>(p, workspace, dev, stream);                      \
+  }
+
+}  // namespace wfattn

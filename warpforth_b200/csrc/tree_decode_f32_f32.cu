@@ -1,0 +1,6 @@
+// tree_decode over f32 rows with f32 queries.
+#include "tree_decode.cuh"
+
+namespace wfattn {
+WFATTN_TREE_DEFINE(f32_f32, WFATTN_CACHE_F32, true)
+}  // namespace wfattn

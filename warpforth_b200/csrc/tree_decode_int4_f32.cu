@@ -1,0 +1,6 @@
+// tree_decode over int4 rows with f32 queries.
+#include "tree_decode.cuh"
+
+namespace wfattn {
+WFATTN_TREE_DEFINE(int4_f32, WFATTN_CACHE_INT4, true)
+}  // namespace wfattn
