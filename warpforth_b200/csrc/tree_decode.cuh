@@ -55,7 +55,6 @@ struct Desc {
 
 struct Params {
   CacheView c;
-  int64_t HR;    // segments a sequence: heads * row tiles
   int RT;        // row tiles a head
   int R, G, T;   // query rows a head = G heads x T nodes
   int ctas;      // of the grid
@@ -89,7 +88,11 @@ struct Cfg {
   static constexpr int kOStride = D + 2;  // floats a row of the merge buffer
   static constexpr int kMerge = kKW > 1 ? kWarps * 8 * kNT * kOStride * 4 : 0;
   static constexpr int kStats = kWarps * 8 * kNT * 2 * 4;
-  static constexpr int kCtas = kRowBytes >= 512 ? 1 : kRowBytes == 256 ? 2 : kNT * D <= 64 ? 4 : 3;
+  // CTAs an SM: as many as the registers of the fragments and two stages allow
+  static constexpr int kCtas = kRowBytes >= 512                                     ? 1
+                               : kRowBytes == 256 || (kF32 ? 2 : kNT) * D == 256 ? 2
+                               : kNT * D <= 64                                      ? 4
+                                                                                    : 3;
   static constexpr int kBudget = 227 * 1024 / kCtas - 2048;
   static constexpr int kFit = (kBudget - kMerge - kStats) / kStage;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
@@ -101,6 +104,9 @@ struct Cfg {
 
 // ------------------------------------------------------------- instructions
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(live ? 16 : 0)
@@ -194,11 +200,12 @@ __device__ __forceinline__ uint32_t int4_f16x2(uint32_t w) {
   return kOdd ? hsub2(and_or<0x00f000f0u, 0x54005400u>(w), 0x54805480u)
               : hsub2(and_or<0x000f000fu, 0x64006400u>(w), 0x64086408u);
 }
-// f32 as tf32 terms: the upper 10 fraction bits, and what is left (exact; the
-// product unit takes its upper bits)
-__device__ __forceinline__ uint32_t tf32_hi(uint32_t x) { return x & 0xffffe000u; }
+// f32 as tf32 terms: x to the nearest of 10 fraction bits (so that what the
+// products cut from the rest has no sign of its own), and what is left (exact;
+// the product unit takes its upper bits)
+__device__ __forceinline__ uint32_t tf32_hi(uint32_t x) { return (x + 0x1000u) & 0xffffe000u; }
 __device__ __forceinline__ uint32_t tf32_lo(uint32_t x) {
-  return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u));
+  return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf32_hi(x)));
 }
 
 // ----------------------------------------------------------------- layouts
@@ -253,40 +260,46 @@ __device__ __forceinline__ float v_value(uint32_t v, int row, int d) {
 // -------------------------------------------------------------- work order
 
 struct Seq {
-  int64_t len, total;  // rows before the tree, rows in all
-  int n;               // nodes
-  int64_t units;       // of one segment, at least 1
+  int len, total;  // rows before the tree, rows in all
+  int n;           // nodes
+  int units;       // of one segment, at least 1
 };
 
 template <int kKeys>
-__device__ __forceinline__ Seq sequence(const Params &p, int64_t b, bool report) {
+__device__ __forceinline__ Seq sequence(const Params &p, int b, bool report) {
   Seq s;
-  int64_t len = p.lens[b], n = p.counts ? p.counts[b] : p.T;
+  const int L = (int)p.c.L;
+  int len = p.lens[b], n = p.counts ? p.counts[b] : p.T;
   bool bad = len < 0 || n < 0 || n > p.T;
-  len = len < 0 ? 0 : len;
-  n = n < 0 ? 0 : n > p.T ? p.T : n;
-  bad = bad || len + n > p.c.L;
-  len = imin64(len, p.c.L);
-  n = imin64(n, p.c.L - len);
+  len = max(len, 0);
+  n = min(max(n, 0), p.T);
+  bad = bad || len > L || n > L - len;
+  len = min(len, L);
+  n = min(n, L - len);
   if (bad && report) atomicOr(p.status, kDevBadRowMask);
   s.len = len;
-  s.n = (int)n;
+  s.n = n;
   s.total = len + n;
-  s.units = imax64(1, (s.total + kKeys - 1) / kKeys);
+  s.units = max(1, (s.total - 1) / kKeys + 1);
   return s;
 }
 
-// A position in the order of units.
+// A position in the order of units: sequence, cache head, tile of query rows,
+// unit of keys.
 template <int kKeys>
 struct Cursor {
-  int64_t b, hr, u;
+  int b, h, tile, u;
   Seq s;
-  __device__ __forceinline__ void next(const Params &p) {
-    if (++u < s.units) return;
+  // whether the next unit is another segment's
+  __device__ __forceinline__ bool next(const Params &p) {
+    if (++u < s.units) return false;
     u = 0;
-    if (++hr < p.HR) return;
-    hr = 0;
-    if (++b < p.c.B) s = sequence<kKeys>(p, b, false);
+    if (++tile < p.RT) return true;
+    tile = 0;
+    if (++h < (int)p.c.H) return true;
+    h = 0;
+    if (++b < (int)p.c.B) s = sequence<kKeys>(p, b, false);
+    return true;
   }
 };
 
@@ -296,10 +309,11 @@ __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, 
                                                int64_t &all) {
   __shared__ int64_t warp_sum[kWarps], found[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t per = (p.c.B + kThreads - 1) / kThreads;
-  const int64_t b0 = imin64(p.c.B, threadIdx.x * per), b1 = imin64(p.c.B, b0 + per);
+  const int B = (int)p.c.B, per = (B + kThreads - 1) / kThreads;
+  const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
+  const int64_t HR = p.c.H * p.RT;
   int64_t mine = 0;
-  for (int64_t b = b0; b < b1; ++b) mine += sequence<kKeys>(p, b, blockIdx.x == 0).units * p.HR;
+  for (int b = b0; b < b1; ++b) mine += sequence<kKeys>(p, b, blockIdx.x == 0).units * HR;
   int64_t upto = mine;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
@@ -317,9 +331,10 @@ __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, 
   begin = all * blockIdx.x / p.ctas;
   end = all * (blockIdx.x + 1) / p.ctas;
   if (begin >= upto - mine && begin < upto) {
-    int64_t at = upto - mine, b = b0;
+    int64_t at = upto - mine;
+    int b = b0;
     for (;; ++b) {
-      const int64_t n = sequence<kKeys>(p, b, false).units * p.HR;
+      const int64_t n = sequence<kKeys>(p, b, false).units * HR;
       if (begin < at + n) break;
       at += n;
     }
@@ -328,10 +343,12 @@ __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, 
   }
   __syncthreads();
   Cursor<kKeys> c;
-  c.b = found[0];
+  c.b = (int)found[0];
   c.s = sequence<kKeys>(p, c.b, false);
-  c.hr = found[1] / c.s.units;
-  c.u = found[1] - c.hr * c.s.units;
+  const int64_t hr = found[1] / c.s.units;
+  c.u = (int)(found[1] - hr * c.s.units);
+  c.h = (int)(hr / p.RT);
+  c.tile = (int)(hr - (int64_t)c.h * p.RT);
   return c;
 }
 
@@ -351,7 +368,7 @@ struct Warp {
   float vinv;  // weights carry scale * vinv
 
   // Loads the query rows `row0`.. of cache head h of sequence b.
-  __device__ __forceinline__ void load_q(const Params &p, int64_t b, int64_t h, int row0) {
+  __device__ __forceinline__ void load_q(const Params &p, int b, int h, int row0) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int nt = 0; nt < C::kNT; ++nt) {
@@ -361,7 +378,7 @@ struct Warp {
       float top = 0.f, sum = 0.f;
       if (r < p.R) {
         const int hg = r / p.T, node = r - hg * p.T;
-        const int64_t at = b * p.qs.b + (h * p.G + hg) * p.qs.h + node * p.qs.s;
+        const int64_t at = b * p.qs.b + ((int64_t)h * p.G + hg) * p.qs.h + node * p.qs.s;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
@@ -432,12 +449,14 @@ struct Warp {
     vinv = __uint_as_float(253u << 23);  // 2^126
   }
 
-  // Attends to the 16 keys of rows tr.. of a stage (k, v, scales), key0 their
-  // position.  kTail: some of them are nodes of the tree, or no keys.
+  // Attends to the 16 keys of rows tr.. of the stage `st`, key0 their position.
+  // kTail: some of them are nodes of the tree, or no keys.
   template <bool kTail>
-  __device__ __forceinline__ void tile(uint32_t k, uint32_t v, uint32_t scales, int tr,
-                                       int64_t key0, const Seq &seq) {
+  __device__ __forceinline__ void tile(uint32_t st, int tr, int key0, const Seq &seq) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // rows 16 apart have the same swizzle
+    const uint32_t k = st + tr * C::kRowBytes, v = k + C::kKBytes;
+    const uint32_t scales = st + 2 * C::kKBytes + 4 * tr;
     float c[C::kNT][4];
 #pragma unroll
     for (int nt = 0; nt < C::kNT; ++nt)
@@ -446,7 +465,7 @@ struct Warp {
 
     // ---- S^T = K Q^T
     if constexpr (C::kKind == kBf16) {
-      const int row = tr + (lane & 15);
+      const int row = lane & 15;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         uint32_t a[4];
@@ -457,8 +476,8 @@ struct Warp {
     } else if constexpr (C::kKind == kTf32) {
 #pragma unroll
       for (int j = 0; j < C::D / 16; ++j) {
-        const uint4 x0 = lds128(k + swizzle<C>(tr + g, 16 * (4 * j + t)));
-        const uint4 x1 = lds128(k + swizzle<C>(tr + g + 8, 16 * (4 * j + t)));
+        const uint4 x0 = lds128(k + swizzle<C>(g, 16 * (4 * j + t)));
+        const uint4 x1 = lds128(k + swizzle<C>(g + 8, 16 * (4 * j + t)));
         const uint32_t a[2][4] = {{x0.x, x1.x, x0.y, x1.y}, {x0.z, x1.z, x0.w, x1.w}};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -485,8 +504,8 @@ struct Warp {
       if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
 #pragma unroll
         for (int j = 0; j < C::D / 64; ++j) {
-          const uint4 x0 = lds128(k + swizzle<C>(tr + g, 16 * (t + 4 * j)));
-          const uint4 x1 = lds128(k + swizzle<C>(tr + g + 8, 16 * (t + 4 * j)));
+          const uint4 x0 = lds128(k + swizzle<C>(g, 16 * (t + 4 * j)));
+          const uint4 x1 = lds128(k + swizzle<C>(g + 8, 16 * (t + 4 * j)));
           const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -500,12 +519,12 @@ struct Warp {
         constexpr int kWords = C::D / 32;
         uint32_t w0[kWords], w1[kWords];
         if constexpr (C::D == 64) {
-          const uint2 x0 = lds64(k + swizzle<C>(tr + g, 8 * t));
-          const uint2 x1 = lds64(k + swizzle<C>(tr + g + 8, 8 * t));
+          const uint2 x0 = lds64(k + swizzle<C>(g, 8 * t));
+          const uint2 x1 = lds64(k + swizzle<C>(g + 8, 8 * t));
           w0[0] = x0.x, w0[1] = x0.y, w1[0] = x1.x, w1[1] = x1.y;
         } else {
-          const uint4 x0 = lds128(k + swizzle<C>(tr + g, 16 * t));
-          const uint4 x1 = lds128(k + swizzle<C>(tr + g + 8, 16 * t));
+          const uint4 x0 = lds128(k + swizzle<C>(g, 16 * t));
+          const uint4 x1 = lds128(k + swizzle<C>(g + 8, 16 * t));
           w0[0] = x0.x, w0[1] = x0.y, w0[2] = x0.z, w0[3] = x0.w;
           w1[0] = x1.x, w1[1] = x1.y, w1[2] = x1.z, w1[3] = x1.w;
         }
@@ -526,7 +545,7 @@ struct Warp {
     if constexpr (C::kScaled) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t at = scales + 4 * (tr + g + 8 * i);
+        const uint32_t at = scales + 4 * (g + 8 * i);
         const uint32_t ks = lds32(at), vw = lds32(at + 4 * C::kKeys);
         if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
           vs[i] = __uint_as_float(vw);
@@ -557,8 +576,7 @@ struct Warp {
       for (int e = 0; e < 4; ++e) {
         d[nt][e] = fmaf(c[nt][e], qf[nt][e & 1], -m[nt][e & 1]);
         if constexpr (kTail) {
-          const int64_t key = key0 + g + 8 * (e >> 1);
-          const int64_t j = key - seq.len;
+          const int j = key0 + g + 8 * (e >> 1) - seq.len;
           if (j >= 0 && (j >= seq.n || !(word[nt][e & 1] >> j & 1))) d[nt][e] = -INFINITY;
         }
         raise = raise || d[nt][e] > 4.f;
@@ -677,7 +695,7 @@ struct Warp {
       }
     };
     if constexpr (C::kKind == kBf16) {
-      const int row = tr + (lane & 7) + 8 * (lane >> 4);
+      const int row = (lane & 7) + 8 * (lane >> 4);
 #pragma unroll
       for (int mt = 0; mt < C::kMt; ++mt) {
         uint32_t a[4];
@@ -690,7 +708,7 @@ struct Warp {
         uint4 x[4];  // keys 2t, 2t + 1 of each half
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[i] = lds128(v + swizzle<C>(tr + 2 * t + (i & 1) + 8 * (i >> 1), 16 * (g + 8 * h)));
+          x[i] = lds128(v + swizzle<C>(2 * t + (i & 1) + 8 * (i >> 1), 16 * (g + 8 * h)));
           if constexpr (kTail) {
             uint32_t *y = &x[i].x;
 #pragma unroll
@@ -731,7 +749,7 @@ struct Warp {
       uint32_t x[4][kWords];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = tr + 2 * t + (i & 1) + 8 * (i >> 1);
+        const int row = 2 * t + (i & 1) + 8 * (i >> 1);
         if constexpr (C::D == 64) {
           const uint2 y = lds64(v + swizzle<C>(row, 8 * g));
           x[i][0] = y.x, x[i][1] = y.y;
@@ -755,7 +773,7 @@ struct Warp {
       uint32_t x[4][kWords];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = tr + 2 * t + (i & 1) + 8 * (i >> 1);
+        const int row = 2 * t + (i & 1) + 8 * (i >> 1);
         if constexpr (C::D == 64) {
           x[i][0] = lds32(v + swizzle<C>(row, 4 * g));
         } else {
@@ -796,7 +814,7 @@ struct Warp {
               for (int mt = 0; mt < C::kMt; ++mt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const float y = v_value<C>(v, tr + r, o_index<C>(mt, g, e));
+                  const float y = v_value<C>(v, r, o_index<C>(mt, g, e));
                   if (!(fabsf(y) <= FLT_MAX)) o[nt][mt][2 * e + i] += x * y;
                 }
             }
@@ -844,61 +862,95 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
   }
   if (units <= 0) return;
 
-  auto fetch = [&](int64_t i) {
-    if (i < units) {
-      const int64_t h = ahead.hr / p.RT, at = ahead.u * C::kKeys;
-      const int64_t row = ahead.b * p.c.sb + h * p.c.sh + at;
-      const int live = (int)imin64(C::kKeys, ahead.s.total - at);
-      const uint32_t st = ring + (uint32_t)(i % C::kStages) * C::kStage;
-      const uint8_t *k = p.c.k + row * C::kRowBytes, *v = p.c.v + row * C::kRowBytes;
-      constexpr int kPieces = C::kKBytes / 16;
+  // This thread's 16-byte pieces of a unit's K (and V): every kThreads-th, at
+  // multiples of kStep from its first one, in memory and in the stage.
+  constexpr int kPieces = C::kKBytes / 16 / kThreads, kStep = 16 * kThreads;
+  static_assert(kPieces * kStep == C::kKBytes, "pieces per thread");
+  const int row0 = threadIdx.x * 16 / C::kRowBytes;
+  const uint32_t dst0 = ring + swizzle<C>(row0, threadIdx.x * 16 % C::kRowBytes);
+  // rows 4 apart (512-byte rows) differ in the swizzle, rows 8 apart do not
+  auto place = [&](int j) { return (dst0 ^ (C::kRowBytes == 512 && j % 2 ? 64u : 0u)) + j * kStep; };
+  const uint8_t *k_at, *v_at;  // the unit fetched next, from this thread's first piece
+  const uint8_t *ks_at = nullptr, *vs_at = nullptr;
+  auto aim = [&]() {
+    const int64_t row = ahead.b * p.c.sb + ahead.h * p.c.sh + (int64_t)ahead.u * C::kKeys;
+    k_at = p.c.k + row * C::kRowBytes + threadIdx.x * 16;
+    v_at = p.c.v + row * C::kRowBytes + threadIdx.x * 16;
+    if constexpr (C::kScaled) {
+      ks_at = p.c.k_scale + row * 4;
+      vs_at = p.c.v_scale + row * 4;
+    }
+  };
+  aim();
+  int64_t to_fetch = units;
+  uint32_t fetch_st = 0;  // stage filled next
+  auto fetch = [&]() {
+    if (to_fetch > 0) {
+      --to_fetch;
+      const int live = ahead.s.total - ahead.u * C::kKeys;
+      const uint32_t st = fetch_st;
+      if (live >= C::kKeys) {
 #pragma unroll
-      for (int j = 0; j < kPieces / kThreads; ++j) {
-        const int piece = threadIdx.x + j * kThreads;
-        const int r = piece / (C::kRowBytes / 16), o = piece % (C::kRowBytes / 16) * 16;
-        const uint32_t dst = st + swizzle<C>(r, o);
-        const int64_t src = r < live ? piece * 16 : 0;
-        cp_async16(dst, k + src, r < live);
-        cp_async16(dst + C::kKBytes, v + src, r < live);
-      }
-      if constexpr (C::kScaled) {
-        for (int r = threadIdx.x; r < 2 * C::kKeys; r += kThreads) {
-          const int rr = r % C::kKeys;
-          const uint8_t *s = r < C::kKeys ? p.c.k_scale : p.c.v_scale;
-          cp_async4(st + 2 * C::kKBytes + 4 * r, s + (row + (rr < live ? rr : 0)) * 4, rr < live);
+        for (int j = 0; j < kPieces; ++j) {
+          cp_async16(st + place(j), k_at + j * kStep);
+          cp_async16(st + place(j) + C::kKBytes, v_at + j * kStep);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+          const bool use = row0 + j * (kStep / C::kRowBytes) < live;
+          cp_async16(st + place(j), use ? k_at + j * kStep : p.c.k, use);
+          cp_async16(st + place(j) + C::kKBytes, use ? v_at + j * kStep : p.c.v, use);
         }
       }
-      ahead.next(p);
+      if constexpr (C::kScaled) {
+#pragma unroll
+        for (int j = 0; j < 2 * C::kKeys / kThreads; ++j) {
+          const int r = threadIdx.x + j * kThreads, rr = r % C::kKeys;
+          const uint8_t *from = r < C::kKeys ? ks_at : vs_at;
+          const bool use = rr < live;
+          cp_async4(ring + st + 2 * C::kKBytes + 4 * r, use ? from + 4 * rr : p.c.k_scale, use);
+        }
+      }
+      fetch_st = fetch_st == (C::kStages - 1) * C::kStage ? 0 : fetch_st + C::kStage;
+      if (ahead.next(p)) {
+        if (to_fetch > 0) aim();
+      } else {
+        k_at += C::kKBytes;
+        v_at += C::kKBytes;
+        if constexpr (C::kScaled) {
+          ks_at += 4 * C::kKeys;
+          vs_at += 4 * C::kKeys;
+        }
+      }
     }
     cp_async_commit();
   };
-  static_assert(C::kKBytes / 16 % kThreads == 0, "pieces per thread");
 
 #pragma unroll 1
-  for (int i = 0; i < C::kStages - 1; ++i) fetch(i);
+  for (int i = 0; i < C::kStages - 1; ++i) fetch();
   Warp<C> w;
   bool fresh = true;  // the segment's queries are not loaded yet
   bool headed = cur.u == 0;  // it begins in this CTA
+  uint32_t st = ring;
 #pragma unroll 1
   for (int64_t i = 0; i < units; ++i) {
-    const int64_t h = cur.hr / p.RT;
-    const int tile = (int)(cur.hr - h * p.RT);
-    if (fresh) w.load_q(p, cur.b, h, tile * C::kRows + rw * 8 * C::kNT);
+    if (fresh) w.load_q(p, cur.b, cur.h, cur.tile * C::kRows + rw * 8 * C::kNT);
     fresh = false;
     cp_async_wait<C::kStages - 2>();
     __syncthreads();  // the unit is here, and the stage refilled next is read
-    fetch(i + C::kStages - 1);
-    const uint32_t st = ring + (uint32_t)(i % C::kStages) * C::kStage;
-    const int64_t key0 = cur.u * C::kKeys;
+    fetch();
+    const int key0 = cur.u * C::kKeys;
 #pragma unroll 1
     for (int j = 0; j < C::kTiles; ++j) {
       const int tr = 16 * (kw + C::kKW * j);
-      if (key0 + tr >= cur.s.total) break;
-      if (key0 + tr + 16 <= cur.s.len)
-        w.template tile<false>(st, st + C::kKBytes, st + 2 * C::kKBytes, tr, key0 + tr, cur.s);
+      if (tr >= cur.s.total - key0) break;
+      if (tr + 16 <= cur.s.len - key0)
+        w.template tile<false>(st, tr, key0 + tr, cur.s);
       else
-        w.template tile<true>(st, st + C::kKBytes, st + 2 * C::kKBytes, tr, key0 + tr, cur.s);
+        w.template tile<true>(st, tr, key0 + tr, cur.s);
     }
+    st = st == ring + (C::kStages - 1) * C::kStage ? ring : st + C::kStage;
 
     const bool done = cur.u + 1 == cur.s.units;
     if (done || i + 1 == units) {
@@ -935,7 +987,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
             const int r = (rw * C::kNT + nt) * 8 + 2 * t + e;
             if (whole) {
               bool live;
-              uint8_t *to = out_row(p, cur.b, h, tile * C::kRows + r, cur.s.n, kSize, live);
+              uint8_t *to = out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, kSize, live);
               const float inv = live && w.l[nt][e] != 0.f ? 1.f / w.l[nt][e] : 0.f;
               if (!to) continue;
 #pragma unroll
@@ -992,7 +1044,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
           }
           if (whole) {
             bool live;
-            uint8_t *to = out_row(p, cur.b, h, tile * C::kRows + r, cur.s.n, kSize, live);
+            uint8_t *to = out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, kSize, live);
             if (to) store_out<C::kF32>(to, dd, live && l != 0.f ? o / l : 0.f);
           } else {
             part[x] = o;
@@ -1006,7 +1058,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
       if (!done && headed && threadIdx.x == 0) {
         // goes on: unit s lies in CTA ((s + 1) * ctas - 1) / all
         const int64_t last = begin + i + (cur.s.units - 1 - cur.u);
-        p.desc[blockIdx.x].seg = cur.b * p.HR + cur.hr;
+        p.desc[blockIdx.x].seg = ((int64_t)cur.b * p.c.H + cur.h) * p.RT + cur.tile;
         p.desc[blockIdx.x].last = (int32_t)(((last + 1) * p.ctas - 1) / all);
       }
       fresh = true;
@@ -1026,11 +1078,11 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Desc desc = p.desc[blockIdx.x];
   if (desc.seg < 0) return;
-  const int64_t b = desc.seg / p.HR, hr = desc.seg - b * p.HR, h = hr / p.RT;
-  const Seq s = sequence<kKeys>(p, b, false);
+  const int64_t bh = desc.seg / p.RT, b = bh / p.c.H, h = bh - b * p.c.H;
+  const Seq s = sequence<kKeys>(p, (int)b, false);
   const int row = blockIdx.y;
   bool live = false;
-  uint8_t *to = out_row(p, b, h, (int)(hr - h * p.RT) * kRows + row, s.n, kF32 ? 4 : 2, live);
+  uint8_t *to = out_row(p, b, h, (int)(desc.seg - bh * p.RT) * kRows + row, s.n, kF32 ? 4 : 2, live);
   if (!to) return;
   constexpr int kVals = D / 32;
   const float *ml = p.part + (int64_t)p.ctas * 2 * kRows * D;
@@ -1112,10 +1164,10 @@ size_t workspace_bytes() {
 template <class C>
 cudaError_t launch(Params p, void *workspace, const DeviceInfo &dev, cudaStream_t stream) {
   p.RT = (p.R + C::kRows - 1) / C::kRows;
-  p.HR = p.c.H * p.RT;
+  const int64_t segs = p.c.B * p.c.H * p.RT;
   const int64_t units = (p.c.L + C::kKeys - 1) / C::kKeys;  // of a segment, at most
   const int64_t most = (dev.sm_count < kMaxSms ? dev.sm_count : kMaxSms) * C::kCtas;
-  p.ctas = (int)imin64(most, units > most ? most : units * (p.c.B * p.HR > most ? most : p.c.B * p.HR));
+  p.ctas = (int)imin64(most, units > most ? most : units * imin64(segs, most));
   p.desc = static_cast<Desc *>(workspace);
   p.part = reinterpret_cast<float *>(p.desc + most);
   cudaError_t err = ensure_smem_attr(reinterpret_cast<const void *>(split_kernel<C>), C::kSmem,
