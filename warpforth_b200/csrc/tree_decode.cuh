@@ -57,6 +57,8 @@ struct Params {
   CacheView c;
   int RT;        // row tiles a head
   int R, G, T;   // query rows a head = G heads x T nodes
+  uint32_t over_T;  // ceil(2^32 / T)
+  bool q_vec, o_vec;  // rows of q (o) are aligned for vector loads (stores)
   int ctas;      // of the grid
   const uint8_t *q;
   uint8_t *o;
@@ -70,6 +72,11 @@ struct Params {
   unsigned int *status;
 };
 
+// r / T, exact for r < 2^26: r (over_T T - 2^32) < r T stays below 2^32.
+__device__ __forceinline__ int over_T(const Params &p, int r) {
+  return p.T == 1 ? r : (int)__umulhi((uint32_t)r, p.over_T);
+}
+
 enum Kind { kF16, kBf16, kTf32 };
 
 template <int kFmt_, int D_, bool kF32_, int kNT_, int kRW_>
@@ -81,25 +88,32 @@ struct Cfg {
                                                             : kF16;
   static constexpr bool kScaled = CacheRow<kFmt, D>::kScaled;
   static constexpr int kRowBytes = CacheRow<kFmt, D>::kBytes;
-  static constexpr int kRows = 8 * kNT * kRW;               // query rows of a CTA
-  static constexpr int kKeys = kRowBytes <= 64 ? 128 : 64;  // keys of a unit
+  static constexpr int kRows = 8 * kNT * kRW;  // query rows of a CTA
+  // keys of a unit: about 16 to 32 KB of K and V
+  static constexpr int kKeys = kRowBytes == 32    ? 256
+                               : kRowBytes == 64  ? (kNT * D > 128 ? 256 : 128)
+                               : kRowBytes == 128 ? 128
+                                                  : 64;
+  // 16-key tiles taken together: two independent chains of products hide their
+  // latency; rows of 256 bytes and more have it hidden by their own length
+  static constexpr int kKT = kRowBytes <= 128 ? 2 : 1;
+  static constexpr int kGroups = kKeys / (16 * kKT * kKW);  // of a warp in a unit
   static constexpr int kKBytes = kKeys * kRowBytes;
-  static constexpr int kStage = 2 * kKBytes + (kScaled ? 8 * kKeys : 0);
-  static constexpr int kOStride = D + 2;  // floats a row of the merge buffer
-  static constexpr int kMerge = kKW > 1 ? kWarps * 8 * kNT * kOStride * 4 : 0;
+  static constexpr int kOStride = D + 4;  // floats a row where warps are joined
+  static constexpr int kMerge = kWarps * 8 * kNT * kOStride * 4;  // in a used stage
+  static constexpr int kData = 2 * kKBytes + (kScaled ? 8 * kKeys : 0);
+  static constexpr int kStage = kData > kMerge ? kData : kMerge;
   static constexpr int kStats = kWarps * 8 * kNT * 2 * 4;
   // CTAs an SM: as many as the registers of the fragments and two stages allow
   static constexpr int kCtas = kRowBytes >= 512                                     ? 1
                                : kRowBytes == 256 || (kF32 ? 2 : kNT) * D == 256 ? 2
-                               : kNT * D <= 64                                      ? 4
+                               : kNT * D <= 64 && kRowBytes <= 64                  ? 4
                                                                                     : 3;
-  static constexpr int kBudget = 227 * 1024 / kCtas - 2048;
-  static constexpr int kFit = (kBudget - kMerge - kStats) / kStage;
+  static constexpr int kFit = (227 * 1024 / kCtas - 2048 - kStats) / kStage;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
   static_assert(kStages >= 2, "shared memory budget");
-  static constexpr int kSmem = kStages * kStage + kMerge + kStats;
-  static constexpr int kTiles = kKeys / 16 / kKW;  // 16-key tiles of a warp in a unit
-  static constexpr int kMt = D / 16;               // row tiles of O^T
+  static constexpr int kSmem = kStages * kStage + kStats;
+  static constexpr int kMt = D / 16;  // row tiles of O^T
 };
 
 // ------------------------------------------------------------- instructions
@@ -214,25 +228,16 @@ __device__ __forceinline__ uint32_t tf32_lo(uint32_t x) {
 // inside 128-byte lines so that the loads of a fragment (8 rows, or 4 row
 // pairs, at one offset) fall into different banks.
 template <class C>
-__device__ __forceinline__ uint32_t swizzle(uint32_t r, uint32_t o) {
-  const uint32_t x = C::kKind == kBf16    ? r & 7
-                     : C::kRowBytes >= 128 ? (r & 6) ^ ((r & 1) << 2)
-                     : C::kRowBytes == 64  ? r & 6
-                                           : (r >> 1) & 2;
-  return (r * C::kRowBytes + o) ^ (x << 4);
+__host__ __device__ constexpr uint32_t swizzle_bits(uint32_t r) {  // linear in the bits of r
+  return (C::kKind == kBf16     ? r & 7
+          : C::kRowBytes >= 128 ? (r & 6) ^ ((r & 1) << 2)
+          : C::kRowBytes == 64  ? r & 6
+                                : (r >> 1) & 2)
+         << 4;
 }
-
-// Which value of the row the element e of product step s, lane column t, is:
-// steps are 16 values (4 elements a lane) or, for tf32, 8 (2 elements).
 template <class C>
-__device__ __forceinline__ int q_index(int s, int t, int e) {
-  if constexpr (C::kKind == kBf16) return 16 * s + 2 * t + (e & 1) + 8 * (e >> 1);
-  if constexpr (C::kKind == kTf32) return 4 * (4 * (s >> 1) + t) + 2 * (s & 1) + e;
-  if constexpr (C::kFmt == WFATTN_CACHE_E4M3)
-    return 16 * (t + 4 * (s >> 2)) + 4 * (s & 3) + e;
-  // int4: codes n and n + 4 of a word make a pair
-  const int n = 2 * (s & 1) + (e >> 1);
-  return (C::D / 4) * t + 8 * (s >> 1) + n + 4 * (e & 1);
+__device__ __forceinline__ uint32_t swizzle(uint32_t r, uint32_t o) {
+  return (r * C::kRowBytes + o) ^ swizzle_bits<C>(r);
 }
 
 // Which value the row g (r = 0) or g + 8 (r = 1) of O^T's tile mt is.
@@ -354,46 +359,98 @@ __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, 
 
 // ------------------------------------------------------------------ kernel
 
+// What a warp holds of a segment: 8 kNT query rows.  Lane 4 g + t has row g of a
+// fragment's 8 (16: g and g + 8) and columns 2t, 2t + 1.
 template <class C>
 struct Warp {
-  // fragments of the queries, and of the output
+  // product steps along a row are 16 values (4 a lane) or, in tf32, 8 (2)
   static constexpr int kSteps = C::kKind == kTf32 ? C::D / 8 : C::D / 16;
+  static constexpr int kE = C::kKind == kTf32 ? 2 : 4;
   static constexpr int kQTerms = C::kKind == kF16 && C::kF32 ? 2 : 1;
+  static constexpr int kPTerms = C::kKind == kBf16 || (C::kKind == kF16 && C::kF32) ? 2 : 1;
   uint32_t q[C::kNT][kSteps][2 * kQTerms];
   float o[C::kNT][C::kMt][4];
-  // per query 2t, 2t + 1 of each n-tile
-  float qf[C::kNT][2], qsum[C::kNT][2];
+  // of queries 2t, 2t + 1 of each 8:
+  float qf[C::kNT][2], qsum[C::kNT][2];  // score = product * qf; sum of q (int4)
   uint64_t word[C::kNT][2];
   float m[C::kNT][2], l[C::kNT][2], om[C::kNT][2];
-  float vinv;  // weights carry scale * vinv
+  float vinv;  // f16 weights carry scale * vinv
 
-  // Loads the query rows `row0`.. of cache head h of sequence b.
+  // The values of one query row that this lane multiplies, step by step.  Any
+  // order along a row will do as long as K's fragments have the same.
+  __device__ __forceinline__ void load_row(const Params &p, int64_t at, float (&x)[kSteps][kE]) {
+    const int t = threadIdx.x & 3;
+    const float *qf32 = reinterpret_cast<const float *>(p.q) + at;
+    const uint16_t *q16 = reinterpret_cast<const uint16_t *>(p.q) + at;
+    if constexpr (C::kKind == kBf16) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint16_t *from = q16 + 16 * s + 8 * i + 2 * t;
+          const uint32_t w = p.q_vec ? *reinterpret_cast<const uint32_t *>(from)
+                                     : from[0] | (uint32_t)from[1] << 16;
+          x[s][2 * i] = ptx::bf16_lo(w), x[s][2 * i + 1] = ptx::bf16_hi(w);
+        }
+      return;
+    }
+    // runs of consecutive values: 4 (tf32), 16 (e4m3), D/4 (int4)
+    constexpr int kRun = C::kKind == kTf32 ? 4 : C::kFmt == WFATTN_CACHE_E4M3 ? 16 : C::D / 4;
+#pragma unroll
+    for (int j = 0; j < C::D / 4 / kRun; ++j) {
+      const int from = kRun * (t + 4 * j);
+      float y[kRun];
+      if constexpr (C::kF32) {
+        if (p.q_vec) {
+#pragma unroll
+          for (int i = 0; i < kRun; i += 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(qf32 + from + i);
+            y[i] = v.x, y[i + 1] = v.y, y[i + 2] = v.z, y[i + 3] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kRun; ++i) y[i] = qf32[from + i];
+        }
+      } else {
+        if (p.q_vec) {
+#pragma unroll
+          for (int i = 0; i < kRun; i += 8) {
+            float v[8];
+            cache_load8<WFATTN_CACHE_BF16>(reinterpret_cast<const uint8_t *>(q16 + from + i), 0, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[i + e] = v[e];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kRun; ++i) y[i] = ptx::bf16_lo(q16[from + i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        if constexpr (C::kFmt == WFATTN_CACHE_INT4)  // codes n and n + 4 of a word are a pair
+          x[2 * (i / 8) + (i & 3) / 2][2 * (i & 1) + (i >> 2 & 1)] = y[i];
+        else
+          x[kRun / kE * j + i / kE][i % kE] = y[i];
+      }
+    }
+  }
+
+  // Begins a segment: loads the query rows row0.. of cache head h of sequence b.
   __device__ __forceinline__ void load_q(const Params &p, int b, int h, int row0) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int nt = 0; nt < C::kNT; ++nt) {
       const int r = row0 + 8 * nt + g;
-      float x[kSteps][C::kKind == kTf32 ? 2 : 4];
-      constexpr int kE = C::kKind == kTf32 ? 2 : 4;
-      float top = 0.f, sum = 0.f;
+      float x[kSteps][kE];
+      float top = 0.f, sum = 0.f, mul = 1.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x[s][e] = 0.f;
       if (r < p.R) {
-        const int hg = r / p.T, node = r - hg * p.T;
-        const int64_t at = b * p.qs.b + ((int64_t)h * p.G + hg) * p.qs.h + node * p.qs.s;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-          for (int e = 0; e < kE; ++e) {
-            const int64_t i = at + q_index<C>(s, t, e);
-            x[s][e] = C::kF32 ? reinterpret_cast<const float *>(p.q)[i]
-                              : ptx::bf16_lo(reinterpret_cast<const uint16_t *>(p.q)[i]);
-          }
-      } else {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-          for (int e = 0; e < kE; ++e) x[s][e] = 0.f;
+        const int hg = over_T(p, r), node = r - hg * p.T;
+        load_row(p, b * p.qs.b + ((int64_t)h * p.G + hg) * p.qs.h + node * p.qs.s, x);
       }
-      float mul = 1.f;
       if constexpr (C::kKind == kF16) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
@@ -429,14 +486,20 @@ struct Warp {
           }
         }
       }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const float f = p.scale_log2 / mul;  // a power of two: exact
+      if constexpr (C::kFmt == WFATTN_CACHE_INT4) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      }
+      // 1 / mul is a power of two as well
+      const float f = p.scale_log2 * __uint_as_float((254u << 23) - __float_as_uint(mul));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {  // from query g to queries 2t, 2t + 1
-        qf[nt][i] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + i));
-        qsum[nt][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i));
-        const int rr = row0 + 8 * nt + 2 * t + i, node = rr % p.T;
+        qf[nt][i] = p.scale_log2;
+        if constexpr (C::kKind == kF16) qf[nt][i] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + i));
+        if constexpr (C::kFmt == WFATTN_CACHE_INT4)
+          qsum[nt][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i));
+        const int rr = row0 + 8 * nt + 2 * t + i;
+        const int node = rr - over_T(p, rr) * p.T;
         word[nt][i] = p.tree ? p.tree[b * p.tree_stride + node] : (2ull << node) - 1;
         m[nt][i] = -FLT_MAX;
         l[nt][i] = om[nt][i] = 0.f;
@@ -449,21 +512,16 @@ struct Warp {
     vinv = __uint_as_float(253u << 23);  // 2^126
   }
 
-  // Attends to the 16 keys of rows tr.. of the stage `st`, key0 their position.
-  // kTail: some of them are nodes of the tree, or no keys.
-  template <bool kTail>
-  __device__ __forceinline__ void tile(uint32_t st, int tr, int key0, const Seq &seq) {
+  // c = K Q^T of the 16 keys at k.
+  __device__ __forceinline__ void scores(uint32_t k, float (&c)[C::kNT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    // rows 16 apart have the same swizzle
-    const uint32_t k = st + tr * C::kRowBytes, v = k + C::kKBytes;
-    const uint32_t scales = st + 2 * C::kKBytes + 4 * tr;
-    float c[C::kNT][4];
+    // two chains: even and odd steps, or in split products the leading one and
+    // the small ones
+    float c2[C::kNT][4];
 #pragma unroll
     for (int nt = 0; nt < C::kNT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) c[nt][e] = 0.f;
-
-    // ---- S^T = K Q^T
+      for (int e = 0; e < 4; ++e) c[nt][e] = c2[nt][e] = 0.f;
     if constexpr (C::kKind == kBf16) {
       const int row = lane & 15;
 #pragma unroll
@@ -471,7 +529,8 @@ struct Warp {
         uint32_t a[4];
         ldmatrix4<false>(k + swizzle<C>(row, 32 * s + 16 * (lane >> 4)), a);
 #pragma unroll
-        for (int nt = 0; nt < C::kNT; ++nt) mma<kBf16>(c[nt], a, q[nt][s][0], q[nt][s][1]);
+        for (int nt = 0; nt < C::kNT; ++nt)
+          mma<kBf16>(s & 1 ? c2[nt] : c[nt], a, q[nt][s][0], q[nt][s][1]);
       }
     } else if constexpr (C::kKind == kTf32) {
 #pragma unroll
@@ -487,8 +546,8 @@ struct Warp {
 #pragma unroll
           for (int nt = 0; nt < C::kNT; ++nt) {
             const uint32_t *qq = q[nt][2 * j + i];
-            mma<kTf32>(c[nt], hi, tf32_lo(qq[0]), tf32_lo(qq[1]));
-            mma<kTf32>(c[nt], lo, tf32_hi(qq[0]), tf32_hi(qq[1]));
+            mma<kTf32>(c2[nt], hi, tf32_lo(qq[0]), tf32_lo(qq[1]));
+            mma<kTf32>(c2[nt], lo, tf32_hi(qq[0]), tf32_hi(qq[1]));
             mma<kTf32>(c[nt], hi, tf32_hi(qq[0]), tf32_hi(qq[1]));
           }
         }
@@ -497,8 +556,8 @@ struct Warp {
       auto step = [&](int s, const uint32_t(&a)[4]) {
 #pragma unroll
         for (int nt = 0; nt < C::kNT; ++nt) {
-          if constexpr (kQTerms == 2) mma<kF16>(c[nt], a, q[nt][s][2], q[nt][s][3]);
-          mma<kF16>(c[nt], a, q[nt][s][0], q[nt][s][1]);
+          if constexpr (kQTerms == 2) mma<kF16>(c2[nt], a, q[nt][s][2], q[nt][s][3]);
+          mma<kF16>(kQTerms == 1 && s & 1 ? c2[nt] : c[nt], a, q[nt][s][0], q[nt][s][1]);
         }
       };
       if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
@@ -539,109 +598,21 @@ struct Warp {
           }
       }
     }
-
-    // ---- scales of keys g and g + 8
-    float vs[2] = {1.f, 1.f}, vm[2] = {0.f, 0.f};
-    if constexpr (C::kScaled) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t at = scales + 4 * (g + 8 * i);
-        const uint32_t ks = lds32(at), vw = lds32(at + 4 * C::kKeys);
-        if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
-          vs[i] = __uint_as_float(vw);
-#pragma unroll
-          for (int nt = 0; nt < C::kNT; ++nt) {
-            c[nt][2 * i] *= __uint_as_float(ks);
-            c[nt][2 * i + 1] *= __uint_as_float(ks);
-          }
-        } else {
-          const float s = ptx::bf16_lo(ks), mid = fmaf(8.f, s, ptx::bf16_hi(ks));
-          vs[i] = ptx::bf16_lo(vw);
-          vm[i] = fmaf(8.f, vs[i], ptx::bf16_hi(vw));
-#pragma unroll
-          for (int nt = 0; nt < C::kNT; ++nt) {
-            c[nt][2 * i] = fmaf(c[nt][2 * i], s, mid * qsum[nt][0]);
-            c[nt][2 * i + 1] = fmaf(c[nt][2 * i + 1], s, mid * qsum[nt][1]);
-          }
-        }
-      }
-    }
-
-    // ---- weights: 2^(score - m), m raised first where a score is far above it
-    float d[C::kNT][4];
-    bool raise = false;
 #pragma unroll
     for (int nt = 0; nt < C::kNT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        d[nt][e] = fmaf(c[nt][e], qf[nt][e & 1], -m[nt][e & 1]);
-        if constexpr (kTail) {
-          const int j = key0 + g + 8 * (e >> 1) - seq.len;
-          if (j >= 0 && (j >= seq.n || !(word[nt][e & 1] >> j & 1))) d[nt][e] = -INFINITY;
-        }
-        raise = raise || d[nt][e] > 4.f;
-      }
-    if constexpr (C::kScaled) raise = raise || fmaxf(vs[0], vs[1]) * vinv > 2048.f;
-    if (__any_sync(0xffffffffu, raise)) {
-      float ratio = 1.f;
-      if constexpr (C::kScaled) {
-        float top = fmaxf(vs[0], vs[1]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        if (top * vinv > 2048.f) {  // the same in the whole warp
-          // 2^7 <= top * vinv < 2^8: weights of 2^4 times scales up to 2^11
-          // stay below 2^16, and a weight has all its 11 bits down to 2^-21
-          const int f = min(max(261 - (int)(__float_as_uint(top) >> 23), 1), 253);
-          const float now = __uint_as_float((uint32_t)f << 23);
-          ratio = now / vinv;
-          vinv = now;
-        }
-      }
+      for (int e = 0; e < 4; ++e) c[nt][e] += c2[nt][e];
+  }
+
+  // The weights of a tile as the narrow operand of V^T P^T.
+  struct Probs {
+    uint32_t b[C::kNT][C::kKind == kTf32 ? 1 : kPTerms][2];  // [term][keys 0-7, 8-15]
+    float f[C::kNT][C::kKind == kTf32 ? 4 : 1];  // tf32: query g, keys 2t, 2t + 1 of each half
+  };
+  // pv: weights of keys g, g + 8 (by pairs) for queries 2t, 2t + 1
+  __device__ __forceinline__ void operands(const float (&pv)[C::kNT][4], Probs &pr) {
 #pragma unroll
-      for (int nt = 0; nt < C::kNT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float top = m[nt][i];
-#pragma unroll
-          for (int e = i; e < 4; e += 2)
-            if (d[nt][e] != -INFINITY) top = fmaxf(top, c[nt][e] * qf[nt][i]);
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float f = ptx::ex2_approx(m[nt][i] - top);
-          m[nt][i] = top;
-          l[nt][i] *= f;
-          om[nt][i] *= f;
-#pragma unroll
-          for (int e = i; e < 4; e += 2)
-            if (d[nt][e] != -INFINITY) d[nt][e] = fmaf(c[nt][e], qf[nt][i], -top);
-#pragma unroll
-          for (int mt = 0; mt < C::kMt; ++mt) {
-            o[nt][mt][i] *= f * ratio;
-            o[nt][mt][2 + i] *= f * ratio;
-          }
-        }
-    }
-    // P^T as the narrow operand: [term][keys 0-7, 8-15]
-    constexpr int kPTerms = C::kKind == kBf16 || (C::kKind == kF16 && C::kF32) ? 2 : 1;
-    uint32_t pb[C::kNT][kPTerms][2];
-    float pf[C::kNT][4];  // tf32: weight of query g at keys 2t, 2t+1 of each half
-    float pv[C::kNT][4];
-    const float w[2] = {vs[0] * vinv, vs[1] * vinv};
-#pragma unroll
-    for (int nt = 0; nt < C::kNT; ++nt) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = ptx::ex2_approx(d[nt][e]);
-        l[nt][e & 1] += x;
-        pv[nt][e] = C::kScaled ? x * w[e >> 1] : x;
-        if (kTail && C::kScaled && d[nt][e] == -INFINITY) pv[nt][e] = 0.f;  // scale NaN
-        if constexpr (C::kFmt == WFATTN_CACHE_INT4) {
-          const float y = x * vm[e >> 1];
-          om[nt][e & 1] += kTail && d[nt][e] == -INFINITY ? 0.f : y;
-        }
-      }
+    for (int nt = 0; nt < C::kNT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float x = pv[nt][2 * i], y = pv[nt][2 * i + 1];
@@ -649,25 +620,30 @@ struct Warp {
           const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
           const uint32_t hi = movmatrix(__byte_perm(a, b, 0x7632));
           const uint32_t lo = movmatrix(__byte_perm(a, b, 0x5410));
-          pf[nt][2 * i] = __uint_as_float(__byte_perm(lo, hi, 0x5410));
-          pf[nt][2 * i + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
+          pr.f[nt][2 * i] = __uint_as_float(__byte_perm(lo, hi, 0x5410));
+          pr.f[nt][2 * i + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
         } else if constexpr (C::kKind == kBf16) {
           const uint32_t hi = ptx::pack_bf16x2(x, y);
-          pb[nt][0][i] = movmatrix(hi);
-          pb[nt][1][i] = movmatrix(ptx::pack_bf16x2(x - ptx::bf16_lo(hi), y - ptx::bf16_hi(hi)));
+          pr.b[nt][0][i] = movmatrix(hi);
+          pr.b[nt][1][i] =
+              movmatrix(ptx::pack_bf16x2(x - ptx::bf16_lo(hi), y - ptx::bf16_hi(hi)));
         } else {
           const uint32_t hi = pack_f16x2(x, y);
-          pb[nt][0][i] = movmatrix(hi);
+          pr.b[nt][0][i] = movmatrix(hi);
           if constexpr (kPTerms == 2) {
             const float2 f = ptx::f16x2_to_f32(hi);
-            pb[nt][1][i] = movmatrix(pack_f16x2(x - f.x, y - f.y));
+            pr.b[nt][1][i] = movmatrix(pack_f16x2(x - f.x, y - f.y));
           }
         }
       }
-    }
+  }
 
-    // ---- O^T += V^T P^T
-    bool odd = false;  // tail: V holds something that is not finite
+  // O^T += V^T P^T over the 16 keys at v.  kTail: what of V is not finite is
+  // left out, and the return value tells whether there is any.
+  template <bool kTail>
+  __device__ __forceinline__ bool values(uint32_t v, const Probs &pr) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    bool odd = false;
     // f32 results: a tile's product is added in f32 arithmetic, so that cut
     // bits do not pile up along the keys
     auto add = [&](int mt, uint32_t(&a)[4]) {
@@ -683,14 +659,14 @@ struct Warp {
       for (int nt = 0; nt < C::kNT; ++nt) {
         if constexpr (C::kF32) {
           float z[4] = {0.f, 0.f, 0.f, 0.f};
-          if constexpr (kPTerms == 2) mma<C::kKind>(z, a, pb[nt][1][0], pb[nt][1][1]);
-          mma<C::kKind>(z, a, pb[nt][0][0], pb[nt][0][1]);
+          if constexpr (kPTerms == 2) mma<C::kKind>(z, a, pr.b[nt][1][0], pr.b[nt][1][1]);
+          mma<C::kKind>(z, a, pr.b[nt][0][0], pr.b[nt][0][1]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[nt][mt][e] += z[e];
         } else {
           if constexpr (kPTerms == 2)
-            mma<C::kKind>(o[nt][mt], a, pb[nt][1][0], pb[nt][1][1]);
-          mma<C::kKind>(o[nt][mt], a, pb[nt][0][0], pb[nt][0][1]);
+            mma<C::kKind>(o[nt][mt], a, pr.b[nt][1][0], pr.b[nt][1][1]);
+          mma<C::kKind>(o[nt][mt], a, pr.b[nt][0][0], pr.b[nt][0][1]);
         }
       }
     };
@@ -705,42 +681,40 @@ struct Warp {
     } else if constexpr (C::kKind == kTf32) {
 #pragma unroll
       for (int h = 0; h < C::D / 32; ++h) {
-        uint4 x[4];  // keys 2t, 2t + 1 of each half
+        uint32_t x[4][4];  // keys 2t, 2t + 1 of each half
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[i] = lds128(v + swizzle<C>(2 * t + (i & 1) + 8 * (i >> 1), 16 * (g + 8 * h)));
+          const uint4 y = lds128(v + swizzle<C>(2 * t + (i & 1) + 8 * (i >> 1), 16 * (g + 8 * h)));
+          x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
           if constexpr (kTail) {
-            uint32_t *y = &x[i].x;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if ((y[e] & 0x7f800000u) == 0x7f800000u) y[e] = 0, odd = true;
+              if ((x[i][e] & 0x7f800000u) == 0x7f800000u) x[i][e] = 0, odd = true;
           }
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int mt = 2 * h + j;
           uint32_t hi[2][4], lo[2][4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t a[4] = {j ? x[2 * i].z : x[2 * i].x, j ? x[2 * i].w : x[2 * i].y,
-                                   j ? x[2 * i + 1].z : x[2 * i + 1].x,
-                                   j ? x[2 * i + 1].w : x[2 * i + 1].y};
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) hi[i][e] = tf32_hi(a[e]), lo[i][e] = tf32_lo(a[e]);
-          }
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t a = x[2 * i + (e >> 1)][2 * j + (e & 1)];
+              hi[i][e] = tf32_hi(a), lo[i][e] = tf32_lo(a);
+            }
 #pragma unroll
           for (int nt = 0; nt < C::kNT; ++nt) {
             float z[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint32_t p0 = __float_as_uint(pf[nt][2 * i]);
-              const uint32_t p1 = __float_as_uint(pf[nt][2 * i + 1]);
+              const uint32_t p0 = __float_as_uint(pr.f[nt][2 * i]);
+              const uint32_t p1 = __float_as_uint(pr.f[nt][2 * i + 1]);
               mma<kTf32>(z, hi[i], tf32_lo(p0), tf32_lo(p1));
               mma<kTf32>(z, lo[i], tf32_hi(p0), tf32_hi(p1));
               mma<kTf32>(z, hi[i], tf32_hi(p0), tf32_hi(p1));
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[nt][mt][e] += z[e];
+            for (int e = 0; e < 4; ++e) o[nt][2 * h + j][e] += z[e];
           }
         }
       }
@@ -796,28 +770,189 @@ struct Warp {
           }
         }
     }
-    if constexpr (kTail && C::kFmt != WFATTN_CACHE_INT4) {
-      // What is not finite was left out of the products, where a weight of 0
-      // would spread it: queries that see its key get it here.
-      if (__any_sync(0xffffffffu, odd)) {
+    return odd;
+  }
+
+  // What values<true>() left out, where a weight of 0 would have spread it:
+  // queries that see its key get it here.  pv: < 0 where the key is not seen.
+  __device__ __forceinline__ void not_finite(uint32_t v, const float (&pv)[C::kNT][4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if constexpr (C::kFmt != WFATTN_CACHE_INT4) {
 #pragma unroll 1
-        for (int r = 0; r < 16; ++r)
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float x = __shfl_sync(0xffffffffu, r < 8 ? pv[nt][i] : pv[nt][2 + i],
+                                        4 * (r & 7) + t);
+            if (x < 0.f) continue;
+#pragma unroll
+            for (int mt = 0; mt < C::kMt; ++mt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float y = v_value<C>(v, r, o_index<C>(mt, g, e));
+                if (!(fabsf(y) <= FLT_MAX)) o[nt][mt][2 * e + i] += x * y;
+              }
+          }
+    }
+  }
+
+  // Attends to the 16 kKT keys of rows tr.. of the stage `st`, key0 their
+  // position.  tail: some of them are nodes of the tree, or no keys.
+  __device__ __forceinline__ void group(uint32_t st, int tr, int key0, const Seq &seq) {
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    const bool tail = key0 + 16 * C::kKT > seq.len;
+    const uint32_t k = st + tr * C::kRowBytes;  // rows 16 apart have the same swizzle
+    const uint32_t scales = st + 2 * C::kKBytes + 4 * (tr + g);
+    float c[C::kKT][C::kNT][4], vs[C::kKT][2], vm[C::kKT][2];
+#pragma unroll
+    for (int j = 0; j < C::kKT; ++j) scores(k + 16 * j * C::kRowBytes, c[j]);
+
+    // ---- scales of keys g and g + 8
+    if constexpr (C::kScaled) {
+#pragma unroll
+      for (int j = 0; j < C::kKT; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t at = scales + 4 * (16 * j + 8 * i);
+          const uint32_t ks = lds32(at), vw = lds32(at + 4 * C::kKeys);
+          if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
+            vs[j][i] = __uint_as_float(vw);
+#pragma unroll
+            for (int nt = 0; nt < C::kNT; ++nt) {
+              c[j][nt][2 * i] *= __uint_as_float(ks);
+              c[j][nt][2 * i + 1] *= __uint_as_float(ks);
+            }
+          } else {
+            const float s = ptx::bf16_lo(ks), mid = fmaf(8.f, s, ptx::bf16_hi(ks));
+            vs[j][i] = ptx::bf16_lo(vw);
+            vm[j][i] = fmaf(8.f, vs[j][i], ptx::bf16_hi(vw));
+#pragma unroll
+            for (int nt = 0; nt < C::kNT; ++nt) {
+              c[j][nt][2 * i] = fmaf(c[j][nt][2 * i], s, mid * qsum[nt][0]);
+              c[j][nt][2 * i + 1] = fmaf(c[j][nt][2 * i + 1], s, mid * qsum[nt][1]);
+            }
+          }
+        }
+    }
+
+    // ---- weights: 2^(score - m), m raised first where a score is far above it
+    float d[C::kKT][C::kNT][4], high = -INFINITY, vtop = 0.f;
+#pragma unroll
+    for (int j = 0; j < C::kKT; ++j) {
+#pragma unroll
+      for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          d[j][nt][e] = fmaf(c[j][nt][e], qf[nt][e & 1], -m[nt][e & 1]);
+      if constexpr (C::kScaled) vtop = fmaxf(vtop, fmaxf(vs[j][0], vs[j][1]));
+    }
+    if (tail) {
+#pragma unroll
+      for (int j = 0; j < C::kKT; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int node = key0 + 16 * j + 8 * i + g - seq.len;
 #pragma unroll
           for (int nt = 0; nt < C::kNT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float mine = r < 8 ? (d[nt][i] == -INFINITY ? -1.f : pv[nt][i])
-                                       : (d[nt][2 + i] == -INFINITY ? -1.f : pv[nt][2 + i]);
-              const float x = __shfl_sync(0xffffffffu, mine, 4 * (r & 7) + t);
-              if (x < 0.f) continue;
+            for (int e = 0; e < 2; ++e)
+              if (node >= 0 && (node >= seq.n || !(word[nt][e] >> node & 1)))
+                d[j][nt][2 * i + e] = -INFINITY;
+        }
+    }
 #pragma unroll
-              for (int mt = 0; mt < C::kMt; ++mt)
+    for (int j = 0; j < C::kKT; ++j)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float y = v_value<C>(v, r, o_index<C>(mt, g, e));
-                  if (!(fabsf(y) <= FLT_MAX)) o[nt][mt][2 * e + i] += x * y;
-                }
-            }
+      for (int nt = 0; nt < C::kNT; ++nt)
+        high = fmaxf(high, fmaxf(ptx::fmax3(d[j][nt][0], d[j][nt][1], d[j][nt][2]), d[j][nt][3]));
+    bool raise = high > 4.f;
+    if constexpr (C::kScaled) raise = raise || vtop * vinv > 2048.f;
+    if (__any_sync(0xffffffffu, raise)) {
+      float ratio = 1.f;
+      if constexpr (C::kScaled) {
+        float top = vtop;
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        if (top * vinv > 2048.f) {  // the same in the whole warp
+          // 2^7 <= top * vinv < 2^8: weights of 2^4 times scales up to 2^11
+          // stay below 2^16, and a weight has all its 11 bits down to 2^-21
+          const int f = min(max(261 - (int)(__float_as_uint(top) >> 23), 1), 253);
+          const float now = __uint_as_float((uint32_t)f << 23);
+          ratio = now / vinv;
+          vinv = now;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float top = m[nt][i];
+#pragma unroll
+          for (int j = 0; j < C::kKT; ++j)
+#pragma unroll
+            for (int e = i; e < 4; e += 2)
+              if (d[j][nt][e] != -INFINITY) top = fmaxf(top, c[j][nt][e] * qf[nt][i]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float f = ptx::ex2_approx(m[nt][i] - top);
+          m[nt][i] = top;
+          l[nt][i] *= f;
+          om[nt][i] *= f;
+#pragma unroll
+          for (int j = 0; j < C::kKT; ++j)
+#pragma unroll
+            for (int e = i; e < 4; e += 2)
+              if (d[j][nt][e] != -INFINITY) d[j][nt][e] = fmaf(c[j][nt][e], qf[nt][i], -top);
+#pragma unroll
+          for (int mt = 0; mt < C::kMt; ++mt) {
+            o[nt][mt][i] *= f * ratio;
+            o[nt][mt][2 + i] *= f * ratio;
+          }
+        }
+    }
+
+    float pv[C::kKT][C::kNT][4];
+    Probs pr[C::kKT];
+#pragma unroll
+    for (int j = 0; j < C::kKT; ++j) {
+      const float w[2] = {vs[j][0] * vinv, vs[j][1] * vinv};
+#pragma unroll
+      for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = ptx::ex2_approx(d[j][nt][e]);
+          l[nt][e & 1] += x;
+          pv[j][nt][e] = C::kScaled ? x * w[e >> 1] : x;
+          if constexpr (C::kFmt == WFATTN_CACHE_INT4) {
+            float y = x * vm[j][e >> 1];
+            if (tail && d[j][nt][e] == -INFINITY) y = 0.f;  // a scale may be NaN
+            om[nt][e & 1] += y;
+          }
+          if (C::kScaled && tail && d[j][nt][e] == -INFINITY) pv[j][nt][e] = 0.f;
+        }
+      operands(pv[j], pr[j]);
+    }
+    if (!tail) {
+#pragma unroll
+      for (int j = 0; j < C::kKT; ++j)
+        values<false>(k + C::kKBytes + 16 * j * C::kRowBytes, pr[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::kKT; ++j) {
+        const uint32_t v = k + C::kKBytes + 16 * j * C::kRowBytes;
+        const bool odd = values<true>(v, pr[j]);
+        if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+          for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (d[j][nt][e] == -INFINITY) pv[j][nt][e] = -1.f;
+          not_finite(v, pv[j]);
+        }
       }
     }
   }
@@ -828,7 +963,7 @@ struct Warp {
 __device__ __forceinline__ uint8_t *out_row(const Params &p, int64_t b, int64_t h, int r, int n,
                                             int size, bool &live) {
   if (r >= p.R) return nullptr;
-  const int hg = r / p.T, node = r - hg * p.T;
+  const int hg = over_T(p, r), node = r - hg * p.T;
   live = node < n;
   return p.o + (b * p.os.b + (h * p.G + hg) * p.os.h + node * p.os.s) * size;
 }
@@ -841,11 +976,26 @@ __device__ __forceinline__ void store_out(uint8_t *row, int d, float x) {
     reinterpret_cast<uint16_t *>(row)[d] = (uint16_t)ptx::pack_bf16x2(x, 0.f);
 }
 
+// Four values d.. of an output row.
+template <bool kF32>
+__device__ __forceinline__ void store_out4(const Params &p, uint8_t *row, int d, float4 x) {
+  if (p.o_vec && kF32) {
+    *reinterpret_cast<float4 *>(row + 4 * d) = x;
+  } else if (p.o_vec) {
+    *reinterpret_cast<uint2 *>(row + 2 * d) =
+        make_uint2(ptx::pack_bf16x2(x.x, x.y), ptx::pack_bf16x2(x.z, x.w));
+  } else {
+    store_out<kF32>(row, d, x.x);
+    store_out<kF32>(row, d + 1, x.y);
+    store_out<kF32>(row, d + 2, x.z);
+    store_out<kF32>(row, d + 3, x.w);
+  }
+}
+
 template <class C>
 __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  float *merge = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
-  float *stats = reinterpret_cast<float *>(smem + C::kStages * C::kStage + C::kMerge);
+  float *stats = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
   const uint32_t ring = ptx::smem_u32(smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rw = warp / C::kKW, kw = warp % C::kKW;
@@ -862,20 +1012,30 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
   }
   if (units <= 0) return;
 
-  // This thread's 16-byte pieces of a unit's K (and V): every kThreads-th, at
-  // multiples of kStep from its first one, in memory and in the stage.
-  constexpr int kPieces = C::kKBytes / 16 / kThreads, kStep = 16 * kThreads;
-  static_assert(kPieces * kStep == C::kKBytes, "pieces per thread");
-  const int row0 = threadIdx.x * 16 / C::kRowBytes;
-  const uint32_t dst0 = ring + swizzle<C>(row0, threadIdx.x * 16 % C::kRowBytes);
-  // rows 4 apart (512-byte rows) differ in the swizzle, rows 8 apart do not
-  auto place = [&](int j) { return (dst0 ^ (C::kRowBytes == 512 && j % 2 ? 64u : 0u)) + j * kStep; };
+  // Who loads what of a unit: where every warp reads keys of its own, each warp
+  // loads those and waits for nobody else; otherwise the CTA loads together.
+  // A loader's 16-byte pieces of K (and V) lie kStep apart, in kRuns runs.
+  constexpr bool kOwn = C::kRW == 1;
+  constexpr int kLoaders = kOwn ? 32 : kThreads, kStep = 16 * kLoaders;
+  constexpr int kRuns = kOwn ? C::kGroups : 1;  // a group's rows, kApart rows from the next
+  constexpr int kRunRows = kOwn ? 16 * C::kKT : C::kKeys, kApart = 16 * C::kKT * C::kKW;
+  constexpr int kPieces = kRunRows * C::kRowBytes / kStep;
+  static_assert(kPieces * kStep == kRunRows * C::kRowBytes, "whole pieces");
+  const int loader = kOwn ? lane : threadIdx.x;
+  const int first = kOwn ? kw * kRunRows : 0;        // row
+  const int row0 = loader * 16 / C::kRowBytes;       // in the first kStep bytes of a run
+  const uint32_t dst0 = ring + first * C::kRowBytes + swizzle<C>(row0, loader * 16 % C::kRowBytes);
+  // `first` and runs are multiples of 16 rows, so the swizzle is row0's and the step's
+  auto place = [&](int run, int j) {
+    return (dst0 ^ swizzle_bits<C>(j * kStep / C::kRowBytes)) + j * kStep +
+           run * kApart * C::kRowBytes;
+  };
   const uint8_t *k_at, *v_at;  // the unit fetched next, from this thread's first piece
   const uint8_t *ks_at = nullptr, *vs_at = nullptr;
   auto aim = [&]() {
-    const int64_t row = ahead.b * p.c.sb + ahead.h * p.c.sh + (int64_t)ahead.u * C::kKeys;
-    k_at = p.c.k + row * C::kRowBytes + threadIdx.x * 16;
-    v_at = p.c.v + row * C::kRowBytes + threadIdx.x * 16;
+    const int64_t row = ahead.b * p.c.sb + ahead.h * p.c.sh + (int64_t)ahead.u * C::kKeys + first;
+    k_at = p.c.k + row * C::kRowBytes + loader * 16;
+    v_at = p.c.v + row * C::kRowBytes + loader * 16;
     if constexpr (C::kScaled) {
       ks_at = p.c.k_scale + row * 4;
       vs_at = p.c.v_scale + row * 4;
@@ -887,30 +1047,43 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
   auto fetch = [&]() {
     if (to_fetch > 0) {
       --to_fetch;
-      const int live = ahead.s.total - ahead.u * C::kKeys;
+      const int live = ahead.s.total - ahead.u * C::kKeys - first;  // rows from `first` on
       const uint32_t st = fetch_st;
-      if (live >= C::kKeys) {
+      if (live >= kRunRows + (kRuns - 1) * kApart) {
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j) {
-          cp_async16(st + place(j), k_at + j * kStep);
-          cp_async16(st + place(j) + C::kKBytes, v_at + j * kStep);
-        }
+        for (int r = 0; r < kRuns; ++r)
+#pragma unroll
+          for (int j = 0; j < kPieces; ++j) {
+            const int off = j * kStep + r * kApart * C::kRowBytes;
+            cp_async16(st + place(r, j), k_at + off);
+            cp_async16(st + place(r, j) + C::kKBytes, v_at + off);
+          }
       } else {
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j) {
-          const bool use = row0 + j * (kStep / C::kRowBytes) < live;
-          cp_async16(st + place(j), use ? k_at + j * kStep : p.c.k, use);
-          cp_async16(st + place(j) + C::kKBytes, use ? v_at + j * kStep : p.c.v, use);
-        }
+        for (int r = 0; r < kRuns; ++r)
+#pragma unroll
+          for (int j = 0; j < kPieces; ++j) {
+            const int off = j * kStep + r * kApart * C::kRowBytes;
+            const bool use = row0 + j * (kStep / C::kRowBytes) + r * kApart < live;
+            cp_async16(st + place(r, j), use ? k_at + off : p.c.k, use);
+            cp_async16(st + place(r, j) + C::kKBytes, use ? v_at + off : p.c.v, use);
+          }
       }
       if constexpr (C::kScaled) {
+        // a run's scales of K, then those of V
+        constexpr int kWords = 2 * kRunRows / kLoaders;
 #pragma unroll
-        for (int j = 0; j < 2 * C::kKeys / kThreads; ++j) {
-          const int r = threadIdx.x + j * kThreads, rr = r % C::kKeys;
-          const uint8_t *from = r < C::kKeys ? ks_at : vs_at;
-          const bool use = rr < live;
-          cp_async4(ring + st + 2 * C::kKBytes + 4 * r, use ? from + 4 * rr : p.c.k_scale, use);
-        }
+        for (int r = 0; r < kRuns; ++r)
+#pragma unroll
+          for (int j = 0; j < kWords; ++j) {
+            const int i = loader + j * kLoaders;
+            const int row = (i % kRunRows) + r * kApart;
+            const uint8_t *from = i < kRunRows ? ks_at : vs_at;
+            const bool use = row < live;
+            cp_async4(ring + st + 2 * C::kKBytes + 4 * (first + row) +
+                          (i < kRunRows ? 0 : 4 * C::kKeys),
+                      use ? from + 4 * row : p.c.k_scale, use);
+          }
       }
       fetch_st = fetch_st == (C::kStages - 1) * C::kStage ? 0 : fetch_st + C::kStage;
       if (ahead.next(p)) {
@@ -930,27 +1103,27 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
 #pragma unroll 1
   for (int i = 0; i < C::kStages - 1; ++i) fetch();
   Warp<C> w;
-  bool fresh = true;  // the segment's queries are not loaded yet
+  bool fresh = true;         // the segment's queries are not loaded yet
   bool headed = cur.u == 0;  // it begins in this CTA
-  uint32_t st = ring;
+  uint32_t st = 0;
 #pragma unroll 1
   for (int64_t i = 0; i < units; ++i) {
     if (fresh) w.load_q(p, cur.b, cur.h, cur.tile * C::kRows + rw * 8 * C::kNT);
     fresh = false;
     cp_async_wait<C::kStages - 2>();
-    __syncthreads();  // the unit is here, and the stage refilled next is read
+    // the unit is here, and the stage refilled next has been read
+    if constexpr (kOwn)
+      __syncwarp();
+    else
+      __syncthreads();
     fetch();
     const int key0 = cur.u * C::kKeys;
 #pragma unroll 1
-    for (int j = 0; j < C::kTiles; ++j) {
-      const int tr = 16 * (kw + C::kKW * j);
+    for (int j = 0; j < C::kGroups; ++j) {
+      const int tr = 16 * C::kKT * (kw + C::kKW * j);
       if (tr >= cur.s.total - key0) break;
-      if (tr + 16 <= cur.s.len - key0)
-        w.template tile<false>(st, tr, key0 + tr, cur.s);
-      else
-        w.template tile<true>(st, tr, key0 + tr, cur.s);
+      w.group(ring + st, tr, key0 + tr, cur.s);
     }
-    st = st == ring + (C::kStages - 1) * C::kStage ? ring : st + C::kStage;
 
     const bool done = cur.u + 1 == cur.s.units;
     if (done || i + 1 == units) {
@@ -967,10 +1140,12 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
             if constexpr (C::kFmt == WFATTN_CACHE_INT4)
               w.om[nt][e] += __shfl_xor_sync(0xffffffffu, w.om[nt][e], x);
           }
+          if constexpr (C::kScaled) {
 #pragma unroll
-          for (int mt = 0; mt < C::kMt; ++mt) {
-            w.o[nt][mt][e] = w.o[nt][mt][e] * back + w.om[nt][e];
-            w.o[nt][mt][2 + e] = w.o[nt][mt][2 + e] * back + w.om[nt][e];
+            for (int mt = 0; mt < C::kMt; ++mt) {
+              w.o[nt][mt][e] = w.o[nt][mt][e] * back + w.om[nt][e];
+              w.o[nt][mt][2 + e] = w.o[nt][mt][2 + e] * back + w.om[nt][e];
+            }
           }
         }
       const int slot = headed ? 1 : 0;
@@ -978,83 +1153,67 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
       float *part_ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D +
                        (int64_t)(blockIdx.x * 2 + slot) * C::kRows * 2;
       constexpr int kSize = C::kF32 ? 4 : 2;
-      if constexpr (C::kKW == 1) {
-        // the warp has all the keys of its rows
+      // The warps' sums meet in the stage just read: rows of O, and beside them
+      // maximum and sum.  (With all the keys in one warp this only turns the
+      // fragments into rows.)
+      __syncthreads();
+      float *mine = reinterpret_cast<float *>(smem + st) + warp * 8 * C::kNT * C::kOStride;
 #pragma unroll
-        for (int nt = 0; nt < C::kNT; ++nt)
+      for (int nt = 0; nt < C::kNT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r = (rw * C::kNT + nt) * 8 + 2 * t + e;
-            if (whole) {
-              bool live;
-              uint8_t *to = out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, kSize, live);
-              const float inv = live && w.l[nt][e] != 0.f ? 1.f / w.l[nt][e] : 0.f;
-              if (!to) continue;
+        for (int e = 0; e < 2; ++e) {
+          const int r = 8 * nt + 2 * t + e;
 #pragma unroll
-              for (int mt = 0; mt < C::kMt; ++mt)
+          for (int mt = 0; mt < C::kMt; ++mt)
 #pragma unroll
-                for (int y = 0; y < 2; ++y)
-                  store_out<C::kF32>(to, o_index<C>(mt, g, y),
-                                     inv == 0.f ? 0.f : w.o[nt][mt][2 * y + e] * inv);
-            } else {
-#pragma unroll
-              for (int mt = 0; mt < C::kMt; ++mt)
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-                  part[r * C::D + o_index<C>(mt, g, y)] = w.o[nt][mt][2 * y + e];
-              if (g == 0) {
-                part_ml[2 * r] = w.m[nt][e];
-                part_ml[2 * r + 1] = w.l[nt][e];
-              }
-            }
+            for (int y = 0; y < 2; ++y)
+              mine[r * C::kOStride + o_index<C>(mt, g, y)] = w.o[nt][mt][2 * y + e];
+          if (g == 0) {
+            stats[(warp * 8 * C::kNT + r) * 2] = w.m[nt][e];
+            stats[(warp * 8 * C::kNT + r) * 2 + 1] = w.l[nt][e];
           }
-      } else {
-        // join the warps that have the other keys of the rows
-        float *mine = merge + warp * 8 * C::kNT * C::kOStride;
-#pragma unroll
-        for (int nt = 0; nt < C::kNT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r = 8 * nt + 2 * t + e;
-#pragma unroll
-            for (int mt = 0; mt < C::kMt; ++mt)
-#pragma unroll
-              for (int y = 0; y < 2; ++y)
-                mine[r * C::kOStride + o_index<C>(mt, g, y)] = w.o[nt][mt][2 * y + e];
-            if (g == 0) {
-              stats[(warp * 8 * C::kNT + r) * 2] = w.m[nt][e];
-              stats[(warp * 8 * C::kNT + r) * 2 + 1] = w.l[nt][e];
-            }
-          }
-        __syncthreads();
+        }
+      __syncthreads();
 #pragma unroll 1
-        for (int x = threadIdx.x; x < C::kRows * C::D; x += kThreads) {
-          const int r = x / C::D, dd = x % C::D;
-          const int rr = r % (8 * C::kNT), w0 = r / (8 * C::kNT) * C::kKW;
-          float m = -FLT_MAX, l = 0.f, o = 0.f;
+      for (int x = threadIdx.x; x < C::kRows * C::D / 4; x += kThreads) {
+        const int r = x / (C::D / 4), dd = x % (C::D / 4) * 4;
+        const int at0 = r / (8 * C::kNT) * C::kKW * 8 * C::kNT + r % (8 * C::kNT);
+        float m = -FLT_MAX, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int y = 0; y < C::kKW; ++y)
-            m = fmaxf(m, stats[((w0 + y) * 8 * C::kNT + rr) * 2]);
+        for (int y = 0; y < C::kKW; ++y) m = fmaxf(m, stats[(at0 + y * 8 * C::kNT) * 2]);
 #pragma unroll
-          for (int y = 0; y < C::kKW; ++y) {
-            const int at = (w0 + y) * 8 * C::kNT + rr;
-            const float f = ptx::ex2_approx(stats[at * 2] - m);
-            l = fmaf(stats[at * 2 + 1], f, l);
-            o = fmaf(merge[at * C::kOStride + dd], f, o);
+        for (int y = 0; y < C::kKW; ++y) {
+          const int at = at0 + y * 8 * C::kNT;
+          const float f = ptx::ex2_approx(stats[at * 2] - m);
+          const float4 z =
+              *reinterpret_cast<const float4 *>(smem + st + (at * C::kOStride + dd) * 4);
+          l = fmaf(stats[at * 2 + 1], f, l);
+          o.x = fmaf(z.x, f, o.x), o.y = fmaf(z.y, f, o.y);
+          o.z = fmaf(z.z, f, o.z), o.w = fmaf(z.w, f, o.w);
+        }
+        if (whole) {
+          bool live;
+          uint8_t *to =
+              out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, kSize, live);
+          if (to) {
+            const bool some = live && l != 0.f;
+            const float inv = 1.f / l;
+            store_out4<C::kF32>(p, to, dd,
+                                some ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv)
+                                     : make_float4(0.f, 0.f, 0.f, 0.f));
           }
-          if (whole) {
-            bool live;
-            uint8_t *to = out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, kSize, live);
-            if (to) store_out<C::kF32>(to, dd, live && l != 0.f ? o / l : 0.f);
-          } else {
-            part[x] = o;
-            if (dd == 0) {
-              part_ml[2 * r] = m;
-              part_ml[2 * r + 1] = l;
-            }
+        } else {
+          *reinterpret_cast<float4 *>(part + r * C::D + dd) = o;
+          if (dd == 0) {
+            part_ml[2 * r] = m;
+            part_ml[2 * r + 1] = l;
           }
         }
       }
+      // the stage may be refilled once all have read it (with common loads the
+      // next unit's barrier says so)
+      if constexpr (kOwn) __syncthreads();
       if (!done && headed && threadIdx.x == 0) {
         // goes on: unit s lies in CTA ((s + 1) * ctas - 1) / all
         const int64_t last = begin + i + (cur.s.units - 1 - cur.u);
@@ -1064,6 +1223,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
       fresh = true;
       headed = true;
     }
+    st = st == (C::kStages - 1) * C::kStage ? 0 : st + C::kStage;
     cur.next(p);
   }
   cp_async_wait<0>();
@@ -1164,6 +1324,11 @@ size_t workspace_bytes() {
 template <class C>
 cudaError_t launch(Params p, void *workspace, const DeviceInfo &dev, cudaStream_t stream) {
   p.RT = (p.R + C::kRows - 1) / C::kRows;
+  p.over_T = (uint32_t)(((uint64_t(1) << 32) + p.T - 1) / p.T);  // not used for T = 1
+  const uintptr_t q16 = reinterpret_cast<uintptr_t>(p.q), o16 = reinterpret_cast<uintptr_t>(p.o);
+  constexpr int kVec = C::kF32 ? 4 : 8;  // values in 16 bytes
+  p.q_vec = q16 % 16 == 0 && p.qs.b % kVec == 0 && p.qs.h % kVec == 0 && p.qs.s % kVec == 0;
+  p.o_vec = o16 % 16 == 0 && p.os.b % kVec == 0 && p.os.h % kVec == 0 && p.os.s % kVec == 0;
   const int64_t segs = p.c.B * p.c.H * p.RT;
   const int64_t units = (p.c.L + C::kKeys - 1) / C::kKeys;  // of a segment, at most
   const int64_t most = (dev.sm_count < kMaxSms ? dev.sm_count : kMaxSms) * C::kCtas;

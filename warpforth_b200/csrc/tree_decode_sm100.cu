@@ -6,8 +6,7 @@
 namespace wfattn {
 
 size_t tree_decode_workspace_bytes(const CacheView &c, bool f32, int64_t Hq, int T) {
-  const int64_t rows = Hq / c.H * T;
-  const int R = (int)imin64(rows, 1 << 20);  // the size is the same from 65 rows on
+  const int R = (int)(Hq / c.H * T);  // at most kMaxTreeRows
 #define WFATTN_TREE_CASE(name, fmt, is_f32) \
   if (c.format == fmt && f32 == is_f32) return tree_workspace_##name(c.D, R);
   WFATTN_TREE_KINDS(WFATTN_TREE_CASE)
@@ -21,7 +20,7 @@ cudaError_t launch_tree_decode(const TreeDecodeArgs &a, const DeviceInfo &dev,
   p.c = a.c;
   p.G = (int)(a.Hq / a.c.H);
   p.T = a.T;
-  p.R = p.G * p.T;  // at most 2^31 - 1 rows of queries in all
+  p.R = p.G * p.T;  // at most kMaxTreeRows
   p.q = static_cast<const uint8_t *>(a.q);
   p.o = static_cast<uint8_t *>(a.o);
   p.qs = a.qs;

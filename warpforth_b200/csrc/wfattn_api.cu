@@ -703,10 +703,10 @@ wfattn_status_t check_tree(const wfattn_cache_t *cache, int dtype, int64_t heads
                 (long long)nodes);
   int64_t rows = 0;
   if (heads_q < 1 || heads_q % a->c.H || __builtin_mul_overflow(heads_q, a->c.B * nodes, &rows) ||
-      rows > INT32_MAX)
+      rows > INT32_MAX || heads_q / a->c.H * nodes > kMaxTreeRows)
     return fail(WFATTN_INVALID_ARG,
                 "heads_q must be a multiple of the cache's %lld heads, with at most 2^31-1 rows "
-                "of queries (got %lld heads)", (long long)a->c.H, (long long)heads_q);
+                "of queries, 2^20 of one cache head (got %lld heads)", (long long)a->c.H, (long long)heads_q);
   a->Hq = heads_q;
   a->T = (int)nodes;
   return WFATTN_OK;

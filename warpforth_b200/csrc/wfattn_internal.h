@@ -121,6 +121,7 @@ cudaError_t launch_cache_write(const CacheRowsArgs &a, const DeviceInfo &dev, cu
 cudaError_t launch_cache_read(const CacheRowsArgs &a, const DeviceInfo &dev, cudaStream_t stream);
 
 constexpr int kMaxTreeNodes = 64;
+constexpr int64_t kMaxTreeRows = 1 << 20;  // query rows of one cache head
 
 struct CacheKeepArgs {
   CacheView c;
