@@ -359,10 +359,15 @@ WFATTN_API wfattn_status_t wfattn_cache_keep(const wfattn_cache_t *cache, const 
  * Rows that a node does not see do not reach its output, whatever they hold.
  * A negative length counts as 0, a count is clamped to 0..nodes, and rows past
  * max_len are not read (recorded, see above).
- * scale <= 0 selects 1/sqrt(head_dim).  workspace: at least
- * wfattn_tree_decode_workspace_size() bytes (0 for a bad cache or size),
- * 16-byte aligned; calls that share one must be ordered on one stream.
+ * scale <= 0 selects 1/sqrt(head_dim).
+ * workspace: at least wfattn_tree_decode_workspace_size() bytes (0 for a bad
+ *         cache or size), 16-byte aligned.  Its first
+ *         WFATTN_TREE_DECODE_ZEROED bytes must be zero before the first call
+ *         on it, and every call leaves them so; nothing else may write them
+ *         in between.  Calls that share a workspace, of any shapes, must be
+ *         ordered on one stream.
  */
+#define WFATTN_TREE_DECODE_ZEROED 4096
 WFATTN_API size_t wfattn_tree_decode_workspace_size(const wfattn_cache_t *cache, int dtype,
                                                     int64_t heads_q, int64_t nodes);
 

@@ -15,7 +15,7 @@ def _cache(**kw):
     c = dict(format=_lib.CACHE_E4M3, head_dim=64, batch=2, heads=3, max_len=10, batch_stride=30,
              head_stride=10, k=16, v=16, k_scale=16, v_scale=16)
     c.update(kw)
-    return _lib.Cache(**c)
+    return ctypes.byref(_lib.Cache(**c))
 
 
 def _write(cache, dtype=_lib.DTYPE_BF16, n=4, k=16, v=16, starts=16, strides=None):

@@ -21,12 +21,10 @@ _CACHE = ("KVCache", "cache_write", "cache_read", "cache_keep", "tree_decode", "
 
 
 def __getattr__(name):  # lazy: importing the package does not import torch
-    if name in _CACHE:
-        from . import cache
+    if name not in __all__:
+        raise AttributeError(name)
+    from . import cache, warpforth
 
-        return getattr(cache, name)
-    if name in __all__:
-        from . import warpforth
-
-        return getattr(warpforth, name)
-    raise AttributeError(name)
+    value = getattr(cache if name in _CACHE else warpforth, name)
+    globals()[name] = value  # the next look-up finds it
+    return value

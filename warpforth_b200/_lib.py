@@ -16,6 +16,7 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libwfattn.so"
 OK, INVALID_ARG, UNSUPPORTED, CUDA_ERROR, TIMEOUT = range(5)
 # wfattn_dtype_t
 DTYPE_F32, DTYPE_BF16 = 0, 1
+TREE_DECODE_ZEROED = 4096  # bytes of a tree_decode workspace that start at zero
 # wfattn_cache_format_t
 CACHE_F32, CACHE_BF16, CACHE_E4M3, CACHE_INT4 = range(4)
 
@@ -111,21 +112,20 @@ def load() -> ctypes.CDLL:
     lib.wfattn_peer_close.argtypes = [_vp, ctypes.c_int]
     lib.wfattn_peer_free.restype = ctypes.c_int
     lib.wfattn_peer_free.argtypes = [_vp, ctypes.c_int]
-    _cache = ctypes.POINTER(Cache)
+    # The cache calls take strides as packed bytes and the cache as an address: a c_void_p
+    # argument converts in a tenth of a typed pointer's time, and decode steps make many calls.
     lib.wfattn_cache_write.restype = ctypes.c_int
-    lib.wfattn_cache_write.argtypes = [_cache, ctypes.c_int, _i64, _vp, _i64p, _vp, _i64p, _vp,
-                                       _vp, _vp]
+    lib.wfattn_cache_write.argtypes = [_vp, ctypes.c_int, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
     lib.wfattn_cache_read.restype = ctypes.c_int
-    lib.wfattn_cache_read.argtypes = [_cache, ctypes.c_int, _i64, _vp, _i64p, _vp, _i64p, _vp,
-                                      _vp, ctypes.c_int, _vp]
+    lib.wfattn_cache_read.argtypes = [_vp, ctypes.c_int, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                                      ctypes.c_int, _vp]
     lib.wfattn_cache_keep.restype = ctypes.c_int
-    lib.wfattn_cache_keep.argtypes = [_cache, _vp, _i64, _vp, _i64, _vp, _vp, _vp]
+    lib.wfattn_cache_keep.argtypes = [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp]
     lib.wfattn_tree_decode_workspace_size.restype = ctypes.c_size_t
-    lib.wfattn_tree_decode_workspace_size.argtypes = [_cache, ctypes.c_int, _i64, _i64]
+    lib.wfattn_tree_decode_workspace_size.argtypes = [_vp, ctypes.c_int, _i64, _i64]
     lib.wfattn_tree_decode.restype = ctypes.c_int
-    lib.wfattn_tree_decode.argtypes = [_cache, ctypes.c_int, _i64, _i64, _vp, _i64p, _vp, _vp,
-                                       _i64, _vp, _vp, _i64p, ctypes.c_float, _vp,
-                                       ctypes.c_size_t, _vp]
+    lib.wfattn_tree_decode.argtypes = [_vp, ctypes.c_int, _i64, _i64, _vp, _vp, _vp, _vp, _i64,
+                                       _vp, _vp, _vp, ctypes.c_float, _vp, ctypes.c_size_t, _vp]
     _lib = lib
     return lib
 

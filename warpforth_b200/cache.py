@@ -20,6 +20,7 @@ stream of the cache's device.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -122,45 +123,47 @@ class KVCache:
         self._c = _lib.Cache(_FORMATS[fmt][0], self.head_dim, batch, heads, max_len, sb, sh,
                              _ptr(k), _ptr(v), _ptr(k_scale) if scaled else None,
                              _ptr(v_scale) if scaled else None)
-        self._ref = ctypes.byref(self._c)
+        self._at = ctypes.addressof(self._c)
+        self._batch_shape = torch.Size((batch,))
+        self._tree_bytes: dict[tuple, int] = {}  # workspace sizes by call shape
 
 
-def _call(cache: KVCache, fn, *args) -> None:
+_strides = struct.Struct("3q").pack  # of a 4-d tensor, as the library takes them
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _run(cache: KVCache, fn, *args) -> None:
     """fn(cache, *args, stream) with the cache's device current."""
-    index = cache.device.index
-    if index == torch.cuda.current_device():
-        _lib.check(fn(cache._ref, *args, _stream_handle(cache.device)))
-        return
-    with torch.cuda.device(index):
-        _lib.check(fn(cache._ref, *args, _stream_handle(cache.device)))
+    if cache.device.index == _current_device():
+        status = fn(cache._at, *args, _stream_handle(cache.device))
+    else:
+        with torch.cuda.device(cache.device):
+            status = fn(cache._at, *args, _stream_handle(cache.device))
+    if status:
+        _lib.check(status)
 
 
-def _check_ints(name: str, t: torch.Tensor, shape: tuple[int, ...], cache: KVCache,
-                dtype: torch.dtype = torch.int32) -> int:
+def _ints(name: str, t: torch.Tensor, shape, cache: KVCache,
+          dtype: torch.dtype = torch.int32) -> int:
+    """The address of integers with a unit last stride on the cache's device."""
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != cache.device or \
             t.shape != shape:
-        raise ValueError(f"{name} must be {dtype} of shape {shape} on {cache.device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)} on {cache.device}")
+    if t.stride(-1) != 1 and shape[-1] > 1:
         raise ValueError(f"{name} must have a unit last stride")
     return t.data_ptr()
 
 
-def _counts(counts, cache: KVCache) -> int | None:
-    return None if counts is None else _check_ints("counts", counts, (cache.batch,), cache)
-
-
-def _check_rows(name: str, t: torch.Tensor, shape: tuple[int, ...], dtype, cache: KVCache) -> None:
+def _rows(name: str, t: torch.Tensor, shape, dtype, cache: KVCache) -> bytes:
+    """The strides of f32 or bf16 rows of this shape on the cache's device."""
     if not isinstance(t, torch.Tensor) or t.shape != shape or t.device != cache.device:
         raise ValueError(f"{name} must be of shape {tuple(shape)} on {cache.device}")
     if t.dtype != dtype or dtype not in _DTYPES:
         raise ValueError(f"{name} must be float32 or bfloat16, as its companions (got {t.dtype})")
-    if t.stride(-1) != 1:
+    a, b, c, d = t.stride()
+    if d != 1:
         raise ValueError(f"{name} must have a unit head_dim stride")
-
-
-def _strides(t: torch.Tensor) -> ctypes.Array:
-    st = t.stride()
-    return (ctypes.c_int64 * 3)(st[0], st[1], st[2])
+    return _strides(a, b, c)
 
 
 def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, *,
@@ -171,16 +174,14 @@ def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, starts: torch.
     ``counts[b]`` rows of sequence b are taken (all n without ``counts``).  The other rows of the
     cache stay as they are.
     """
-    _require_cuda("k", k)
-    if k.dim() != 4:
-        raise ValueError(f"k must be [batch, heads, n, head_dim], got {tuple(k.shape)}")
-    n = k.shape[2]
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise ValueError("k must be a [batch, heads, n, head_dim] tensor")
+    dtype, n = k.dtype, k.shape[2]
     shape = (cache.batch, cache.heads, n, cache.head_dim)
-    _check_rows("k", k, shape, k.dtype, cache)
-    _check_rows("v", v, shape, k.dtype, cache)
-    at = _check_ints("starts", starts, (cache.batch,), cache)
-    _call(cache, _lib.load().wfattn_cache_write, _DTYPES[k.dtype], n, k.data_ptr(), _strides(k),
-          v.data_ptr(), _strides(v), at, _counts(counts, cache))
+    ks, vs = _rows("k", k, shape, dtype, cache), _rows("v", v, shape, dtype, cache)
+    _run(cache, _lib.load().wfattn_cache_write, _DTYPES[dtype], n, k.data_ptr(), ks, v.data_ptr(),
+         vs, _ints("starts", starts, cache._batch_shape, cache),
+         None if counts is None else _ints("counts", counts, cache._batch_shape, cache))
 
 
 def cache_read(cache: KVCache, starts: torch.Tensor, rows: int, *,
@@ -198,15 +199,16 @@ def cache_read(cache: KVCache, starts: torch.Tensor, rows: int, *,
         dtype = dtype or (torch.float32 if cache.fmt == "f32" else torch.bfloat16)
         if dtype not in _DTYPES:
             raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
-        k, v = (torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
+        k, v = torch.empty((2, *shape), dtype=dtype, device=cache.device)
+        ks = vs = None  # contiguous
     else:
         k, v = out
-        for name, t in (("out[0]", k), ("out[1]", v)):
-            _check_rows(name, t, shape, dtype or k.dtype, cache)
-    at = _check_ints("starts", starts, (cache.batch,), cache)
-    _call(cache, _lib.load().wfattn_cache_read, _DTYPES[k.dtype], shape[2], k.data_ptr(),
-          _strides(k), v.data_ptr(), _strides(v), at, _counts(counts, cache),
-          1 if out is None else 0)
+        dtype = dtype or k.dtype
+        ks, vs = (_rows(name, t, shape, dtype, cache) for name, t in (("out[0]", k), ("out[1]", v)))
+    _run(cache, _lib.load().wfattn_cache_read, _DTYPES[dtype], shape[2], k.data_ptr(), ks,
+         v.data_ptr(), vs, _ints("starts", starts, cache._batch_shape, cache),
+         None if counts is None else _ints("counts", counts, cache._batch_shape, cache),
+         out is None)
     return k, v
 
 
@@ -220,14 +222,16 @@ def cache_keep(cache: KVCache, lens: torch.Tensor, path: torch.Tensor, *,
     Returns ``out`` (a new int32 [batch] tensor when not given, never ``lens`` itself):
     ``lens + counts``.
     """
-    at = _check_ints("lens", lens, (cache.batch,), cache)
+    at = _ints("lens", lens, cache._batch_shape, cache)
     if not isinstance(path, torch.Tensor) or path.dim() != 2:
         raise ValueError("path must be int32 [batch, depth]")
-    to = _check_ints("path", path, (cache.batch, path.shape[1]), cache)
+    depth = path.shape[1]
+    steps = _ints("path", path, (cache.batch, depth), cache)
     if out is None:
-        out = torch.empty_like(lens, memory_format=torch.contiguous_format)
-    _call(cache, _lib.load().wfattn_cache_keep, at, path.shape[1], to, path.stride(0),
-          _counts(counts, cache), _check_ints("out", out, (cache.batch,), cache))
+        out = lens.new_empty(cache._batch_shape)
+    _run(cache, _lib.load().wfattn_cache_keep, at, depth, steps, path.stride(0),
+         None if counts is None else _ints("counts", counts, cache._batch_shape, cache),
+         _ints("out", out, cache._batch_shape, cache))
     return out
 
 
@@ -248,31 +252,32 @@ def tree_decode(q: torch.Tensor, cache: KVCache, kv_lens: torch.Tensor, *,
 
     Returns [batch, heads_q, n, head_dim] of q's dtype (``out`` where given).
     """
-    _require_cuda("q", q)
-    if q.dim() != 4:
-        raise ValueError(f"q must be [batch, heads_q, nodes, head_dim], got {tuple(q.shape)}")
-    b, hq, n, d = q.shape
-    _check_rows("q", q, (cache.batch, hq, n, cache.head_dim), q.dtype, cache)
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise ValueError("q must be a [batch, heads_q, nodes, head_dim] tensor")
+    dtype, shape = q.dtype, q.shape
+    _, hq, n, _ = shape
+    qs = _rows("q", q, (cache.batch, hq, n, cache.head_dim), dtype, cache)
     if out is None:
-        out = torch.empty((b, hq, n, d), dtype=q.dtype, device=q.device)
+        out, os = q.new_empty(shape), None  # contiguous
     else:
-        _check_rows("out", out, q.shape, q.dtype, cache)
-    at = _check_ints("kv_lens", kv_lens, (b,), cache)
+        os = _rows("out", out, shape, dtype, cache)
+    at = _ints("kv_lens", kv_lens, cache._batch_shape, cache)
     words, words_stride = None, 0
     if tree is not None:
-        shape = (n,) if isinstance(tree, torch.Tensor) and tree.dim() == 1 else (b, n)
-        words = _check_ints("tree", tree, shape, cache, torch.int64)
-        words_stride = 0 if tree.dim() == 1 else tree.stride(0)
+        one = isinstance(tree, torch.Tensor) and tree.dim() == 1
+        words = _ints("tree", tree, (n,) if one else (cache.batch, n), cache, torch.int64)
+        words_stride = 0 if one else tree.stride(0)
+    count = None if nodes is None else _ints("nodes", nodes, cache._batch_shape, cache)
     lib = _lib.load()
-    dtype = _DTYPES[q.dtype]
-    nbytes = int(lib.wfattn_tree_decode_workspace_size(cache._ref, dtype, hq, n))
-    if nbytes == 0:
-        _lib.check_last(lib)
-    ws = (workspace or DecodeWorkspace()).get(nbytes, q.device)
-    count = None if nodes is None else _check_ints("nodes", nodes, (b,), cache)
-    _call(cache, lib.wfattn_tree_decode, dtype, hq, n, q.data_ptr(), _strides(q), at, words,
-          words_stride, count, out.data_ptr(), _strides(out), float(scale) if scale else 0.0,
-          ws.data_ptr(), ws.numel())
+    nbytes = cache._tree_bytes.get((dtype, hq, n))
+    if nbytes is None:
+        nbytes = lib.wfattn_tree_decode_workspace_size(cache._at, _DTYPES[dtype], hq, n)
+        if nbytes == 0:
+            _lib.check_last(lib)
+        cache._tree_bytes[dtype, hq, n] = nbytes
+    ws = (workspace or DecodeWorkspace()).get_tree(nbytes, cache.device)
+    _run(cache, lib.wfattn_tree_decode, _DTYPES[dtype], hq, n, q.data_ptr(), qs, at, words,
+         words_stride, count, out.data_ptr(), os, scale or 0.0, ws.data_ptr(), ws.numel())
     return out
 
 

@@ -51,34 +51,30 @@ __device__ __forceinline__ float2 f16x2_to_f32(uint32_t w) {
 
 }  // namespace ptx
 
-// Eight consecutive values of a row as f32, from the row's eight codes at
-// `codes` (8 f32, 8 bf16, 8 bytes or 4 bytes) and its scale word.
+// Eight consecutive values of a row as f32, from the row's eight codes (32, 16,
+// 8 or 4 bytes) and its scale word.
 template <int kFmt>
-__device__ __forceinline__ void cache_load8(const uint8_t *codes, uint32_t scale, float (&f)[8]) {
+__device__ __forceinline__ void cache_values8(const uint32_t *w, uint32_t scale, float (&f)[8]) {
   if constexpr (kFmt == WFATTN_CACHE_F32) {
-    const float4 a = *reinterpret_cast<const float4 *>(codes);
-    const float4 b = *reinterpret_cast<const float4 *>(codes + 16);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-    f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else if constexpr (kFmt == WFATTN_CACHE_BF16) {
-    const uint4 w = *reinterpret_cast<const uint4 *>(codes);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[2 * i] = ptx::bf16_lo(u[i]), f[2 * i + 1] = ptx::bf16_hi(u[i]);
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+  } else if constexpr (kFmt == WFATTN_CACHE_BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = ptx::bf16_lo(w[i]), f[2 * i + 1] = ptx::bf16_hi(w[i]);
   } else if constexpr (kFmt == WFATTN_CACHE_E4M3) {
-    const uint2 w = *reinterpret_cast<const uint2 *>(codes);
     const float s = __uint_as_float(scale);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 x = ptx::f16x2_to_f32(ptx::e4m3x2_to_f16x2((i < 2 ? w.x : w.y) >> (16 * (i & 1))));
+      const float2 x = ptx::f16x2_to_f32(ptx::e4m3x2_to_f16x2(w[i / 2] >> (16 * (i & 1))));
       f[2 * i] = x.x * s, f[2 * i + 1] = x.y * s;
     }
   } else {
-    const uint32_t w = *reinterpret_cast<const uint32_t *>(codes);
     const float s = ptx::bf16_lo(scale), m = ptx::bf16_hi(scale);
-    // s u is exact in f32 (8 and 4 bits), so one rounding is left either way
+    // 2^23 + u has the code in its low bits; s u is exact in f32 (8 and 4
+    // bits), so one rounding is left
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = fmaf(s, (float)((w >> (4 * i)) & 15u), m);
+    for (int i = 0; i < 8; ++i)
+      f[i] = fmaf(s, __uint_as_float((w[0] >> (4 * i) & 15u) | 0x4b000000u) - 8388608.f, m);
   }
 }
 

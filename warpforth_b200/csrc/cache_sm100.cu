@@ -1,41 +1,66 @@
 // cache_sm100.cu -- writing, reading and keeping rows of a key/value cache
 // (formats: include/wfattn.h).
 //
-// All three are moves of rows: a row of D values is D/8 lanes' work, 8 values
-// (16 or 32 bytes) a lane, so loads and stores are 4 to 32 bytes a lane and a
-// warp touches whole 128-byte lines.  A row's maximum (e4m3) or its extremes
-// (int4) are shuffles over its lanes; nothing goes through shared memory.
+// All three are moves of rows, bound by HBM.  A row of D values is D/8 lanes'
+// work, 8 values (16 or 32 bytes) a lane, so loads and stores are 4 to 32 bytes
+// a lane and a warp touches whole 128-byte lines.  A row's largest magnitude
+// (e4m3) or its extremes (int4) are shuffles over its lanes; nothing goes
+// through shared memory.
 #include "cache_format.cuh"
 
 namespace wfattn {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kRowsAtOnce = 4;  // of a lane group, in flight together
 
 struct RowsParams {
   CacheView c;
   uint8_t *x[2];          // rows of new (or read) keys, values
   Strides3 xs[2];         // element strides
   uint32_t n, rows;       // rows a head, rows in all
+  uint32_t tiles;         // blocks a head (long form)
   const int32_t *starts, *counts;
   bool zero_rest;
   unsigned int *status;
 };
 
-// The 8 values x[0..7] of the caller's rows as f32.  kVec: 16-byte aligned.
+// Eight values of the caller's rows, as they are in memory.
+template <bool kF32>
+struct Raw {
+  uint32_t w[kF32 ? 8 : 4];
+};
+
+// kVec: 16-byte aligned.
 template <bool kF32, bool kVec>
-__device__ __forceinline__ void rows_load8(const uint8_t *x, float (&f)[8]) {
-  if constexpr (kF32 && kVec) {
-    cache_load8<WFATTN_CACHE_F32>(x, 0, f);
+__device__ __forceinline__ Raw<kF32> load_raw(const uint8_t *x) {
+  Raw<kF32> r;
+  if constexpr (kVec) {
+#pragma unroll
+    for (int i = 0; i < (kF32 ? 2 : 1); ++i) {
+      const uint4 v = reinterpret_cast<const uint4 *>(x)[i];
+      r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
+    }
   } else if constexpr (kF32) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = reinterpret_cast<const float *>(x)[i];
-  } else if constexpr (kVec) {
-    cache_load8<WFATTN_CACHE_BF16>(x, 0, f);
+    for (int i = 0; i < 8; ++i) r.w[i] = reinterpret_cast<const uint32_t *>(x)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      f[i] = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(x)[i] << 16);
+    for (int i = 0; i < 4; ++i)
+      r.w[i] = reinterpret_cast<const uint16_t *>(x)[2 * i] |
+               (uint32_t)reinterpret_cast<const uint16_t *>(x)[2 * i + 1] << 16;
+  }
+  return r;
+}
+
+template <bool kF32>
+__device__ __forceinline__ void to_f32(const Raw<kF32> &r, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (kF32)
+      f[i] = __uint_as_float(r.w[i]);
+    else
+      f[i] = i & 1 ? ptx::bf16_hi(r.w[i / 2]) : ptx::bf16_lo(r.w[i / 2]);
   }
 }
 
@@ -61,6 +86,76 @@ __device__ __forceinline__ void rows_store8(uint8_t *x, const float (&f)[8]) {
   }
 }
 
+// ---- extremes of a row; NaN wins both ways
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t min_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+template <bool kF32, int kLanes>
+__device__ __forceinline__ void row_extremes(const Raw<kF32> &x, float &lo, float &hi) {
+  if constexpr (kF32) {
+    lo = hi = __uint_as_float(x.w[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      lo = min_nan(lo, __uint_as_float(x.w[i]));
+      hi = max_nan(hi, __uint_as_float(x.w[i]));
+    }
+#pragma unroll
+    for (int m = 1; m < kLanes; m <<= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+    }
+  } else {
+    uint32_t l = x.w[0], h = x.w[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) l = min_nan_bf16x2(l, x.w[i]), h = max_nan_bf16x2(h, x.w[i]);
+#pragma unroll
+    for (int m = 1; m < kLanes; m <<= 1) {
+      l = min_nan_bf16x2(l, __shfl_xor_sync(0xffffffffu, l, m));
+      h = max_nan_bf16x2(h, __shfl_xor_sync(0xffffffffu, h, m));
+    }
+    lo = min_nan(ptx::bf16_lo(l), ptx::bf16_hi(l));
+    hi = max_nan(ptx::bf16_lo(h), ptx::bf16_hi(h));
+  }
+}
+
+// The largest magnitude of a row as f32 bits, which order like |x|: infinities
+// and NaN are the largest.
+template <bool kF32, int kLanes>
+__device__ __forceinline__ uint32_t row_top(const Raw<kF32> &x) {
+  uint32_t top = 0;
+  if constexpr (kF32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, x.w[i] & 0x7fffffffu);
+#pragma unroll
+    for (int m = 1; m < kLanes; m <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
+    return top;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = __vmaxu2(top, x.w[i] & 0x7fff7fffu);
+#pragma unroll
+  for (int m = 1; m < kLanes; m <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, m));
+  return max(top << 16, top & 0xffff0000u);
+}
+
 // x as the nearest bf16 not above (kDown) or not below it; x finite.
 template <bool kDown>
 __device__ __forceinline__ float to_bf16_directed(float x) {
@@ -72,173 +167,201 @@ __device__ __forceinline__ float to_bf16_directed(float x) {
 
 // Stores 8 values of a row in the cache's format; the row's kLanes lanes call
 // it together (every lane of the warp does, `live` or not).
-template <int kFmt, int kLanes>
+template <int kFmt, bool kF32, int kLanes>
 __device__ __forceinline__ void cache_store8(uint8_t *codes, uint8_t *scale, bool first, bool live,
-                                             const float (&f)[8]) {
+                                             const Raw<kF32> &x) {
+  float f[8];
+  to_f32<kF32>(x, f);
   if constexpr (kFmt == WFATTN_CACHE_F32) {
     if (live) rows_store8<true, true>(codes, f);
   } else if constexpr (kFmt == WFATTN_CACHE_BF16) {
     if (live) rows_store8<false, true>(codes, f);
+  } else if constexpr (kFmt == WFATTN_CACHE_E4M3) {
+    const uint32_t top = row_top<kF32, kLanes>(x);
+    const bool bad = top >= 0x7f800000u;
+    // 448 = 1.75 * 2^8: the exponent of the smallest 2^e with |x| <= 448 2^e
+    const int e = max((int)(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // x 2^-e is exact: one rounding
+      w[i] = ptx::pack_e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv);
+    if (!live) return;
+    *reinterpret_cast<uint2 *>(codes) =
+        bad ? make_uint2(0, 0) : make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    if (first)
+      *reinterpret_cast<uint32_t *>(scale) = bad ? 0x7fc00000u : (uint32_t)(127 + e) << 23;
   } else {
-    // |x| as an integer orders like |x|; infinities and NaN are the largest
-    uint32_t top = 0;
+    float lo, hi;
+    row_extremes<kF32, kLanes>(x, lo, hi);
+    const float m = to_bf16_directed<true>(lo);
+    const float s = to_bf16_directed<false>(__fdiv_rn(__fsub_rn(hi, m), 15.f));
+    // the largest bf16; a NaN or an infinity among the values, or a span past f32
+    const bool bad = !(s <= 3.38953139e38f);
+    // u = rint(fl(a / s)), a = fl(x - m) >= 0.  a <= 15 s (1 + 2^-23), so u is in
+    // 0..15 without a clamp.  t = a (1 / s) + 1.5 2^23 holds rint(a (1 / s)) in
+    // its low bits; a (1 / s) is within 1e-5 of a / s, so only values that near
+    // a half need the division itself.
+    constexpr float kMagic = 12582912.f;
+    const float inv = __frcp_rn(s);
+    float a[8], t[8], far = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-#pragma unroll
-    for (int m = 1; m < kLanes; m <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
-    bool bad = top >= 0x7f800000u;
-    if constexpr (kFmt == WFATTN_CACHE_E4M3) {
-      // 448 = 1.75 * 2^8: the exponent of the smallest 2^e with |x| <= 448 2^e
-      const int e = max((int)(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
-      const float inv = bad ? 0.f : __uint_as_float((uint32_t)(127 - e) << 23);
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)  // x 2^-e is exact: one rounding
-        w[i] = ptx::pack_e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv);
-      if (!live) return;
-      *reinterpret_cast<uint2 *>(codes) =
-          bad ? make_uint2(0, 0) : make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-      if (first)
-        *reinterpret_cast<uint32_t *>(scale) = bad ? 0x7fc00000u : (uint32_t)(127 + e) << 23;
-    } else {
-      float lo = f[0], hi = f[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) lo = fminf(lo, f[i]), hi = fmaxf(hi, f[i]);
-#pragma unroll
-      for (int m = 1; m < kLanes; m <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
-      }
-      const float m = to_bf16_directed<true>(lo);
-      const float s = to_bf16_directed<false>(__fdiv_rn(__fsub_rn(hi, m), 15.f));
-      bad = bad || !(s <= 3.38953139e38f);  // the largest bf16
-      uint32_t w = 0;
-      if (!bad && s > 0.f) {
-        // rint(fl(a / s)): a * (1 / s) is within 4 ulp of it, so only values
-        // next to a half need the division itself
-        const float inv = __frcp_rn(s);
-        float r[8];
-        bool near_half = inv > 1e38f;  // 1 / s overflows
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float a = __fsub_rn(f[i], m), y = a * inv;
-          r[i] = rintf(y);
-          near_half = near_half || fabsf(fabsf(y - r[i]) - 0.5f) < 1e-5f;
-        }
-        if (near_half) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) r[i] = rintf(__fdiv_rn(__fsub_rn(f[i], m), s));
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w |= (uint32_t)fminf(fmaxf(r[i], 0.f), 15.f) << (4 * i);
-      }
-      if (!live) return;
-      *reinterpret_cast<uint32_t *>(codes) = w;
-      if (first)
-        *reinterpret_cast<uint32_t *>(scale) =
-            bad ? 0x7fc07fc0u : (__float_as_uint(s) >> 16) | (__float_as_uint(m) & 0xffff0000u);
+    for (int i = 0; i < 8; ++i) {
+      a[i] = __fsub_rn(f[i], m);
+      t[i] = fmaf(a[i], inv, kMagic);
+      far = fmaxf(far, fabsf(fmaf(a[i], inv, kMagic - t[i])));
     }
+    if (!(far < 0.49999f) || !(inv < 1e38f)) {  // or 1 / s overflows
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = kMagic + (s > 0.f ? rintf(__fdiv_rn(a[i], s)) : 0.f);
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) w = w * 16 + __float_as_uint(t[i]);
+    w -= 0x4b400000u * 0x11111111u;  // the bits of kMagic in all of them
+    if (!live) return;
+    *reinterpret_cast<uint32_t *>(codes) = bad ? 0u : w;
+    if (first)
+      *reinterpret_cast<uint32_t *>(scale) =
+          bad ? 0x7fc07fc0u : (__float_as_uint(s) >> 16) | (__float_as_uint(m) & 0xffff0000u);
   }
 }
 
-// Where the caller's row r of one head lies in the cache (-1: not live).
-__device__ __forceinline__ int64_t cache_row(const RowsParams &p, uint32_t bh, uint32_t i,
-                                             int64_t b, bool report) {
-  int32_t n = p.counts ? p.counts[b] : (int32_t)p.n;
-  const int64_t at = (int64_t)p.starts[b] + i;
-  bool bad = n < 0 || n > (int32_t)p.n;
-  n = n > (int32_t)p.n ? (int32_t)p.n : n;
-  const bool live = (int32_t)i < n;
-  const bool inside = at >= 0 && at < p.c.L;
-  if (report && (bad || (live && !inside))) atomicOr(p.status, kDevBadRowMask);
-  const int64_t h = bh - b * p.c.H;
-  return live && inside ? b * p.c.sb + h * p.c.sh + at : -1;
+// Which of a head's rows i < n are live, and its first row's position: those in
+// [from, to), at positions start + i.
+struct Span {
+  int64_t start;
+  int from, to;
+};
+__device__ __forceinline__ Span live_rows(const RowsParams &p, uint32_t b, bool report) {
+  const int n = (int)p.n, start = p.starts[b];
+  const int count = p.counts ? p.counts[b] : n;
+  Span s;
+  s.start = start;
+  s.to = min(max(count, 0), n);
+  s.from = start < 0 ? (int)imin64(s.to, -(int64_t)start) : 0;
+  const int last = (int)imax64(s.from, imin64(s.to, p.c.L - start));
+  if (report && (count < 0 || count > n || (s.to > 0 && (start < 0 || last < s.to))))
+    atomicOr(p.status, kDevBadRowMask);
+  s.to = last;
+  return s;
 }
 
-// One row (of K or of V) a lane group, kRows of them one after the other.
-template <int kFmt, int D, bool kF32, bool kVec, bool kWrite, int kRows>
+// Rows of K (or V) of one head: kLong, a block's share of them, contiguous, a
+// lane group taking every kGroups-th; else one row a group, whichever head's.
+template <int kFmt, int D, bool kF32, bool kVec, bool kWrite, bool kLong>
 __global__ void __launch_bounds__(kThreads) cache_rows_kernel(const RowsParams p) {
-  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes;
-  constexpr int kRowBytes = CacheRow<kFmt, D>::kBytes;
-  const int which = blockIdx.y, lane = threadIdx.x % kLanes;
-  uint8_t *codes = which ? p.c.v : p.c.k;
-  uint8_t *scales = which ? p.c.v_scale : p.c.k_scale;
+  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes, kRows = kLong ? kRowsAtOnce : 1;
+  constexpr int kRowBytes = CacheRow<kFmt, D>::kBytes, kSize = kF32 ? 4 : 2;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int which = blockIdx.y;
+  uint32_t bh, i0;
+  if constexpr (kLong) {
+    bh = blockIdx.x / p.tiles;
+    i0 = (blockIdx.x - bh * p.tiles) * (kGroups * kRows) + group;
+  } else {
+    const uint32_t r = blockIdx.x * kGroups + group;
+    bh = min(r, p.rows - 1) / p.n;
+    i0 = r - bh * p.n;  // p.n in a group past the last row
+  }
+  const uint32_t H = (uint32_t)p.c.H, b = bh / H, h = bh - b * H;
   const Strides3 xs = p.xs[which];
-  int64_t row[kRows];
-  uint8_t *x[kRows];
+  uint8_t *x = p.x[which] + (b * xs.b + h * xs.h + i0 * xs.s + lane * 8) * kSize;
+  const int64_t step = (int64_t)kGroups * xs.s * kSize;
+  Raw<kF32> raw[kRows];
+  if constexpr (kWrite) {  // every row exists: no need to know which are live
 #pragma unroll
-  for (int j = 0; j < kRows; ++j) {
-    const uint32_t r = (blockIdx.x * kRows + j) * kGroups + threadIdx.x / kLanes;
-    row[j] = -1;
-    x[j] = nullptr;
-    if (r < p.rows) {
-      const uint32_t bh = r / p.n, i = r - bh * p.n;
-      const uint32_t b = bh / (uint32_t)p.c.H;
-      row[j] = cache_row(p, bh, i, b, lane == 0 && which == 0);
-      x[j] = p.x[which] + (b * xs.b + (int64_t)(bh - b * (uint32_t)p.c.H) * xs.h + i * xs.s +
-                           lane * 8) * (kF32 ? 4 : 2);
+    for (int j = 0; j < kRows; ++j) {
+      raw[j] = Raw<kF32>{};
+      if (i0 + j * kGroups < p.n) raw[j] = load_raw<kF32, kVec>(x + j * step);
     }
   }
-  float f[kRows][8];
+  const Span span = live_rows(p, b, i0 == 0 && lane == 0 && which == 0 && h == 0);
+  const int64_t row0 = b * p.c.sb + h * p.c.sh + span.start + i0;
+  uint8_t *codes = (which ? p.c.v : p.c.k) + row0 * kRowBytes + lane * (kRowBytes / kLanes);
+  uint8_t *scales = (which ? p.c.v_scale : p.c.k_scale) + row0 * 4;
+  bool live[kRows];
 #pragma unroll
   for (int j = 0; j < kRows; ++j) {
+    const int i = (int)i0 + j * kGroups;
+    live[j] = i >= span.from && i < span.to;
+  }
+  if constexpr (kWrite) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[j][e] = 0.f;
-    if (row[j] >= 0) {
-      if constexpr (kWrite) {
-        rows_load8<kF32, kVec>(x[j], f[j]);
-      } else {
-        const uint32_t s = CacheRow<kFmt, D>::kScaled
-                               ? *reinterpret_cast<const uint32_t *>(scales + row[j] * 4)
-                               : 0u;
-        cache_load8<kFmt>(codes + row[j] * kRowBytes + lane * (kRowBytes / kLanes), s, f[j]);
+    for (int j = 0; j < kRows; ++j)
+      cache_store8<kFmt, kF32, kLanes>(codes + j * kGroups * kRowBytes, scales + j * kGroups * 4,
+                                       lane == 0, live[j], raw[j]);
+  } else {
+    constexpr int kWords = kRowBytes / kLanes / 4;
+    uint32_t w[kRows][kWords], scale[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const uint32_t *from = reinterpret_cast<const uint32_t *>(codes + j * kGroups * kRowBytes);
+      scale[j] = 0;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) w[j][k] = 0;
+      if (live[j]) {
+        if constexpr (kWords % 4 == 0) {
+#pragma unroll
+          for (int k = 0; k < kWords; k += 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(from + k);
+            w[j][k] = v.x, w[j][k + 1] = v.y, w[j][k + 2] = v.z, w[j][k + 3] = v.w;
+          }
+        } else if constexpr (kWords == 2) {
+          const uint2 v = *reinterpret_cast<const uint2 *>(from);
+          w[j][0] = v.x, w[j][1] = v.y;
+        } else {
+          w[j][0] = *from;
+        }
+        if constexpr (CacheRow<kFmt, D>::kScaled)
+          scale[j] = *reinterpret_cast<const uint32_t *>(scales + j * kGroups * 4);
       }
     }
-  }
 #pragma unroll
-  for (int j = 0; j < kRows; ++j) {
-    if constexpr (kWrite)
-      cache_store8<kFmt, kLanes>(codes + row[j] * kRowBytes + lane * (kRowBytes / kLanes),
-                                 scales + row[j] * 4, lane == 0, row[j] >= 0, f[j]);
-    else if (row[j] >= 0 || (p.zero_rest && x[j]))
-      rows_store8<kF32, kVec>(x[j], f[j]);
+    for (int j = 0; j < kRows; ++j) {
+      if (live[j] || (p.zero_rest && i0 + j * kGroups < p.n)) {
+        float f[8];  // zeros where the row is not live: codes and scale are 0
+        cache_values8<kFmt>(w[j], scale[j], f);
+        rows_store8<kF32, kVec>(x + j * step, f);
+      }
+    }
   }
 }
 
 template <int kFmt, int D, bool kF32, bool kVec, bool kWrite>
-cudaError_t launch_rows(const RowsParams &p, const DeviceInfo &dev, cudaStream_t stream) {
-  constexpr uint32_t kGroups = kThreads / (D / 8);
-  // One row a group keeps every SM busy on few rows; with rows for four full
-  // waves, four a group keep four times the bytes in flight.
-  const uint32_t blocks = (p.rows + kGroups - 1) / kGroups;
-  if (blocks < 32u * (uint32_t)dev.sm_count)
-    cache_rows_kernel<kFmt, D, kF32, kVec, kWrite, 1><<<dim3(blocks, 2), kThreads, 0, stream>>>(p);
-  else
-    cache_rows_kernel<kFmt, D, kF32, kVec, kWrite, 4>
-        <<<dim3((blocks + 3) / 4, 2), kThreads, 0, stream>>>(p);
+cudaError_t launch_rows(RowsParams p, cudaStream_t stream) {
+  constexpr uint32_t kGroups = kThreads / (D / 8), kTile = kGroups * kRowsAtOnce;
+  // The long form has four rows a group in flight and its addresses and lengths
+  // once a block; below half a block's rows a head it would idle.
+  if (p.n >= kTile / 2) {
+    p.tiles = (p.n + kTile - 1) / kTile;
+    cache_rows_kernel<kFmt, D, kF32, kVec, kWrite, true>
+        <<<dim3(p.rows / p.n * p.tiles, 2), kThreads, 0, stream>>>(p);
+  } else {
+    cache_rows_kernel<kFmt, D, kF32, kVec, kWrite, false>
+        <<<dim3((p.rows + kGroups - 1) / kGroups, 2), kThreads, 0, stream>>>(p);
+  }
   return cudaGetLastError();
 }
 
 template <int kFmt, int D, bool kWrite>
-cudaError_t launch_rows_fd(const RowsParams &p, bool f32, const DeviceInfo &dev,
-                           cudaStream_t stream) {
+cudaError_t launch_rows_fd(const RowsParams &p, bool f32, cudaStream_t stream) {
   const int64_t m = f32 ? 4 : 8;  // elements in 16 bytes
   bool vec = true;
   for (int w = 0; w < 2; ++w)
     vec = vec && (reinterpret_cast<uintptr_t>(p.x[w]) & 15u) == 0 && p.xs[w].b % m == 0 &&
           p.xs[w].h % m == 0 && p.xs[w].s % m == 0;
   if (f32)
-    return vec ? launch_rows<kFmt, D, true, true, kWrite>(p, dev, stream)
-               : launch_rows<kFmt, D, true, false, kWrite>(p, dev, stream);
-  return vec ? launch_rows<kFmt, D, false, true, kWrite>(p, dev, stream)
-             : launch_rows<kFmt, D, false, false, kWrite>(p, dev, stream);
+    return vec ? launch_rows<kFmt, D, true, true, kWrite>(p, stream)
+               : launch_rows<kFmt, D, true, false, kWrite>(p, stream);
+  return vec ? launch_rows<kFmt, D, false, true, kWrite>(p, stream)
+             : launch_rows<kFmt, D, false, false, kWrite>(p, stream);
 }
 
 template <int kFmt, bool kWrite>
-cudaError_t launch_rows_f(const RowsParams &p, bool f32, const DeviceInfo &dev,
-                          cudaStream_t stream) {
-  return p.c.D == 64 ? launch_rows_fd<kFmt, 64, kWrite>(p, f32, dev, stream)
-                     : launch_rows_fd<kFmt, 128, kWrite>(p, f32, dev, stream);
+cudaError_t launch_rows_f(const RowsParams &p, bool f32, cudaStream_t stream) {
+  return p.c.D == 64 ? launch_rows_fd<kFmt, 64, kWrite>(p, f32, stream)
+                     : launch_rows_fd<kFmt, 128, kWrite>(p, f32, stream);
 }
 
 template <bool kWrite>
@@ -251,15 +374,16 @@ cudaError_t launch_rows_any(const CacheRowsArgs &a, const DeviceInfo &dev, cudaS
   p.xs[1] = a.vs;
   p.n = (uint32_t)a.n;
   p.rows = (uint32_t)(a.c.B * a.c.H * a.n);  // at most 2^31 - 1
+  p.tiles = 0;
   p.starts = a.starts;
   p.counts = a.counts;
   p.zero_rest = a.zero_rest;
   p.status = dev.status;
   switch (a.c.format) {
-    case WFATTN_CACHE_F32: return launch_rows_f<WFATTN_CACHE_F32, kWrite>(p, a.f32, dev, stream);
-    case WFATTN_CACHE_BF16: return launch_rows_f<WFATTN_CACHE_BF16, kWrite>(p, a.f32, dev, stream);
-    case WFATTN_CACHE_E4M3: return launch_rows_f<WFATTN_CACHE_E4M3, kWrite>(p, a.f32, dev, stream);
-    default: return launch_rows_f<WFATTN_CACHE_INT4, kWrite>(p, a.f32, dev, stream);
+    case WFATTN_CACHE_F32: return launch_rows_f<WFATTN_CACHE_F32, kWrite>(p, a.f32, stream);
+    case WFATTN_CACHE_BF16: return launch_rows_f<WFATTN_CACHE_BF16, kWrite>(p, a.f32, stream);
+    case WFATTN_CACHE_E4M3: return launch_rows_f<WFATTN_CACHE_E4M3, kWrite>(p, a.f32, stream);
+    default: return launch_rows_f<WFATTN_CACHE_INT4, kWrite>(p, a.f32, stream);
   }
 }
 

@@ -30,9 +30,10 @@
 // shares to a grid of kCtas CTAs an SM, whatever the lengths.  A CTA streams
 // its units through a ring of cp.async stages without regard to where a
 // segment (one sequence, head and tile) ends; a segment that lies in one CTA
-// is written out directly, the others as partials (maximum, sum, unnormalised
-// output) that a second kernel joins in order: no atomics, the same bits every
-// time.  Four warps split the keys of a unit or, with more rows, the rows.
+// is written out directly.  Of the others every CTA writes its part (maximum,
+// sum, unnormalised output) to the workspace, and the CTA whose part is the last
+// to arrive, by a counter, joins them in their order: the same bits every time.
+// Four warps split the keys of a unit or, with more rows, the rows.
 #pragma once
 
 #include <float.h>
@@ -46,12 +47,9 @@ namespace tree {
 constexpr int kThreads = 128, kWarps = 4;
 constexpr int kMaxSms = 148;  // CTAs are dealt for at most this many SMs
 
-// Per CTA, written by every launch before the joining kernel reads it.
-struct Desc {
-  int64_t seg;  // segment that begins in this CTA and goes on in later ones, or -1
-  int32_t last;  // its last CTA
-  int32_t head;  // 1: the CTA's first piece is a partial (slot 0)
-};
+// Counters of arrived parts, at the start of the workspace: zero before the
+// first launch on it, and left at zero by each (atomicInc wraps).
+constexpr int kCounters = WFATTN_TREE_DECODE_ZEROED / sizeof(unsigned int);  // one a CTA
 
 struct Params {
   CacheView c;
@@ -67,8 +65,8 @@ struct Params {
   const uint64_t *tree;
   int64_t tree_stride;
   float scale_log2;
-  Desc *desc;
-  float *part;   // [ctas][2][rows][D], then [ctas][2][rows][2]
+  unsigned int *arrived;  // [kCounters]
+  float *part;   // [ctas][2][rows][D], then [ctas][2][rows][2] (maximum, sum)
   unsigned int *status;
 };
 
@@ -416,7 +414,8 @@ struct Warp {
 #pragma unroll
           for (int i = 0; i < kRun; i += 8) {
             float v[8];
-            cache_load8<WFATTN_CACHE_BF16>(reinterpret_cast<const uint8_t *>(q16 + from + i), 0, v);
+            const uint4 w = *reinterpret_cast<const uint4 *>(q16 + from + i);
+            cache_values8<WFATTN_CACHE_BF16>(&w.x, 0, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[i + e] = v[e];
           }
@@ -992,8 +991,100 @@ __device__ __forceinline__ void store_out4(const Params &p, uint8_t *row, int d,
   }
 }
 
+// Counts this CTA's part of a segment, which its threads have written, as
+// arrived, and joins the parts if it is the last: thread groups take a float4
+// column of a row each and every kth part, eight in flight, and meet in `room`
+// (4 KB of shared memory).  Not inlined: a CTA comes here twice at most, and the
+// loads in flight would cost the main loop its registers.
 template <class C>
-__global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params p) {
+__device__ __noinline__ void join(const Params &p, const Cursor<C::kKeys> &cur, int first,
+                                     int last, int parts, int64_t all, uint8_t *room) {
+  __shared__ int is_last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    is_last = atomicInc(p.arrived + first, parts - 1) == (unsigned)(parts - 1);
+    __threadfence();
+  }
+  __syncthreads();
+  if (!is_last) return;
+  constexpr int kCols = C::D / 4, kAtOnce = 8;
+  const int rows = min(C::kRows, p.R - cur.tile * C::kRows);
+  const float *ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D;
+  const int items = rows * kCols;
+  const int groups = items >= kThreads ? 1 : kThreads / items;  // 1, 2, 4, 8 or fewer
+  const int group = items >= kThreads ? 0 : threadIdx.x / items;
+  const bool sparse = all < p.ctas;  // some CTAs have no unit
+#pragma unroll 1
+  for (int x = items >= kThreads ? threadIdx.x : threadIdx.x % items; x < items; x += kThreads) {
+    const int r = x / kCols, dd = x % kCols * 4;
+    float m = -FLT_MAX, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (group < groups) {
+#pragma unroll 1
+      for (int c0 = first + group; c0 <= last; c0 += groups * kAtOnce) {
+        float2 s[kAtOnce];
+        float4 z[kAtOnce];
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          const int c = c0 + j * groups;
+          s[j] = make_float2(-FLT_MAX, 0.f);
+          z[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (c <= last && !(sparse && all * c / p.ctas == all * (c + 1) / p.ctas)) {
+            const int64_t at = (int64_t)(c * 2 + (c == first)) * C::kRows + r;
+            s[j] = __ldcg(reinterpret_cast<const float2 *>(ml + at * 2));
+            z[j] = __ldcg(reinterpret_cast<const float4 *>(p.part + at * C::D + dd));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) top = fmaxf(top, s[j].x);
+        const float f = ptx::ex2_approx(m - top);
+        m = top;
+        l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          const float w = ptx::ex2_approx(s[j].x - m);
+          l = fmaf(s[j].y, w, l);
+          o.x = fmaf(z[j].x, w, o.x), o.y = fmaf(z[j].y, w, o.y);
+          o.z = fmaf(z[j].z, w, o.z), o.w = fmaf(z[j].w, w, o.w);
+        }
+      }
+    }
+    if (groups > 1) {  // one pass: items < kThreads
+      float4 *sums = reinterpret_cast<float4 *>(room);
+      float2 *mls = reinterpret_cast<float2 *>(room + kThreads * sizeof(float4));
+      if (group < groups) {
+        sums[threadIdx.x] = o;
+        mls[threadIdx.x] = make_float2(m, l);
+      }
+      __syncthreads();
+      if (group > 0) return;
+      for (int y = 1; y < groups; ++y) m = fmaxf(m, mls[y * items + x].x);
+      const float f = ptx::ex2_approx(mls[x].x - m);
+      l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+      for (int y = 1; y < groups; ++y) {
+        const float2 s = mls[y * items + x];
+        const float4 z = sums[y * items + x];
+        const float w = ptx::ex2_approx(s.x - m);
+        l = fmaf(s.y, w, l);
+        o.x = fmaf(z.x, w, o.x), o.y = fmaf(z.y, w, o.y);
+        o.z = fmaf(z.z, w, o.z), o.w = fmaf(z.w, w, o.w);
+      }
+    }
+    if (group > 0) return;
+    bool live;
+    uint8_t *to = out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, C::kF32 ? 4 : 2, live);
+    const bool some = live && l != 0.f;
+    const float inv = 1.f / l;
+    store_out4<C::kF32>(p, to, dd,
+                        some ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv)
+                             : make_float4(0.f, 0.f, 0.f, 0.f));
+  }
+}
+
+template <class C>
+__global__ void __launch_bounds__(kThreads, C::kCtas) tree_decode_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   float *stats = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
   const uint32_t ring = ptx::smem_u32(smem);
@@ -1003,13 +1094,6 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
   int64_t begin, end, all;
   Cursor<C::kKeys> cur = share<C::kKeys>(p, begin, end, all), ahead = cur;
   const int64_t units = end - begin;
-  if (threadIdx.x == 0) {
-    Desc d;
-    d.seg = -1;
-    d.last = 0;
-    d.head = units > 0 && cur.u > 0;
-    p.desc[blockIdx.x] = d;
-  }
   if (units <= 0) return;
 
   // Who loads what of a unit: where every warp reads keys of its own, each warp
@@ -1102,223 +1186,149 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) split_kernel(const Params 
 
 #pragma unroll 1
   for (int i = 0; i < C::kStages - 1; ++i) fetch();
-  Warp<C> w;
-  bool fresh = true;         // the segment's queries are not loaded yet
-  bool headed = cur.u == 0;  // it begins in this CTA
+  bool headed = cur.u == 0;  // the segment begins in this CTA
   uint32_t st = 0;
+  int64_t i = 0;
 #pragma unroll 1
-  for (int64_t i = 0; i < units; ++i) {
-    if (fresh) w.load_q(p, cur.b, cur.h, cur.tile * C::kRows + rw * 8 * C::kNT);
-    fresh = false;
-    cp_async_wait<C::kStages - 2>();
-    // the unit is here, and the stage refilled next has been read
-    if constexpr (kOwn)
-      __syncwarp();
-    else
-      __syncthreads();
-    fetch();
-    const int key0 = cur.u * C::kKeys;
+  while (i < units) {  // a segment, or the part of it in this share
+    Warp<C> w;
+    w.load_q(p, cur.b, cur.h, cur.tile * C::kRows + rw * 8 * C::kNT);
+    bool done;
 #pragma unroll 1
-    for (int j = 0; j < C::kGroups; ++j) {
-      const int tr = 16 * C::kKT * (kw + C::kKW * j);
-      if (tr >= cur.s.total - key0) break;
-      w.group(ring + st, tr, key0 + tr, cur.s);
+    while (true) {  // a unit
+      cp_async_wait<C::kStages - 2>();
+      // the unit is here, and the stage refilled next has been read
+      if constexpr (kOwn)
+        __syncwarp();
+      else
+        __syncthreads();
+      fetch();
+      const int key0 = cur.u * C::kKeys;
+#pragma unroll 1
+      for (int j = 0; j < C::kGroups; ++j) {
+        const int tr = 16 * C::kKT * (kw + C::kKW * j);
+        if (tr >= cur.s.total - key0) break;
+        w.group(ring + st, tr, key0 + tr, cur.s);
+      }
+      done = cur.u + 1 == cur.s.units;
+      if (done || i + 1 == units) break;
+      ++i;
+      ++cur.u;
+      st = st == (C::kStages - 1) * C::kStage ? 0 : st + C::kStage;
     }
 
-    const bool done = cur.u + 1 == cur.s.units;
-    if (done || i + 1 == units) {
-      const bool whole = done && headed;
-      const int g = lane >> 2, t = lane & 3;
-      const float back = C::kScaled ? 1.f / w.vinv : 1.f;
+    const bool whole = done && headed;
+    const int g = lane >> 2, t = lane & 3;
+    const float back = C::kScaled ? 1.f / w.vinv : 1.f;
 #pragma unroll
-      for (int nt = 0; nt < C::kNT; ++nt)
+    for (int nt = 0; nt < C::kNT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            w.l[nt][e] += __shfl_xor_sync(0xffffffffu, w.l[nt][e], x);
-            if constexpr (C::kFmt == WFATTN_CACHE_INT4)
-              w.om[nt][e] += __shfl_xor_sync(0xffffffffu, w.om[nt][e], x);
-          }
-          if constexpr (C::kScaled) {
+        for (int x = 4; x < 32; x <<= 1) {
+          w.l[nt][e] += __shfl_xor_sync(0xffffffffu, w.l[nt][e], x);
+          if constexpr (C::kFmt == WFATTN_CACHE_INT4)
+            w.om[nt][e] += __shfl_xor_sync(0xffffffffu, w.om[nt][e], x);
+        }
+        if constexpr (C::kScaled) {
 #pragma unroll
-            for (int mt = 0; mt < C::kMt; ++mt) {
-              w.o[nt][mt][e] = w.o[nt][mt][e] * back + w.om[nt][e];
-              w.o[nt][mt][2 + e] = w.o[nt][mt][2 + e] * back + w.om[nt][e];
-            }
+          for (int mt = 0; mt < C::kMt; ++mt) {
+            w.o[nt][mt][e] = w.o[nt][mt][e] * back + w.om[nt][e];
+            w.o[nt][mt][2 + e] = w.o[nt][mt][2 + e] * back + w.om[nt][e];
           }
         }
-      const int slot = headed ? 1 : 0;
-      float *part = p.part + (int64_t)(blockIdx.x * 2 + slot) * C::kRows * C::D;
-      float *part_ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D +
-                       (int64_t)(blockIdx.x * 2 + slot) * C::kRows * 2;
-      constexpr int kSize = C::kF32 ? 4 : 2;
-      // The warps' sums meet in the stage just read: rows of O, and beside them
-      // maximum and sum.  (With all the keys in one warp this only turns the
-      // fragments into rows.)
-      __syncthreads();
-      float *mine = reinterpret_cast<float *>(smem + st) + warp * 8 * C::kNT * C::kOStride;
+      }
+    const int slot = headed ? 1 : 0;
+    float *part = p.part + (int64_t)(blockIdx.x * 2 + slot) * C::kRows * C::D;
+    float *part_ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D +
+                     (int64_t)(blockIdx.x * 2 + slot) * C::kRows * 2;
+    constexpr int kSize = C::kF32 ? 4 : 2;
+    // The warps' sums meet in the stage just read: rows of O, and beside them
+    // maximum and sum.  (With all the keys in one warp this only turns the
+    // fragments into rows.)
+    __syncthreads();
+    float *mine = reinterpret_cast<float *>(smem + st) + warp * 8 * C::kNT * C::kOStride;
 #pragma unroll
-      for (int nt = 0; nt < C::kNT; ++nt)
+    for (int nt = 0; nt < C::kNT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = 8 * nt + 2 * t + e;
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * nt + 2 * t + e;
 #pragma unroll
-          for (int mt = 0; mt < C::kMt; ++mt)
+        for (int mt = 0; mt < C::kMt; ++mt)
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
-              mine[r * C::kOStride + o_index<C>(mt, g, y)] = w.o[nt][mt][2 * y + e];
-          if (g == 0) {
-            stats[(warp * 8 * C::kNT + r) * 2] = w.m[nt][e];
-            stats[(warp * 8 * C::kNT + r) * 2 + 1] = w.l[nt][e];
-          }
+          for (int y = 0; y < 2; ++y)
+            mine[r * C::kOStride + o_index<C>(mt, g, y)] = w.o[nt][mt][2 * y + e];
+        if (g == 0) {
+          stats[(warp * 8 * C::kNT + r) * 2] = w.m[nt][e];
+          stats[(warp * 8 * C::kNT + r) * 2 + 1] = w.l[nt][e];
         }
-      __syncthreads();
+      }
+    __syncthreads();
 #pragma unroll 1
-      for (int x = threadIdx.x; x < C::kRows * C::D / 4; x += kThreads) {
-        const int r = x / (C::D / 4), dd = x % (C::D / 4) * 4;
-        const int at0 = r / (8 * C::kNT) * C::kKW * 8 * C::kNT + r % (8 * C::kNT);
-        float m = -FLT_MAX, l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x = threadIdx.x; x < C::kRows * C::D / 4; x += kThreads) {
+      const int r = x / (C::D / 4), dd = x % (C::D / 4) * 4;
+      const int at0 = r / (8 * C::kNT) * C::kKW * 8 * C::kNT + r % (8 * C::kNT);
+      float m = -FLT_MAX, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int y = 0; y < C::kKW; ++y) m = fmaxf(m, stats[(at0 + y * 8 * C::kNT) * 2]);
+      for (int y = 0; y < C::kKW; ++y) m = fmaxf(m, stats[(at0 + y * 8 * C::kNT) * 2]);
 #pragma unroll
-        for (int y = 0; y < C::kKW; ++y) {
-          const int at = at0 + y * 8 * C::kNT;
-          const float f = ptx::ex2_approx(stats[at * 2] - m);
-          const float4 z =
-              *reinterpret_cast<const float4 *>(smem + st + (at * C::kOStride + dd) * 4);
-          l = fmaf(stats[at * 2 + 1], f, l);
-          o.x = fmaf(z.x, f, o.x), o.y = fmaf(z.y, f, o.y);
-          o.z = fmaf(z.z, f, o.z), o.w = fmaf(z.w, f, o.w);
+      for (int y = 0; y < C::kKW; ++y) {
+        const int at = at0 + y * 8 * C::kNT;
+        const float f = ptx::ex2_approx(stats[at * 2] - m);
+        const float4 z =
+            *reinterpret_cast<const float4 *>(smem + st + (at * C::kOStride + dd) * 4);
+        l = fmaf(stats[at * 2 + 1], f, l);
+        o.x = fmaf(z.x, f, o.x), o.y = fmaf(z.y, f, o.y);
+        o.z = fmaf(z.z, f, o.z), o.w = fmaf(z.w, f, o.w);
+      }
+      if (whole) {
+        bool live;
+        uint8_t *to =
+            out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, kSize, live);
+        if (to) {
+          const bool some = live && l != 0.f;
+          const float inv = 1.f / l;
+          store_out4<C::kF32>(p, to, dd,
+                              some ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv)
+                                   : make_float4(0.f, 0.f, 0.f, 0.f));
         }
-        if (whole) {
-          bool live;
-          uint8_t *to =
-              out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, kSize, live);
-          if (to) {
-            const bool some = live && l != 0.f;
-            const float inv = 1.f / l;
-            store_out4<C::kF32>(p, to, dd,
-                                some ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv)
-                                     : make_float4(0.f, 0.f, 0.f, 0.f));
-          }
-        } else {
-          *reinterpret_cast<float4 *>(part + r * C::D + dd) = o;
-          if (dd == 0) {
-            part_ml[2 * r] = m;
-            part_ml[2 * r + 1] = l;
-          }
+      } else {
+        *reinterpret_cast<float4 *>(part + r * C::D + dd) = o;
+        if (dd == 0) {
+          part_ml[2 * r] = m;
+          part_ml[2 * r + 1] = l;
         }
       }
-      // the stage may be refilled once all have read it (with common loads the
-      // next unit's barrier says so)
-      if constexpr (kOwn) __syncthreads();
-      if (!done && headed && threadIdx.x == 0) {
-        // goes on: unit s lies in CTA ((s + 1) * ctas - 1) / all
-        const int64_t last = begin + i + (cur.s.units - 1 - cur.u);
-        p.desc[blockIdx.x].seg = ((int64_t)cur.b * p.c.H + cur.h) * p.RT + cur.tile;
-        p.desc[blockIdx.x].last = (int32_t)(((last + 1) * p.ctas - 1) / all);
-      }
-      fresh = true;
-      headed = true;
     }
+    if (!whole) {
+      // Units s.. of the segment lie in CTAs x with all x / ctas <= s: the
+      // one of s is ((s + 1) ctas - 1) / all.  CTAs without units are passed
+      // over; there are none, or no CTA has two.
+      const int64_t s0 = begin + i - cur.u;
+      const int first_cta = headed ? (int)blockIdx.x : (int)(((s0 + 1) * p.ctas - 1) / all);
+      const int last_cta = (int)(((s0 + cur.s.units) * p.ctas - 1) / all);
+      const int parts = min(last_cta - first_cta + 1, cur.s.units);
+      join<C>(p, cur, first_cta, last_cta, parts, all, smem + st);
+    }
+    // the stage may be refilled once all have read it (with common loads the
+    // next unit's barrier says so)
+    if constexpr (kOwn) __syncthreads();
+    headed = true;
     st = st == (C::kStages - 1) * C::kStage ? 0 : st + C::kStage;
     cur.next(p);
+    ++i;
   }
   cp_async_wait<0>();
-}
-
-// Joins the partials of a segment that more than one CTA worked on: block
-// (x, y) the row y of the one that begins in CTA x.  Warps take every fourth
-// partial, eight loads in flight each; then the four sums are joined.
-template <int D, bool kF32, int kRows, int kKeys>
-__global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
-  __shared__ float sums[kWarps][D + 2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Desc desc = p.desc[blockIdx.x];
-  if (desc.seg < 0) return;
-  const int64_t bh = desc.seg / p.RT, b = bh / p.c.H, h = bh - b * p.c.H;
-  const Seq s = sequence<kKeys>(p, (int)b, false);
-  const int row = blockIdx.y;
-  bool live = false;
-  uint8_t *to = out_row(p, b, h, (int)(desc.seg - bh * p.RT) * kRows + row, s.n, kF32 ? 4 : 2, live);
-  if (!to) return;
-  constexpr int kVals = D / 32;
-  const float *ml = p.part + (int64_t)p.ctas * 2 * kRows * D;
-  const int first = (int)blockIdx.x, n = desc.last - first + 1;
-  float m = -FLT_MAX, l = 0.f, o[kVals];
-#pragma unroll
-  for (int i = 0; i < kVals; ++i) o[i] = 0.f;
-  for (int c0 = warp; c0 < n; c0 += 32 * kWarps) {
-    // lane i: piece c0 + 4 i
-    const int c = c0 + kWarps * lane;
-    float mc = -FLT_MAX, lc = 0.f;
-    if (c < n && (c == 0 || p.desc[first + c].head)) {
-      const float *at = ml + ((int64_t)((first + c) * 2 + (c == 0)) * kRows + row) * 2;
-      mc = at[0];
-      lc = at[1];
-    }
-    float top = fmaxf(m, mc);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float f = ptx::ex2_approx(m - top);
-    const float w = lc == 0.f && mc == -FLT_MAX ? 0.f : ptx::ex2_approx(mc - top);
-    float lw = lc * w;
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, x);
-    l = l * f + lw;
-    m = top;
-#pragma unroll
-    for (int i = 0; i < kVals; ++i) o[i] *= f;
-    const int count = min(32, (n - c0 + kWarps - 1) / kWarps);
-    const unsigned some = __ballot_sync(0xffffffffu, w != 0.f);
-    for (int j = 0; j < count; j += 8) {
-      float x[8][kVals];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int cc = c0 + kWarps * (j + k);
-        const bool use = j + k < 32 && (some >> ((j + k) & 31) & 1);
-        const float *at = p.part + ((int64_t)((first + cc) * 2 + (cc == 0)) * kRows + row) * D +
-                          lane * kVals;
-#pragma unroll
-        for (int i = 0; i < kVals; ++i) x[k][i] = use ? at[i] : 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float wk = __shfl_sync(0xffffffffu, w, (j + k) & 31);
-#pragma unroll
-        for (int i = 0; i < kVals; ++i) o[i] = fmaf(x[k][i], wk, o[i]);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kVals; ++i) sums[warp][lane * kVals + i] = o[i];
-  if (lane == 0) {
-    sums[warp][D] = m;
-    sums[warp][D + 1] = l;
-  }
-  __syncthreads();
-  if ((int)threadIdx.x >= D) return;
-  float top = sums[0][D];
-#pragma unroll
-  for (int i = 1; i < kWarps; ++i) top = fmaxf(top, sums[i][D]);
-  float total = 0.f, x = 0.f;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    const float f = ptx::ex2_approx(sums[i][D] - top);
-    total = fmaf(sums[i][D + 1], f, total);
-    x = fmaf(sums[i][threadIdx.x], f, x);
-  }
-  store_out<kF32>(to, threadIdx.x, live && total != 0.f ? x / total : 0.f);
 }
 
 // ------------------------------------------------------------------ launch
 
 template <class C>
 size_t workspace_bytes() {
-  const size_t ctas = (size_t)kMaxSms * C::kCtas;
-  return ctas * (sizeof(Desc) + 2 * C::kRows * (C::D + 2) * sizeof(float));
+  static_assert(C::kCtas * kMaxSms <= kCounters && C::kStage >= 24 * kThreads, "join");
+  return kCounters * sizeof(unsigned int) +
+         (size_t)kMaxSms * C::kCtas * 2 * C::kRows * (C::D + 2) * sizeof(float);
 }
 
 template <class C>
@@ -1333,16 +1343,12 @@ cudaError_t launch(Params p, void *workspace, const DeviceInfo &dev, cudaStream_
   const int64_t units = (p.c.L + C::kKeys - 1) / C::kKeys;  // of a segment, at most
   const int64_t most = (dev.sm_count < kMaxSms ? dev.sm_count : kMaxSms) * C::kCtas;
   p.ctas = (int)imin64(most, units > most ? most : units * imin64(segs, most));
-  p.desc = static_cast<Desc *>(workspace);
-  p.part = reinterpret_cast<float *>(p.desc + most);
-  cudaError_t err = ensure_smem_attr(reinterpret_cast<const void *>(split_kernel<C>), C::kSmem,
-                                     dev.device);
+  p.arrived = static_cast<unsigned int *>(workspace);
+  p.part = reinterpret_cast<float *>(p.arrived + kCounters);
+  cudaError_t err = ensure_smem_attr(reinterpret_cast<const void *>(tree_decode_kernel<C>),
+                                     C::kSmem, dev.device);
   if (err != cudaSuccess) return err;
-  split_kernel<C><<<p.ctas, kThreads, C::kSmem, stream>>>(p);
-  err = cudaGetLastError();
-  if (err != cudaSuccess || units == 1) return err;  // no segment is split
-  join_kernel<C::D, C::kF32, C::kRows, C::kKeys>
-      <<<dim3(p.ctas, C::kRows < p.R ? C::kRows : p.R), kThreads, 0, stream>>>(p);
+  tree_decode_kernel<C><<<p.ctas, kThreads, C::kSmem, stream>>>(p);
   return cudaGetLastError();
 }
 

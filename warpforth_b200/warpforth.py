@@ -187,10 +187,21 @@ def attention_multicast_ptr(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o
 
 
 class DecodeWorkspace:
-    """Caller-owned scratch for ``decode`` (grown on demand, reused across calls)."""
+    """Caller-owned scratch for ``decode`` and ``tree_decode`` (grown on demand, reused across
+    calls; calls that share one must be ordered on one stream)."""
 
     def __init__(self) -> None:
         self.buffer: torch.Tensor | None = None
+        self.tree_buffer: torch.Tensor | None = None
+
+    def get_tree(self, nbytes: int, device: torch.device) -> torch.Tensor:
+        """``tree_decode``'s own scratch: it begins with counters that only its calls may write."""
+        buffer = self.tree_buffer
+        if buffer is None or buffer.numel() < nbytes or buffer.device != device:
+            buffer = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            buffer[:_lib.TREE_DECODE_ZEROED].zero_()
+            self.tree_buffer = buffer
+        return buffer
 
     def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
         if self.buffer is None or self.buffer.numel() < nbytes or self.buffer.device != device:
