@@ -199,7 +199,8 @@ def cache_read(cache: KVCache, starts: torch.Tensor, rows: int, *,
         dtype = dtype or (torch.float32 if cache.fmt == "f32" else torch.bfloat16)
         if dtype not in _DTYPES:
             raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
-        k, v = torch.empty((2, *shape), dtype=dtype, device=cache.device)
+        k = torch.empty(shape, dtype=dtype, device=cache.device)
+        v = torch.empty_like(k)
         ks = vs = None  # contiguous
     else:
         k, v = out
@@ -228,7 +229,7 @@ def cache_keep(cache: KVCache, lens: torch.Tensor, path: torch.Tensor, *,
     depth = path.shape[1]
     steps = _ints("path", path, (cache.batch, depth), cache)
     if out is None:
-        out = lens.new_empty(cache._batch_shape)
+        out = torch.empty_like(lens)
     _run(cache, _lib.load().wfattn_cache_keep, at, depth, steps, path.stride(0),
          None if counts is None else _ints("counts", counts, cache._batch_shape, cache),
          _ints("out", out, cache._batch_shape, cache))

@@ -148,12 +148,14 @@ __device__ __forceinline__ uint32_t row_top(const Raw<kF32> &x) {
 #pragma unroll
     for (int m = 1; m < kLanes; m <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
     return top;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __vmaxu2(top, x.w[i] & 0x7fff7fffu);
+#pragma unroll
+    for (int m = 1; m < kLanes; m <<= 1)
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, m));
+    return max(top << 16, top & 0xffff0000u);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = __vmaxu2(top, x.w[i] & 0x7fff7fffu);
-#pragma unroll
-  for (int m = 1; m < kLanes; m <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, m));
-  return max(top << 16, top & 0xffff0000u);
 }
 
 // x as the nearest bf16 not above (kDown) or not below it; x finite.

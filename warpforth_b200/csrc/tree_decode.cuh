@@ -27,7 +27,8 @@
 //
 // Work: a unit is kKeys keys of one (sequence, cache head, tile of query
 // rows); the units of all sequences in order are dealt in equal contiguous
-// shares to a grid of kCtas CTAs an SM, whatever the lengths.  A CTA streams
+// shares to a grid of kCtas CTAs an SM, whatever the lengths (short segments
+// whole).  A CTA streams
 // its units through a ring of cp.async stages without regard to where a
 // segment (one sequence, head and tile) ends; a segment that lies in one CTA
 // is written out directly.  Of the others every CTA writes its part (maximum,
@@ -306,17 +307,28 @@ struct Cursor {
   }
 };
 
-// Finds this CTA's share [begin, end) of the units and where it begins.
+// Finds this CTA's share [begin, end) of the units and where it begins.  Where
+// no segment has more than kShort units the shares are whole segments: a few
+// units' difference in load costs less than joining parts.
+constexpr int kShort = 4;
+
 template <int kKeys>
 __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, int64_t &end,
                                                int64_t &all) {
-  __shared__ int64_t warp_sum[kWarps], found[2];
+  __shared__ int64_t warp_sum[kWarps], offset, stop;
+  __shared__ Cursor<kKeys> found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int B = (int)p.c.B, per = (B + kThreads - 1) / kThreads;
   const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
   const int64_t HR = p.c.H * p.RT;
   int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += sequence<kKeys>(p, b, blockIdx.x == 0).units * HR;
+  int longest = 0;
+  Seq s;
+  for (int b = b0; b < b1; ++b) {
+    s = sequence<kKeys>(p, b, blockIdx.x == 0);
+    mine += s.units * HR;
+    longest = max(longest, s.units);
+  }
   int64_t upto = mine;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
@@ -324,35 +336,38 @@ __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, 
     if (lane >= x) upto += y;
   }
   if (lane == 31) warp_sum[warp] = upto;
-  __syncthreads();
+  const bool whole = !__syncthreads_or(longest > kShort);
   all = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) upto += warp_sum[w];
     all += warp_sum[w];
   }
-  begin = all * blockIdx.x / p.ctas;
-  end = all * (blockIdx.x + 1) / p.ctas;
-  if (begin >= upto - mine && begin < upto) {
-    int64_t at = upto - mine;
-    int b = b0;
-    for (;; ++b) {
-      const int64_t n = sequence<kKeys>(p, b, false).units * HR;
-      if (begin < at + n) break;
-      at += n;
+  // unit (or, with whole segments, segment) where the share begins and ends
+  const int64_t total = whole ? B * HR : all;
+  const int64_t from = total * blockIdx.x / p.ctas, to = total * (blockIdx.x + 1) / p.ctas;
+  int64_t at = upto - mine;  // first unit of this thread's sequences
+  for (int b = b0; b < b1; ++b) {
+    if (per > 1) s = sequence<kKeys>(p, b, false);
+    const int64_t n = s.units * HR;
+    const int64_t lo = whole ? b * HR : at, hi = whole ? lo + HR : at + n;
+    if (from >= lo && from < hi) {
+      const int64_t into = whole ? (from - lo) * s.units : from - lo;
+      const int hr = (int)(into / s.units);
+      offset = at + into;
+      found.b = b;
+      found.u = (int)(into - (int64_t)hr * s.units);
+      found.h = hr / p.RT;
+      found.tile = hr - found.h * p.RT;
+      found.s = s;
     }
-    found[0] = b;
-    found[1] = begin - at;
+    if (to > lo && to <= hi) stop = whole ? at + (to - lo) * s.units : to;
+    at += n;
   }
   __syncthreads();
-  Cursor<kKeys> c;
-  c.b = (int)found[0];
-  c.s = sequence<kKeys>(p, c.b, false);
-  const int64_t hr = found[1] / c.s.units;
-  c.u = (int)(found[1] - hr * c.s.units);
-  c.h = (int)(hr / p.RT);
-  c.tile = (int)(hr - (int64_t)c.h * p.RT);
-  return c;
+  begin = offset;
+  end = to > from ? stop : begin;
+  return found;
 }
 
 // ------------------------------------------------------------------ kernel
