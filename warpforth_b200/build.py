@@ -41,7 +41,8 @@ SOURCES = ["wfattn_api.cu", "attn_f32.cu", "attn_f32_tc_sm100.cu", "attn_bf16_sm
            "tree_decode_e4m3_bf16.cu", "tree_decode_e4m3_f32.cu", "tree_decode_int4_bf16.cu",
            "tree_decode_int4_f32.cu", "tma_map.cu"]
 HEADERS = ["wfattn_internal.h", "sm100_ptx.cuh", "tma_map.h", "exp2_poly.cuh",
-           "cache_format.cuh", "tree_decode.cuh"]
+           "cache_format.cuh", "tree_decode.cuh",
+           "tree_decode_wide.cuh", "tree_decode_launch.cuh"]
 
 
 def nvcc() -> str:

@@ -82,6 +82,7 @@ template <int kFmt_, int D_, bool kF32_, int kNT_, int kRW_>
 struct Cfg {
   static constexpr int kFmt = kFmt_, D = D_, kNT = kNT_, kRW = kRW_, kKW = kWarps / kRW_;
   static constexpr bool kF32 = kF32_;  // queries and output
+  static constexpr bool kWide = false;
   static constexpr Kind kKind = kFmt == WFATTN_CACHE_F32    ? kTf32
                                 : kFmt == WFATTN_CACHE_BF16 ? kBf16
                                                             : kF16;
@@ -1012,8 +1013,8 @@ __device__ __forceinline__ void store_out4(const Params &p, uint8_t *row, int d,
 // (4 KB of shared memory).  Not inlined: a CTA comes here twice at most, and the
 // loads in flight would cost the main loop its registers.
 template <class C>
-__device__ __noinline__ void join(const Params &p, const Cursor<C::kKeys> &cur, int first,
-                                     int last, int parts, int64_t all, uint8_t *room) {
+__device__ __noinline__ void join(const Params &p, int b, int h, int tile, int n, int first,
+                                  int last, int parts, int64_t all, uint8_t *room) {
   __shared__ int is_last;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -1024,7 +1025,7 @@ __device__ __noinline__ void join(const Params &p, const Cursor<C::kKeys> &cur, 
   __syncthreads();
   if (!is_last) return;
   constexpr int kCols = C::D / 4, kAtOnce = 8;
-  const int rows = min(C::kRows, p.R - cur.tile * C::kRows);
+  const int rows = min(C::kRows, p.R - tile * C::kRows);
   const float *ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D;
   const int items = rows * kCols;
   const int groups = items >= kThreads ? 1 : kThreads / items;  // 1, 2, 4, 8 or fewer
@@ -1089,7 +1090,7 @@ __device__ __noinline__ void join(const Params &p, const Cursor<C::kKeys> &cur, 
     }
     if (group > 0) return;
     bool live;
-    uint8_t *to = out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, C::kF32 ? 4 : 2, live);
+    uint8_t *to = out_row(p, b, h, tile * C::kRows + r, n, C::kF32 ? 4 : 2, live);
     const bool some = live && l != 0.f;
     const float inv = 1.f / l;
     store_out4<C::kF32>(p, to, dd,
@@ -1099,7 +1100,8 @@ __device__ __noinline__ void join(const Params &p, const Cursor<C::kKeys> &cur, 
 }
 
 template <class C>
-__global__ void __launch_bounds__(kThreads, C::kCtas) tree_decode_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, C::kCtas) 
+    tree_decode_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   float *stats = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
   const uint32_t ring = ptx::smem_u32(smem);
@@ -1324,7 +1326,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) tree_decode_kernel(const P
       const int first_cta = headed ? (int)blockIdx.x : (int)(((s0 + 1) * p.ctas - 1) / all);
       const int last_cta = (int)(((s0 + cur.s.units) * p.ctas - 1) / all);
       const int parts = min(last_cta - first_cta + 1, cur.s.units);
-      join<C>(p, cur, first_cta, last_cta, parts, all, smem + st);
+      join<C>(p, cur.b, cur.h, cur.tile, cur.s.n, first_cta, last_cta, parts, all, smem + st);
     }
     // the stage may be refilled once all have read it (with common loads the
     // next unit's barrier says so)
@@ -1341,13 +1343,14 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) tree_decode_kernel(const P
 
 template <class C>
 size_t workspace_bytes() {
-  static_assert(C::kCtas * kMaxSms <= kCounters && C::kStage >= 24 * kThreads, "join");
+  static_assert(C::kCtas * kMaxSms <= kCounters, "a counter a CTA");
   return kCounters * sizeof(unsigned int) +
          (size_t)kMaxSms * C::kCtas * 2 * C::kRows * (C::D + 2) * sizeof(float);
 }
 
+// The parameters that go with the configuration.
 template <class C>
-cudaError_t launch(Params p, void *workspace, const DeviceInfo &dev, cudaStream_t stream) {
+void prepare(Params &p, void *workspace, const DeviceInfo &dev) {
   p.RT = (p.R + C::kRows - 1) / C::kRows;
   p.over_T = (uint32_t)(((uint64_t(1) << 32) + p.T - 1) / p.T);  // not used for T = 1
   const uintptr_t q16 = reinterpret_cast<uintptr_t>(p.q), o16 = reinterpret_cast<uintptr_t>(p.o);
@@ -1360,60 +1363,18 @@ cudaError_t launch(Params p, void *workspace, const DeviceInfo &dev, cudaStream_
   p.ctas = (int)imin64(most, units > most ? most : units * imin64(segs, most));
   p.arrived = static_cast<unsigned int *>(workspace);
   p.part = reinterpret_cast<float *>(p.arrived + kCounters);
-  cudaError_t err = ensure_smem_attr(reinterpret_cast<const void *>(tree_decode_kernel<C>),
-                                     C::kSmem, dev.device);
+}
+
+template <class C>
+cudaError_t launch(Params p, void *workspace, const DeviceInfo &dev, cudaStream_t stream) {
+  static_assert(C::kStage >= 24 * kThreads, "room to join in");
+  prepare<C>(p, workspace, dev);
+  const cudaError_t err = ensure_smem_attr(
+      reinterpret_cast<const void *>(tree_decode_kernel<C>), C::kSmem, dev.device);
   if (err != cudaSuccess) return err;
   tree_decode_kernel<C><<<p.ctas, kThreads, C::kSmem, stream>>>(p);
   return cudaGetLastError();
 }
 
-// Calls f with the configuration for R query rows a cache head: one 8-row tile
-// a warp while the rows fit, then two (not with f32 queries, whose fragments
-// are twice as large), then warps take different rows instead of keys.
-template <int kFmt, bool kF32, int D, class F>
-auto with_rows(int R, F f) {
-  if (R <= 8) return f(Cfg<kFmt, D, kF32, 1, 1>{});
-  if constexpr (kF32) {
-    if (R <= 16) return f(Cfg<kFmt, D, true, 1, 2>{});
-    return f(Cfg<kFmt, D, true, 1, 4>{});
-  } else {
-    if (R <= 16) return f(Cfg<kFmt, D, false, 2, 1>{});
-    if (R <= 32) return f(Cfg<kFmt, D, false, 2, 2>{});
-    return f(Cfg<kFmt, D, false, 2, 4>{});
-  }
-}
-
-template <int kFmt, bool kF32>
-size_t workspace_for(int D, int R) {
-  auto f = [](auto cfg) { return workspace_bytes<decltype(cfg)>(); };
-  return D == 64 ? with_rows<kFmt, kF32, 64>(R, f) : with_rows<kFmt, kF32, 128>(R, f);
-}
-
-template <int kFmt, bool kF32>
-cudaError_t launch_for(const Params &p, void *workspace, const DeviceInfo &dev,
-                       cudaStream_t stream) {
-  auto f = [&](auto cfg) { return launch<decltype(cfg)>(p, workspace, dev, stream); };
-  return p.c.D == 64 ? with_rows<kFmt, kF32, 64>(p.R, f) : with_rows<kFmt, kF32, 128>(p.R, f);
-}
-
 }  // namespace tree
-
-// One translation unit a row format and query type (tree_decode_*.cu).
-#define WFATTN_TREE_KINDS(X)                                                           \
-  X(f32_f32, WFATTN_CACHE_F32, true) X(bf16_bf16, WFATTN_CACHE_BF16, false)            \
-  X(e4m3_bf16, WFATTN_CACHE_E4M3, false) X(e4m3_f32, WFATTN_CACHE_E4M3, true)          \
-  X(int4_bf16, WFATTN_CACHE_INT4, false) X(int4_f32, WFATTN_CACHE_INT4, true)
-#define WFATTN_TREE_DECLARE(name, fmt, f32)                                            \
-  size_t tree_workspace_##name(int D, int R);                                          \
-  cudaError_t tree_launch_##name(const tree::Params &p, void *workspace,               \
-                                 const DeviceInfo &dev, cudaStream_t stream);
-WFATTN_TREE_KINDS(WFATTN_TREE_DECLARE)
-
-#define WFATTN_TREE_DEFINE(name, fmt, f32)                                             \
-  size_t tree_workspace_##name(int D, int R) { return tree::workspace_for<fmt, f32>(D, R); } \
-  cudaError_t tree_launch_##name(const tree::Params &p, void *workspace,               \
-                                 const DeviceInfo &dev, cudaStream_t stream) {         \
-    return tree::launch_for<fmt, f32>(p, workspace, dev, stream);                      \
-  }
-
 }  // namespace wfattn

@@ -1,7 +1,7 @@
 // tree_decode_sm100.cu -- attention of a tree of drafted tokens over a
-// key/value cache: choice of the kernel (tree_decode.cuh) by row format and
+// key/value cache: choice of the kernel (tree_decode_launch.cuh) by row format and
 // query type.
-#include "tree_decode.cuh"
+#include "tree_decode_launch.cuh"
 
 namespace wfattn {
 
