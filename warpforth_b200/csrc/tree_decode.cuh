@@ -316,11 +316,11 @@ constexpr int kShort = 4;
 template <int kKeys>
 __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, int64_t &end,
                                                int64_t &all) {
-  __shared__ int64_t warp_sum[kWarps], offset, stop;
+  __shared__ int64_t warp_sum[8], offset, stop;
   __shared__ Cursor<kKeys> found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int B = (int)p.c.B, per = (B + kThreads - 1) / kThreads;
-  const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
+  const int b0 = (int)imin64(B, (int64_t)threadIdx.x * per), b1 = min(B - b0, per) + b0;
   const int64_t HR = p.c.H * p.RT;
   int64_t mine = 0;
   int longest = 0;
@@ -339,8 +339,7 @@ __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, 
   if (lane == 31) warp_sum[warp] = upto;
   const bool whole = !__syncthreads_or(longest > kShort);
   all = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < (int)blockDim.x / 32; ++w) {
     if (w < warp) upto += warp_sum[w];
     all += warp_sum[w];
   }
@@ -1007,6 +1006,11 @@ __device__ __forceinline__ void store_out4(const Params &p, uint8_t *row, int d,
   }
 }
 
+// A barrier of the CTA's first kThreads threads (in one kernel all of them).
+__device__ __forceinline__ void rows_barrier() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+}
+
 // Counts this CTA's part of a segment, which its threads have written, as
 // arrived, and joins the parts if it is the last: thread groups take a float4
 // column of a row each and every kth part, eight in flight, and meet in `room`
@@ -1016,13 +1020,13 @@ template <class C>
 __device__ __noinline__ void join(const Params &p, int b, int h, int tile, int n, int first,
                                   int last, int parts, int64_t all, uint8_t *room) {
   __shared__ int is_last;
-  __syncthreads();
+  rows_barrier();
   if (threadIdx.x == 0) {
     __threadfence();
     is_last = atomicInc(p.arrived + first, parts - 1) == (unsigned)(parts - 1);
     __threadfence();
   }
-  __syncthreads();
+  rows_barrier();
   if (!is_last) return;
   constexpr int kCols = C::D / 4, kAtOnce = 8;
   const int rows = min(C::kRows, p.R - tile * C::kRows);
@@ -1074,7 +1078,7 @@ __device__ __noinline__ void join(const Params &p, int b, int h, int tile, int n
         sums[threadIdx.x] = o;
         mls[threadIdx.x] = make_float2(m, l);
       }
-      __syncthreads();
+      rows_barrier();
       if (group > 0) return;
       for (int y = 1; y < groups; ++y) m = fmaxf(m, mls[y * items + x].x);
       const float f = ptx::ex2_approx(mls[x].x - m);
