@@ -1,0 +1,99 @@
+"""Generation with drafted trees over a key/value cache: drafting and acceptance on the CPU, GPT-2 on
+the GPU.  Over an f32 cache the tokens are those of plain greedy generation; a difference is only
+accepted where the stock model's top two logits are within 1e-4 (a tie that f32 rounding may break
+either way)."""
+
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytest.importorskip("transformers")
+
+
+def test_drafts_follow_the_longest_earlier_match_first():
+    from warpforth_b200.gpt2 import draft_tree
+
+    tokens = [1, 2, 3, 9, 4, 5, 2, 3, 7, 8, 1, 2, 3]
+    drafted, parents = draft_tree(tokens, 64, depth=2)
+    # after 1 2 3 came 9 4; after 2 3 came 7 8 too
+    assert drafted == [3, 9, 4, 7, 8] and parents == [-1, 0, 1, 0, 3]
+    assert draft_tree(tokens, 1) == ([3], [-1])
+    drafted, parents = draft_tree(tokens, 4, depth=8)
+    assert drafted == [3, 9, 4, 5] and parents == [-1, 0, 1, 2]
+    assert draft_tree([5], 8) == ([5], [-1])
+    assert draft_tree([5, 6], 8) == ([6], [-1])
+    drafted, parents = draft_tree([4, 4, 4, 4], 8)
+    assert drafted[:2] == [4, 4] and all(p < i for i, p in enumerate(parents))
+
+
+def test_acceptance_walks_the_chosen_tokens():
+    from warpforth_b200.gpt2 import accepted_path
+
+    drafted, parents = [3, 9, 4, 7, 8], [-1, 0, 1, 0, 3]
+    assert accepted_path(drafted, parents, [7, 0, 0, 8, 1]) == [0, 3, 4]
+    assert accepted_path(drafted, parents, [9, 5, 0, 0, 0]) == [0, 1]
+    assert accepted_path(drafted, parents, [1, 4, 0, 8, 0]) == [0]
+    assert accepted_path([3], [-1], [3]) == [0]
+
+
+@pytest.fixture(scope="module")
+def gpt2():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from warpforth_b200 import gpt2
+
+    return gpt2
+
+
+def _assert_same_or_tie(model, want, got, prompt_len):
+    a, b = want[0].tolist(), got[0].tolist()
+    assert len(a) == len(b)
+    if a == b:
+        return
+    p = next(i for i in range(len(a)) if a[i] != b[i])
+    assert p >= prompt_len
+    with torch.no_grad():
+        logits = model(want[:, :p]).logits[0, -1].float()
+    top2 = torch.topk(logits, 2).values
+    assert float(top2[0] - top2[1]) < 1e-4, f"tokens diverge at {p} without a tie"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nodes,chunk", [(1, 512), (12, 512), (64, 7)])
+def test_drafted_tokens_are_the_greedy_ones(gpt2, nodes, chunk):
+    model = gpt2.random_gpt2(seed=1)
+    prompt = gpt2.synthetic_prompt(32, seed=1)
+    want = gpt2.generate(model, prompt, 64, use_cache=True)
+    got, runs = gpt2.generate_drafted(model, prompt, 64, nodes=nodes, prompt_chunk=chunk)
+    assert got.shape == (1, 96) and 1 <= runs <= 63
+    if nodes == 1:
+        assert runs == 63
+    _assert_same_or_tie(model, want, got, 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "int4"])
+def test_quantised_caches_generate(gpt2, fmt):
+    model = gpt2.random_gpt2(seed=2)
+    prompt = gpt2.synthetic_prompt(40, seed=2)
+    want = gpt2.generate(model, prompt, 1, use_cache=False)
+    got, _ = gpt2.generate_drafted(model, prompt, 20, nodes=8, cache=fmt)
+    assert got.shape == (1, 60)
+    assert got[0, :40].tolist() == prompt[0].tolist()
+    _assert_same_or_tie(model, want, got[:, :41], 40)  # the prompt is attended to unrounded
+
+
+@pytest.mark.gpu
+def test_generation_to_the_last_position(gpt2):
+    model = gpt2.random_gpt2(seed=3)
+    prompt = torch.arange(990).remainder(5)[None]
+    got, _ = gpt2.generate_drafted(model, prompt, 34, nodes=64, prompt_chunk=400)
+    assert got.shape == (1, 1024)
+    with pytest.raises(ValueError, match="positions"):
+        gpt2.generate_drafted(model, prompt, 35)
+    for bad in (dict(nodes=0), dict(nodes=65), dict(prompt_chunk=0)):
+        with pytest.raises(ValueError):
+            gpt2.generate_drafted(model, prompt[:, :4], 4, **bad)
+    with pytest.raises(ValueError, match="prompt"):
+        gpt2.generate_drafted(model, prompt[0], 4)

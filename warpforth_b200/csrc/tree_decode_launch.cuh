@@ -7,9 +7,12 @@ namespace wfattn {
 namespace tree {
 
 // Calls f with the configuration for R query rows a cache head.  mma.sync takes
-// 8 or 16 rows a warp; above that bf16 queries go to tcgen05, f32 queries, whose
-// products need more terms than tensor memory's operands have, to warps that
-// take different rows.
+// 8 or 16 rows a warp, then pairs of warps take different rows; above 32 rows
+// bf16 queries go to tcgen05, whose 128 rows cost the same however many are
+// there (8 cache heads, 196122 e4m3 keys of each in two sequences, head_dim
+// 128: 20 rows 162 us against 216 on tcgen05, 32 rows 177 against 231, 60 rows
+// 298 against 277, 244 rows 850 against 485).  f32 queries, whose products need
+// more terms, stay with warps that take different rows.
 template <int kFmt, bool kF32, int D, class F>
 auto with_rows(int R, F f) {
   if (R <= 8) return f(Cfg<kFmt, D, kF32, 1, 1>{});
@@ -18,6 +21,7 @@ auto with_rows(int R, F f) {
     return f(Cfg<kFmt, D, true, 1, 4>{});
   } else {
     if (R <= 16) return f(Cfg<kFmt, D, false, 2, 1>{});
+    if (R <= 32) return f(Cfg<kFmt, D, false, 2, 2>{});
     return f(WideCfg<kFmt, D>{});
   }
 }

@@ -14,8 +14,9 @@
 // maximum and the split of work are those of tree_decode.cuh; bf16 weights take
 // two products (two terms).
 //
-// Warps 0-3 turn scores into weights, warps 4-7 bring the rows of the units, and
-// one thread of warp 4 issues the products.  K and V have two buffers, and so
+// Warps 0-3 turn scores into weights, warps 4 and 5 bring the rows of the units,
+// warp 6 issues Q K^T and warp 7 P V (a product leaves a warp every 75 clocks or
+// so, which one warp's other work would add to).  K and V have two buffers, and so
 // have S and P, which share theirs (a thread has read its row of S before it
 // writes P): while the weights of unit i are made, Q K^T of i + 1 is done and
 // the rows of i + 2 follow P V of i.  TMEM columns: twice 64 for S and P, 64 or
@@ -30,7 +31,7 @@
 namespace wfattn {
 namespace tree {
 
-constexpr int kWideThreads = 2 * kThreads;
+constexpr int kWideThreads = 2 * kThreads, kLoaders = 64;
 
 template <int kFmt_, int D_>
 struct WideCfg {
@@ -43,16 +44,17 @@ struct WideCfg {
   static constexpr int kSlab = kKeys * 128;           // bytes of a slab of K or V
   static constexpr int kQSlab = kRows * 128;
   static constexpr int kBuf = 2 * kSlabs * kSlab;     // K and V of a unit
-  static constexpr int kPieces = kKeys * kRowBytes / 16 / kThreads;  // of K (and V) a thread
+  static constexpr int kPieces = kKeys * kRowBytes / 16 / kLoaders;  // of K (and V) a loader
   static constexpr int kWork = kSlabs * kQSlab + 2 * kBuf;
   static constexpr int kSmem = kWork + 1024;          // and room to align
   static constexpr uint32_t kColS = 0, kColO = 128, kCols = 256;  // P: as S; 64 a buffer
+  static_assert(kKeys == kLoaders, "a loader brings a row's scales");
   static_assert(kSmem <= 227 * 1024 / kCtas - 3072, "two CTAs an SM");
 };
 
-__device__ __forceinline__ uint32_t idesc_wide(bool bf16, bool b_mn) {
-  // M 128, N 64, f32 accumulation; formats f16 (0) or bf16 (1)
-  return ptx::idesc_bf16_f32(128, 64, 0, b_mn ? 1 : 0) & (bf16 ? ~0u : ~((1u << 7) | (1u << 10)));
+__device__ __forceinline__ uint32_t idesc_wide(bool bf16, int n, bool b_mn) {
+  // M 128, f32 accumulation; formats f16 (0) or bf16 (1)
+  return ptx::idesc_bf16_f32(128, n, 0, b_mn ? 1 : 0) & (bf16 ? ~0u : ~((1u << 7) | (1u << 10)));
 }
 
 // Byte offset of the 16-byte piece c (8 values) of row r in an operand whose
@@ -308,7 +310,8 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
     tree_decode_wide_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t raw_smem[];
   __shared__ struct {
-    uint64_t kv_full[2], s_full[2], p_full[2], q_full, o_done, drain;
+    // [i & 1] for unit i: a barrier's next phase waits for its last one's readers
+    uint64_t kv_full[2], s_full[2], p_full[2], o_done[2], q_full, drain[2];
     uint32_t tmem;
     int odd[2];  // the last unit in this buffer whose V is not finite
     // read in pairs
@@ -330,14 +333,14 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
   auto bar = [](uint64_t &b) { return ptx::smem_u32(&b); };
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      ptx::mbar_init(bar(sh.kv_full[i]), kThreads);
-      ptx::mbar_init(bar(sh.s_full[i]), 1);
+      ptx::mbar_init(bar(sh.kv_full[i]), kLoaders);
+      ptx::mbar_init(bar(sh.s_full[i]), 2);  // the products, and their issuer
       ptx::mbar_init(bar(sh.p_full[i]), kThreads);
+      ptx::mbar_init(bar(sh.o_done[i]), 1);
+      ptx::mbar_init(bar(sh.drain[i]), 1);
       sh.odd[i] = -1;
     }
     ptx::mbar_init(bar(sh.q_full), kThreads);
-    ptx::mbar_init(bar(sh.o_done), 1);
-    ptx::mbar_init(bar(sh.drain), 1);
     ptx::fence_barrier_init();
   }
   if (warp == 0) {
@@ -349,26 +352,97 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
   ptx::tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  if (warp >= 4) {
-    // ------------------------------------------- rows of K and V, and products
+  if (warp >= 6) {
+    // -------------------------------------------------------------- products
+    // The warp waits in step; lane 0 issues.
+    const uint32_t leader = (tid & 31) == 0;
+    auto wait = [&](uint64_t &b, uint32_t parity) {
+      return __all_sync(0xffffffffu, ptx::mbar_wait(bar(b), parity, p.status)) != 0;
+    };
+    bool ok = true;
+    if (warp == 6) {
+      const uint32_t idesc = idesc_wide(C::kBf16Rows, 64, false);
+      uint32_t segment = 0;
+#pragma unroll 1
+      for (int64_t i = 0; i < units && ok; ++i) {
+        const int buf = (int)(i & 1);
+        const bool first = i == 0 || cur.u == 0;
+        ok = wait(sh.kv_full[buf], (uint32_t)(i >> 1) & 1) &&
+             (!first || wait(sh.q_full, segment & 1)) &&
+             // S had P of the unit before last
+             (i < 2 || wait(sh.o_done[buf], (uint32_t)((i - 2) >> 1) & 1));
+        if (ok) {
+          ptx::tc_fence_after();
+          const uint32_t k = kv_at + buf * C::kBuf;
+#pragma unroll
+          for (int kk = 0; kk < C::D / 16; ++kk)
+            mma_ss_warp(leader, tmem + C::kColS + 64 * buf,
+                        ptx::smem_desc_sw128(q_at + kk / 4 * C::kQSlab + kk % 4 * 32, 16, 1024),
+                        ptx::smem_desc_sw128(k + kk / 4 * C::kSlab + kk % 4 * 32, 16, 1024), idesc,
+                        kk > 0);
+          commit_warp(leader, bar(sh.s_full[buf]));
+          // which has waited for the rows: so have, then, the weights' threads
+          if (leader) ptx::mbar_arrive(bar(sh.s_full[buf]));
+        }
+        segment += first;
+        cur.next(p);
+      }
+    } else {
+      const uint32_t idesc = idesc_wide(C::kBf16Rows, C::D, true);
+#pragma unroll 1
+      for (int64_t i = 0; i < units && ok; ++i) {
+        const int buf = (int)(i & 1);
+        bool first = i == 0 || cur.u == 0;
+        ok = wait(sh.kv_full[buf], (uint32_t)(i >> 1) & 1) &&
+             wait(sh.p_full[buf], (uint32_t)(i >> 1) & 1);
+        if (ok) {
+          ptx::tc_fence_after();
+          // the rows' threads have begun O themselves where V is odd
+          first = first && sh.odd[buf] != (int)(i & 0x7fffffff);
+          const uint32_t v = kv_at + buf * C::kBuf + C::kSlabs * C::kSlab;
+#pragma unroll
+          for (int term = C::kBf16Rows ? 1 : 0; term >= 0; --term)
+#pragma unroll
+            for (int kk = 0; kk < C::kKeys / 16; ++kk)  // 16 keys are two 8-row atoms
+              mma_ts_warp(leader, tmem + C::kColO, tmem + C::kColS + 64 * buf + 32 * term + kk * 8,
+                          ptx::smem_desc_sw128(v + kk * 2048, C::kSlab, 1024), idesc,
+                          !first || kk > 0 || (C::kBf16Rows && term == 0));
+          commit_warp(leader, bar(sh.o_done[buf]));
+        }
+        cur.next(p);
+      }
+    }
+    if (!ok) {  // every product issued has to end before the memory goes
+      commit_warp(leader, bar(sh.drain[warp - 6]));
+      ptx::mbar_wait_drain(bar(sh.drain[warp - 6]), 0);
+    }
+  } else if (warp >= 4) {
+    // --------------------------------------------------------- rows of K and V
     const int t = tid - kThreads;
     constexpr int kRowPieces = C::kRowBytes / 16;
     Cursor<C::kKeys> ahead = cur;
     uint4 held[C::kBf16Rows ? 1 : 2 * C::kPieces];  // codes of K, then of V
-    uint32_t held_scale = 0;  // threads 0-63: of K's rows, 64-127: V's
+    uint32_t held_k = 0, held_v = 0;                // scales of row t
     // The unit fetched next, from this thread's first piece, which the others
-    // follow kThreads pieces apart.
+    // follow kLoaders pieces apart.
     const int row0 = t / kRowPieces, col0 = t % kRowPieces;
-    constexpr int kApart = kThreads / kRowPieces;  // rows
-    static_assert(kThreads % kRowPieces == 0 && kApart % 8 == 0, "one swizzle for all pieces");
+    constexpr int kApart = kLoaders / kRowPieces;  // rows
+    static_assert(kLoaders % kRowPieces == 0 && kApart >= 4, "pieces");
+    // bytes from a piece of row row0 to the same of row row0 + j kApart; the
+    // swizzle changes where rows are 4 apart
+    auto to_piece = [&](uint32_t at, int j) {
+      return (at ^ (j * kApart & 7) << 4) + j * kApart * 128;
+    };
     const uint32_t to0 = kv_at + piece(row0, col0, C::kSlab);
-    const uint8_t *k_at, *v_at, *s_at = nullptr;
+    const uint8_t *k_at, *v_at, *ks_at = nullptr, *vs_at = nullptr;
     auto aim = [&]() {
       const int64_t row = ahead.b * p.c.sb + ahead.h * p.c.sh + (int64_t)ahead.u * C::kKeys;
       k_at = p.c.k + row * C::kRowBytes + t * 16;
       v_at = p.c.v + row * C::kRowBytes + t * 16;
-      if constexpr (C::kScaled)
-        s_at = (t < C::kKeys ? p.c.k_scale : p.c.v_scale) + (row + t % C::kKeys) * 4;
+      if constexpr (C::kScaled) {
+        ks_at = p.c.k_scale + (row + t) * 4;
+        vs_at = p.c.v_scale + (row + t) * 4;
+      }
     };
     aim();
     // Its rows, to the buffer (bf16) or to be held.
@@ -378,14 +452,14 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
       for (int j = 0; j < C::kPieces; ++j) {
         const bool use = row0 + j * kApart < live;
         if constexpr (C::kBf16Rows) {
-          const uint32_t to = to0 + buf * C::kBuf + j * kApart * 128;
-          cp_async16(to, use ? k_at + j * 16 * kThreads : p.c.k, use);
-          cp_async16(to + C::kSlabs * C::kSlab, use ? v_at + j * 16 * kThreads : p.c.v, use);
+          const uint32_t to = to_piece(to0 + buf * C::kBuf, j);
+          cp_async16(to, use ? k_at + j * 16 * kLoaders : p.c.k, use);
+          cp_async16(to + C::kSlabs * C::kSlab, use ? v_at + j * 16 * kLoaders : p.c.v, use);
         } else {
           held[j] = held[C::kPieces + j] = make_uint4(0, 0, 0, 0);
           if (use) {
-            held[j] = *reinterpret_cast<const uint4 *>(k_at + j * 16 * kThreads);
-            held[C::kPieces + j] = *reinterpret_cast<const uint4 *>(v_at + j * 16 * kThreads);
+            held[j] = *reinterpret_cast<const uint4 *>(k_at + j * 16 * kLoaders);
+            held[C::kPieces + j] = *reinterpret_cast<const uint4 *>(v_at + j * 16 * kLoaders);
           }
         }
       }
@@ -396,31 +470,36 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
 #pragma unroll
         for (int j = 0; j < C::kPieces; ++j)
           if (t % 8 == 0 && C::kKeys + row0 + j * kApart < live) {
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(k_at + kUnit + j * 16 * kThreads));
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(v_at + kUnit + j * 16 * kThreads));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(k_at + kUnit + j * 16 * kLoaders));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(v_at + kUnit + j * 16 * kLoaders));
           }
       } else {
-        held_scale = t % C::kKeys < live ? *reinterpret_cast<const uint32_t *>(s_at) : 0u;
+        held_k = held_v = 0;
+        if (t < live) {
+          held_k = *reinterpret_cast<const uint32_t *>(ks_at);
+          held_v = *reinterpret_cast<const uint32_t *>(vs_at);
+        }
       }
       if (ahead.next(p)) {
         if (ahead.b < (int)p.c.B) aim();
       } else {
         k_at += C::kKeys * C::kRowBytes;
         v_at += C::kKeys * C::kRowBytes;
-        if constexpr (C::kScaled) s_at += C::kKeys * 4;
+        if constexpr (C::kScaled) {
+          ks_at += C::kKeys * 4;
+          vs_at += C::kKeys * 4;
+        }
       }
     };
     // Puts the rows held into buffer `buf` as f16.  tail: what is not finite in V
     // becomes 0; returns whether there was any.
     auto place_rows = [&](int buf, bool tail) -> bool {
       bool odd = false;
-      const uint32_t at = kv_at + buf * C::kBuf;
       if constexpr (C::kBf16Rows) {
         if (tail) {  // this thread's own pieces have arrived
 #pragma unroll
           for (int j = 0; j < C::kPieces; ++j) {
-            const uint32_t from =
-                to0 + buf * C::kBuf + C::kSlabs * C::kSlab + j * kApart * 128;
+            const uint32_t from = to_piece(to0 + buf * C::kBuf, j) + C::kSlabs * C::kSlab;
             const uint4 y = lds128(from);
             uint32_t w[4] = {y.x, y.y, y.z, y.w};
             bool here = false;
@@ -434,10 +513,14 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
           }
         }
       } else {
+        constexpr int kParts = C::kFmt == WFATTN_CACHE_E4M3 ? 2 : 4;  // f16 pieces of one
+        uint32_t part[kParts];
+#pragma unroll
+        for (int e = 0; e < kParts; ++e)
+          part[e] = kv_at + buf * C::kBuf + piece(row0, kParts * col0 + e, C::kSlab);
 #pragma unroll
         for (int j = 0; j < 2 * C::kPieces; ++j) {
-          const uint32_t base =
-              at + j % C::kPieces * kApart * 128 + (j < C::kPieces ? 0 : C::kSlabs * C::kSlab);
+          const uint32_t half = j < C::kPieces ? 0 : C::kSlabs * C::kSlab;
           const uint32_t w[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
           if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
             uint32_t f[8];
@@ -450,67 +533,39 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
                 if ((f[e] & 0x7c000000u) == 0x7c000000u) f[e] &= 0xffffu, odd = true;
               }
             }
-            sts128(base + piece(row0, 2 * col0, C::kSlab), make_uint4(f[0], f[1], f[2], f[3]));
-            sts128(base + piece(row0, 2 * col0 + 1, C::kSlab), make_uint4(f[4], f[5], f[6], f[7]));
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              sts128(to_piece(part[e], j % C::kPieces) + half,
+                     make_uint4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]));
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              sts128(base + piece(row0, 4 * col0 + e, C::kSlab),
+              sts128(to_piece(part[e], j % C::kPieces) + half,
                      make_uint4(int4_f16x2<false>(w[e]), int4_f16x2<true>(w[e]),
                                 int4_f16x2<false>(w[e] >> 8), int4_f16x2<true>(w[e] >> 8)));
           }
         }
-        const int r = t % C::kKeys;
-        float *s = t < C::kKeys ? sh.k_scale[buf] : sh.v_scale[buf];
-        float *m = t < C::kKeys ? sh.k_mid[buf] : sh.v_mid[buf];
         if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
-          s[r] = __uint_as_float(held_scale);
+          sh.k_scale[buf][t] = __uint_as_float(held_k);
+          sh.v_scale[buf][t] = __uint_as_float(held_v);
         } else {
-          s[r] = ptx::bf16_lo(held_scale);
-          m[r] = fmaf(8.f, ptx::bf16_lo(held_scale), ptx::bf16_hi(held_scale));
+          const float ks = ptx::bf16_lo(held_k), vs = ptx::bf16_lo(held_v);
+          sh.k_scale[buf][t] = ks;
+          sh.v_scale[buf][t] = vs;
+          sh.k_mid[buf][t] = fmaf(8.f, ks, ptx::bf16_hi(held_k));
+          sh.v_mid[buf][t] = fmaf(8.f, vs, ptx::bf16_hi(held_v));
         }
       }
       return odd;
     };
-    const uint32_t leader = t == 0;
-    const uint32_t idesc_qk = idesc_wide(C::kBf16Rows, false);
-    const uint32_t idesc_pv = idesc_wide(C::kBf16Rows, true);
-    auto issue_pv = [&](int64_t i, bool first) -> bool {
-      const int buf = (int)(i & 1);
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar(sh.p_full[buf]), (uint32_t)(i >> 1) & 1,
-                                                  p.status)))
-        return false;
-      ptx::tc_fence_after();
-      // O has sums from before this segment's first unit only if V was odd there
-      first = first && sh.odd[buf] != (int)(i & 0x7fffffff);
-      const uint32_t v = kv_at + buf * C::kBuf + C::kSlabs * C::kSlab;
-#pragma unroll
-      for (int term = C::kBf16Rows ? 1 : 0; term >= 0; --term)
-#pragma unroll
-        for (int kk = 0; kk < C::kKeys / 16; ++kk)
-#pragma unroll
-          for (int s = 0; s < C::kSlabs; ++s)
-            mma_ts_warp(leader, tmem + C::kColO + 64 * s,
-                        tmem + C::kColS + 64 * buf + 32 * term + kk * 8,
-                        ptx::smem_desc_sw128(v + s * C::kSlab + kk * 2048, C::kSlab, 1024),
-                        idesc_pv, !first || kk > 0 || (C::kBf16Rows && term == 0));
-      commit_warp(leader, bar(sh.o_done));
-      return true;
-    };
-
-    bool ok = true, before_first = false;
-    uint32_t segment = 0;
     if constexpr (!C::kBf16Rows) fetch(0);
 #pragma unroll 1
     for (int64_t i = 0; i < units; ++i) {
       const int buf = (int)(i & 1);
-      const bool first = i == 0 || cur.u == 0;
       // the buffer is free after P V of the unit before last
-      if (i >= 2) ok = ptx::mbar_wait(bar(sh.o_done), (uint32_t)i & 1, p.status);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
+      if (i >= 2 &&
+          !ptx::mbar_wait(bar(sh.o_done[buf]), (uint32_t)((i - 2) >> 1) & 1, p.status))
         break;
-      }
       if constexpr (C::kBf16Rows) {
         fetch(buf);
         cp_async_wait<0>();
@@ -520,37 +575,7 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
       ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(bar(sh.kv_full[buf]));
       if (!C::kBf16Rows && i + 1 < units) fetch(0);
-      if (warp == 4) {
-        // A segment's queries come after the results of the one before, which
-        // wait for its last P V; within a segment Q K^T goes first.
-        if (first && i > 0) ok = issue_pv(i - 1, before_first);
-        ok = ok && ptx::mbar_wait(bar(sh.kv_full[buf]), (uint32_t)(i >> 1) & 1, p.status) &&
-             (!first || ptx::mbar_wait(bar(sh.q_full), segment & 1, p.status));
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) {
-          ptx::tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < C::D / 16; ++kk)
-            mma_ss_warp(
-                leader, tmem + C::kColS + 64 * buf,
-                ptx::smem_desc_sw128(q_at + kk / 4 * C::kQSlab + kk % 4 * 32, 16, 1024),
-                ptx::smem_desc_sw128(kv_at + buf * C::kBuf + kk / 4 * C::kSlab + kk % 4 * 32, 16,
-                                     1024),
-                idesc_qk, kk > 0);
-          commit_warp(leader, bar(sh.s_full[buf]));
-          if (!first) ok = issue_pv(i - 1, before_first);
-        }
-      }
-      segment += first;
-      before_first = first;
       cur.next(p);
-    }
-    if (warp == 4) {
-      if (ok) ok = issue_pv(units - 1, before_first);
-      if (!ok && leader) {  // every product issued has to end before the memory goes
-        ptx::tc_commit(bar(sh.drain));
-        ptx::mbar_wait_drain(bar(sh.drain), 0);
-      }
     }
     if constexpr (C::kBf16Rows) cp_async_wait<0>();
   } else {
@@ -624,14 +649,13 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
       while (true) {  // a unit
         const int buf = (int)(i & 1);
         const uint32_t parity = (uint32_t)(i >> 1) & 1;
-        wait(sh.kv_full[buf], parity);  // its scales
         wait(sh.s_full[buf], parity);
         ptx::tc_fence_after();
         const bool odd = sh.odd[buf] == (int)(i & 0x7fffffff);
         // a wait ends the same way for a warp, whose loads and stores are common
         if (!idle && __all_sync(0xffffffffu, !failed)) {
           auto wait_o = [&]() {
-            if (i > 0) wait(sh.o_done, (uint32_t)(i - 1) & 1);
+            if (i > 0) wait(sh.o_done[buf ^ 1], (uint32_t)((i - 1) >> 1) & 1);
             ptx::tc_fence_after();
             __syncwarp();
           };
@@ -654,7 +678,7 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
       }
 
       // ---- the segment's end
-      wait(sh.o_done, (uint32_t)i & 1);
+      wait(sh.o_done[i & 1], (uint32_t)(i >> 1) & 1);
       ptx::tc_fence_after();
       const bool whole = done && headed;
       const int64_t slot = (int64_t)blockIdx.x * 2 + (headed ? 1 : 0);

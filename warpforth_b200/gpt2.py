@@ -15,17 +15,25 @@ not support) the prompt goes through the prefill kernel and every later
 single-token step through the split-KV decode kernel (``wfattn_decode_f32``
 for the f32 model) over the cached keys and values.
 
+``generate_drafted`` generates greedily over a ``KVCache`` of its own, f32, e4m3 or 4-bit: each step
+drafts a small tree of tokens (what followed the last words where they stood before), attends from
+all of them at once (``tree_decode``) and keeps those that the model would have chosen
+(``cache_keep``).
+
     python -m warpforth_b200.gpt2 --max-tokens 128      # random-init GPT-2 small
+    python -m warpforth_b200.gpt2 --draft-nodes 12 --cache e4m3
 """
 
 from __future__ import annotations
 
 import argparse
+import contextlib
 import time
 from collections.abc import Callable
 
 import torch
 
+from .cache import KVCache, cache_keep, cache_read, cache_write, tree_decode, tree_words
 from .warpforth import DecodeWorkspace, attention, decode
 
 
@@ -105,6 +113,145 @@ def generate(model, prompt: torch.Tensor, max_new_tokens: int, use_cache: bool =
                           do_sample=False, use_cache=use_cache, pad_token_id=50256)
 
 
+class _CachedAttention:
+    """GPT-2's attention over one ``KVCache`` a layer, for ``generate_drafted``."""
+
+    def __init__(self, model, max_len: int, fmt: str) -> None:
+        cfg, device = model.config, next(model.parameters()).device
+        self.caches = [KVCache(1, cfg.n_head, max_len, cfg.n_embd // cfg.n_head, fmt=fmt,
+                               device=device) for _ in range(cfg.n_layer)]
+        self.lens = torch.zeros(1, dtype=torch.int32, device=device)  # rows in the caches
+        self.start = torch.zeros_like(self.lens)
+        self.length = 0  # the same on the host
+        self.words: torch.Tensor | None = None  # of the drafted tree; None in the prompt
+        self.workspace = DecodeWorkspace()
+
+    def __call__(self, module, query, key, value, attention_mask=None, scaling=None, dropout=0.0,
+                 **kwargs):
+        cache = self.caches[module.layer_idx]
+        cache_write(cache, key, value, self.lens)
+        if self.words is not None:
+            out = tree_decode(query, cache, self.lens, tree=self.words, scale=scaling,
+                              workspace=self.workspace)
+        else:
+            if self.length:  # a later part of the prompt: the rows before it come from the cache
+                key, value = cache_read(cache, self.start, self.length + query.shape[2],
+                                        dtype=query.dtype)
+            out = attention(query, key, value, causal=True, scale=scaling)
+        return out.transpose(1, 2), None
+
+    def keep(self, path: list[int]) -> None:
+        """The nodes of the path follow the rows that are there; the others are dropped."""
+        rows = torch.tensor([path], dtype=torch.int32, device=self.lens.device)
+        lens = self.lens
+        for cache in self.caches:
+            self.lens = cache_keep(cache, lens, rows)
+        self.length += len(path)
+
+
+def draft_tree(tokens: list[int], nodes: int, depth: int = 8) -> tuple[list[int], list[int]]:
+    """A tree of at most ``nodes`` drafted tokens: (tokens, parents), the last token as its root.
+
+    Its branches are what followed earlier places of the last three, two or one tokens, the longest
+    match and the latest place first; common beginnings share their nodes.
+    """
+    drafted, parents = [tokens[-1]], [-1]
+    children: dict[tuple[int, int], int] = {}
+    for n in (3, 2, 1):
+        last = tokens[-n:]
+        for at in range(len(tokens) - n - 1, -1, -1):
+            if len(drafted) >= nodes:
+                return drafted, parents
+            if len(last) < n or tokens[at:at + n] != last:
+                continue
+            node = 0
+            for token in tokens[at + n:at + n + depth]:
+                if (node, token) not in children:
+                    if len(drafted) >= nodes:
+                        break
+                    children[node, token] = len(drafted)
+                    drafted.append(token)
+                    parents.append(node)
+                node = children[node, token]
+    return drafted, parents
+
+
+def accepted_path(drafted: list[int], parents: list[int], chosen: list[int]) -> list[int]:
+    """The nodes from the root on whose tokens the model chose (``chosen[i]`` after node i)."""
+    path = [0]
+    while True:
+        following = [i for i, parent in enumerate(parents)
+                     if parent == path[-1] and drafted[i] == chosen[path[-1]]]
+        if not following:
+            return path
+        path.append(following[0])
+
+
+@contextlib.contextmanager
+def _eager_attention(function):
+    import transformers.models.gpt2.modeling_gpt2 as gpt2_module
+
+    original = gpt2_module.eager_attention_forward
+    gpt2_module.eager_attention_forward = function
+    try:
+        yield
+    finally:
+        gpt2_module.eager_attention_forward = original
+
+
+@torch.no_grad()
+def generate_drafted(model, prompt: torch.Tensor, max_new_tokens: int, *, nodes: int = 12,
+                     cache: str = "f32", prompt_chunk: int = 512) -> tuple[torch.Tensor, int]:
+    """Greedy generation with drafted trees of up to ``nodes`` tokens over a ``cache`` of that format.
+
+    prompt: [1, n].  A prompt longer than ``prompt_chunk`` is read in parts.  Over an f32 cache the
+    tokens are those of ``generate`` (but for ties); the other formats round what is attended to.
+    Returns the tokens [1, n + max_new_tokens] and how many times the model ran after the prompt.
+    """
+    if prompt.dim() != 2 or prompt.shape[0] != 1 or prompt.shape[1] < 1:
+        raise ValueError(f"prompt must be [1, n], got {tuple(prompt.shape)}")
+    if max_new_tokens < 1 or not 1 <= nodes <= 64 or prompt_chunk < 1:
+        raise ValueError("max_new_tokens and prompt_chunk must be >= 1, nodes in 1..64")
+    device = next(model.parameters()).device
+    ids = prompt.to(device)
+    tokens, end = prompt[0].tolist(), prompt.shape[1] + max_new_tokens
+    limit = model.config.n_positions
+    if end > limit:
+        raise ValueError(f"the model has {limit} positions, {end} are asked for")
+    state = _CachedAttention(model, end + nodes, cache)
+    runs = 0
+    with _eager_attention(state):
+        for at in range(0, ids.shape[1], prompt_chunk):
+            part = ids[:, at:at + prompt_chunk]
+            positions = torch.arange(at, at + part.shape[1], device=device)[None]
+            logits = model(part, position_ids=positions, use_cache=False).logits
+            state.lens = state.lens + part.shape[1]
+            state.length += part.shape[1]
+        tokens.append(int(logits[0, -1].argmax()))
+        while len(tokens) < end:
+            drafted, parents = draft_tree(tokens, nodes)
+            # a node past the model's last position is not drafted
+            depths = [0]
+            for parent in parents[1:]:
+                depths.append(depths[parent] + 1)
+            while state.length + max(depths) >= limit:
+                longest = max(depths)
+                keep = [i for i, depth in enumerate(depths) if depth < longest]
+                drafted, parents, depths = ([x[i] for i in keep] for x in (drafted, parents, depths))
+                renamed = {old: new for new, old in enumerate(keep)}
+                parents = [renamed.get(parent, -1) for parent in parents]
+            state.words = tree_words(parents).to(device)
+            positions = torch.tensor([[state.length + depth for depth in depths]], device=device)
+            logits = model(torch.tensor([drafted], device=device), position_ids=positions,
+                           use_cache=False).logits
+            runs += 1
+            chosen = logits[0].argmax(-1).tolist()
+            path = accepted_path(drafted, parents, chosen)
+            state.keep(path)
+            tokens += [drafted[i] for i in path[1:]] + [chosen[path[-1]]]
+    return torch.tensor([tokens[:end]], device=device), runs
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__,
                                  formatter_class=argparse.RawDescriptionHelpFormatter)
@@ -112,6 +259,10 @@ def main() -> None:
     ap.add_argument("--prompt-len", type=int, default=32)
     ap.add_argument("--seed", type=int, default=1)
     ap.add_argument("--use-cache", action="store_true")
+    ap.add_argument("--draft-nodes", type=int, default=0,
+                    help="generate with drafted trees of up to this many tokens (1 to 64)")
+    ap.add_argument("--cache", choices=("f32", "e4m3", "int4"), default="f32",
+                    help="format of the key/value cache under --draft-nodes")
     args = ap.parse_args()
     model = random_gpt2(args.seed)
     prompt = synthetic_prompt(args.prompt_len, args.seed)
@@ -119,13 +270,19 @@ def main() -> None:
     try:
         torch.cuda.synchronize()
         t0 = time.perf_counter()
-        out = generate(model, prompt, args.max_tokens, use_cache=args.use_cache)
+        if args.draft_nodes:
+            out, runs = generate_drafted(model, prompt, args.max_tokens, nodes=args.draft_nodes,
+                                         cache=args.cache)
+        else:
+            out = generate(model, prompt, args.max_tokens, use_cache=args.use_cache)
         torch.cuda.synchronize()
         dt = time.perf_counter() - t0
     finally:
         restore()
     print(out[0].tolist())
     print(f"{args.max_tokens / dt:.1f} tokens/s ({out.shape[1]} tokens total)")
+    if args.draft_nodes:
+        print(f"{runs} runs of the model after the prompt")
 
 
 if __name__ == "__main__":
