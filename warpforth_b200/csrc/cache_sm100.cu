@@ -271,12 +271,10 @@ __global__ void __launch_bounds__(kThreads) cache_rows_kernel(const RowsParams p
   uint8_t *x = p.x[which] + (b * xs.b + h * xs.h + i0 * xs.s + lane * 8) * kSize;
   const int64_t step = (int64_t)kGroups * xs.s * kSize;
   Raw<kF32> raw[kRows];
-  if constexpr (kWrite) {  // every row exists: no need to know which are live
 #pragma unroll
-    for (int j = 0; j < kRows; ++j) {
-      raw[j] = Raw<kF32>{};
-      if (i0 + j * kGroups < p.n) raw[j] = load_raw<kF32, kVec>(x + j * step);
-    }
+  for (int j = 0; j < kRows; ++j) raw[j] = Raw<kF32>{};
+  if constexpr (kWrite && !kLong) {  // the row exists, live or not: no need to wait
+    if (i0 < p.n) raw[0] = load_raw<kF32, kVec>(x);
   }
   const Span span = live_rows(p, b, i0 == 0 && lane == 0 && which == 0 && h == 0);
   const int64_t row0 = b * p.c.sb + h * p.c.sh + span.start + i0;
@@ -287,12 +285,16 @@ __global__ void __launch_bounds__(kThreads) cache_rows_kernel(const RowsParams p
   for (int j = 0; j < kRows; ++j) {
     const int i = (int)i0 + j * kGroups;
     live[j] = i >= span.from && i < span.to;
+    if constexpr (kWrite && kLong) {
+      if (live[j]) raw[j] = load_raw<kF32, kVec>(x + j * step);
+    }
   }
   if constexpr (kWrite) {
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
-      cache_store8<kFmt, kF32, kLanes>(codes + j * kGroups * kRowBytes, scales + j * kGroups * 4,
-                                       lane == 0, live[j], raw[j]);
+      if (__any_sync(0xffffffffu, live[j]))
+        cache_store8<kFmt, kF32, kLanes>(codes + j * kGroups * kRowBytes, scales + j * kGroups * 4,
+                                         lane == 0, live[j], raw[j]);
   } else {
     constexpr int kWords = kRowBytes / kLanes / 4;
     uint32_t w[kRows][kWords], scale[kRows];

@@ -92,15 +92,16 @@ struct Cfg {
   // keys of a unit: about 16 to 32 KB of K and V
   static constexpr int kKeys = kRowBytes == 32    ? 256
                                : kRowBytes == 64  ? (kNT * D > 128 ? 256 : 128)
-                               : kRowBytes == 128 ? 128
-                                                  : 64;
+                               : kRowBytes == 128 && D == 64 ? 128
+                                                             : 64;
   // 16-key tiles taken together: two independent chains of products hide their
-  // latency; rows of 256 bytes and more have it hidden by their own length
-  static constexpr int kKT = kRowBytes <= 128 ? 2 : 1;
+  // latency.  Rows of 128 values have two chains each, and smaller units leave
+  // more of the stages in flight (e4m3, one token, 342k keys of 8 heads: 128 us
+  // against 160 with two tiles and 128 keys).
+  static constexpr int kKT = kRowBytes <= 64 || (kRowBytes == 128 && D == 64) ? 2 : 1;
   static constexpr int kGroups = kKeys / (16 * kKT * kKW);  // of a warp in a unit
   static constexpr int kKBytes = kKeys * kRowBytes;
-  static constexpr int kOStride = D + 4;  // floats a row where warps are joined
-  static constexpr int kMerge = kWarps * 8 * kNT * kOStride * 4;  // in a used stage
+  static constexpr int kMerge = kWarps * 8 * kNT * D * 4;  // sums of O, in a used stage
   static constexpr int kData = 2 * kKBytes + (kScaled ? 8 * kKeys : 0);
   static constexpr int kStage = kData > kMerge ? kData : kMerge;
   static constexpr int kStats = kWarps * 8 * kNT * 2 * 4;
@@ -248,6 +249,15 @@ __device__ __forceinline__ int o_index(int mt, int g, int r) {
   return (C::D / 8) * g + 2 * mt + r;
 }
 
+// Place of value d of row r of the sums where warps meet: groups of four values
+// are permuted so that a fragment's lanes write to different banks (two to one
+// at most) and a row is still read four values at a time.
+template <class C>
+__device__ __forceinline__ int sum_index(int r, int d) {
+  const int x = C::kKind == kBf16 ? r & 6 : C::kKind == kTf32 ? (r & 2) << 1 : r >> 1 & 3;
+  return r * C::D + (d ^ (x << 2));
+}
+
 // One value of a V row in a stage, unscaled (used where a row is not finite).
 template <class C>
 __device__ __forceinline__ float v_value(uint32_t v, int row, int d) {
@@ -313,6 +323,12 @@ struct Cursor {
 // units' difference in load costs less than joining parts.
 constexpr int kShort = 4;
 
+// total * x / parts, x <= parts <= kCounters; 64-bit divisions are long.
+__device__ __forceinline__ int64_t part_of(int64_t total, int x, int parts) {
+  if (total < (int64_t(1) << 32) / kCounters) return (uint32_t)total * (uint32_t)x / (uint32_t)parts;
+  return total * x / parts;
+}
+
 template <int kKeys>
 __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, int64_t &end,
                                                int64_t &all) {
@@ -345,7 +361,8 @@ __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, 
   }
   // unit (or, with whole segments, segment) where the share begins and ends
   const int64_t total = whole ? B * HR : all;
-  const int64_t from = total * blockIdx.x / p.ctas, to = total * (blockIdx.x + 1) / p.ctas;
+  const int64_t from = part_of(total, blockIdx.x, p.ctas);
+  const int64_t to = part_of(total, blockIdx.x + 1, p.ctas);
   int64_t at = upto - mine;  // first unit of this thread's sequences
   for (int b = b0; b < b1; ++b) {
     if (per > 1) s = sequence<kKeys>(p, b, false);
@@ -353,7 +370,8 @@ __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, 
     const int64_t lo = whole ? b * HR : at, hi = whole ? lo + HR : at + n;
     if (from >= lo && from < hi) {
       const int64_t into = whole ? (from - lo) * s.units : from - lo;
-      const int hr = (int)(into / s.units);
+      const int hr = into < (int64_t(1) << 32) ? (int)((uint32_t)into / (uint32_t)s.units)
+                                               : (int)(into / s.units);
       offset = at + into;
       found.b = b;
       found.u = (int)(into - (int64_t)hr * s.units);
@@ -1260,6 +1278,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
         }
       }
     const int slot = headed ? 1 : 0;
+    const int rows = min(C::kRows, p.R - cur.tile * C::kRows);  // that there are
     float *part = p.part + (int64_t)(blockIdx.x * 2 + slot) * C::kRows * C::D;
     float *part_ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D +
                      (int64_t)(blockIdx.x * 2 + slot) * C::kRows * 2;
@@ -1268,38 +1287,44 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
     // maximum and sum.  (With all the keys in one warp this only turns the
     // fragments into rows.)
     __syncthreads();
-    float *mine = reinterpret_cast<float *>(smem + st) + warp * 8 * C::kNT * C::kOStride;
+    float *sums = reinterpret_cast<float *>(smem + st);
 #pragma unroll
     for (int nt = 0; nt < C::kNT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = 8 * nt + 2 * t + e;
+        const int r = warp * 8 * C::kNT + 8 * nt + 2 * t + e;
 #pragma unroll
-        for (int mt = 0; mt < C::kMt; ++mt)
+        for (int mt = 0; mt < C::kMt; ++mt) {
+          if constexpr (C::kKind == kBf16) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-            mine[r * C::kOStride + o_index<C>(mt, g, y)] = w.o[nt][mt][2 * y + e];
-        if (g == 0) {
-          stats[(warp * 8 * C::kNT + r) * 2] = w.m[nt][e];
-          stats[(warp * 8 * C::kNT + r) * 2 + 1] = w.l[nt][e];
+            for (int y = 0; y < 2; ++y)
+              sums[sum_index<C>(r, o_index<C>(mt, g, y))] = w.o[nt][mt][2 * y + e];
+          } else {  // values d and d + 1
+            *reinterpret_cast<float2 *>(sums + sum_index<C>(r, o_index<C>(mt, g, 0))) =
+                make_float2(w.o[nt][mt][e], w.o[nt][mt][2 + e]);
+          }
         }
+        if (g == 0) *reinterpret_cast<float2 *>(stats + r * 2) = make_float2(w.m[nt][e], w.l[nt][e]);
       }
     __syncthreads();
 #pragma unroll 1
-    for (int x = threadIdx.x; x < C::kRows * C::D / 4; x += kThreads) {
+    for (int x = threadIdx.x; x < rows * (C::D / 4); x += kThreads) {
       const int r = x / (C::D / 4), dd = x % (C::D / 4) * 4;
       const int at0 = r / (8 * C::kNT) * C::kKW * 8 * C::kNT + r % (8 * C::kNT);
+      float2 ml[C::kKW];
       float m = -FLT_MAX, l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int y = 0; y < C::kKW; ++y) m = fmaxf(m, stats[(at0 + y * 8 * C::kNT) * 2]);
+      for (int y = 0; y < C::kKW; ++y) {
+        ml[y] = *reinterpret_cast<const float2 *>(stats + (at0 + y * 8 * C::kNT) * 2);
+        m = fmaxf(m, ml[y].x);
+      }
 #pragma unroll
       for (int y = 0; y < C::kKW; ++y) {
-        const int at = at0 + y * 8 * C::kNT;
-        const float f = ptx::ex2_approx(stats[at * 2] - m);
-        const float4 z =
-            *reinterpret_cast<const float4 *>(smem + st + (at * C::kOStride + dd) * 4);
-        l = fmaf(stats[at * 2 + 1], f, l);
+        const float f = ptx::ex2_approx(ml[y].x - m);
+        const float4 z = *reinterpret_cast<const float4 *>(
+            sums + sum_index<C>(at0 + y * 8 * C::kNT, dd));
+        l = fmaf(ml[y].y, f, l);
         o.x = fmaf(z.x, f, o.x), o.y = fmaf(z.y, f, o.y);
         o.z = fmaf(z.z, f, o.z), o.w = fmaf(z.w, f, o.w);
       }
@@ -1316,10 +1341,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
         }
       } else {
         *reinterpret_cast<float4 *>(part + r * C::D + dd) = o;
-        if (dd == 0) {
-          part_ml[2 * r] = m;
-          part_ml[2 * r + 1] = l;
-        }
+        if (dd == 0) *reinterpret_cast<float2 *>(part_ml + 2 * r) = make_float2(m, l);
       }
     }
     if (!whole) {
