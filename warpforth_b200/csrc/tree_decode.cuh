@@ -33,7 +33,9 @@
 // segment (one sequence, head and tile) ends; a segment that lies in one CTA
 // is written out directly.  Of the others every CTA writes its part (maximum,
 // sum, unnormalised output) to the workspace, and the CTA whose part is the last
-// to arrive, by a counter, joins them in their order: the same bits every time.
+// to arrive, by a counter, joins them in their order: the same bits every time
+// (one launch less than a second kernel, which tree_decode_wide.cuh has for its
+// 128 rows).
 // Four warps split the keys of a unit or, with more rows, the rows.
 #pragma once
 
@@ -52,6 +54,12 @@ constexpr int kMaxSms = 148;  // CTAs are dealt for at most this many SMs
 // first launch on it, and left at zero by each (atomicInc wraps).
 constexpr int kCounters = WFATTN_TREE_DECODE_ZEROED / sizeof(unsigned int);  // one a CTA
 
+// The segment that begins in a CTA and goes on in others.
+struct Split {
+  int64_t all;  // units in all
+  int b, h, tile, last;  // the segment (b < 0: none), its last CTA
+};
+
 struct Params {
   CacheView c;
   int RT;        // row tiles a head
@@ -67,6 +75,7 @@ struct Params {
   int64_t tree_stride;
   float scale_log2;
   unsigned int *arrived;  // [kCounters]
+  Split *split;  // [ctas] (tree_decode_wide.cuh)
   float *part;   // [ctas][2][rows][D], then [ctas][2][rows][2] (maximum, sum)
   unsigned int *status;
 };
@@ -1024,71 +1033,89 @@ __device__ __forceinline__ void store_out4(const Params &p, uint8_t *row, int d,
   }
 }
 
-// A barrier of the CTA's first kThreads threads (in one kernel all of them).
-__device__ __forceinline__ void rows_barrier() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+// Adds parts first + begin, first + begin + step, .. up to `last` of values dd.. of
+// row r to (m, l, o), eight in flight.  Part c is slot 1 of CTA first, where the
+// segment begins, and slot 0 of the others; where there are fewer units than
+// CTAs, those without a unit have none.
+template <class C>
+__device__ __forceinline__ void add_parts(const Params &p, int r, int dd, int first, int last,
+                                          int begin, int step, int64_t all, float &m, float &l,
+                                          float4 &o) {
+  constexpr int kAtOnce = 8;
+  const float *ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D;
+  const bool sparse = all < p.ctas;
+#pragma unroll 1
+  for (int c0 = first + begin; c0 <= last; c0 += step * kAtOnce) {
+    float2 s[kAtOnce];
+    float4 z[kAtOnce];
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int c = c0 + j * step;
+      s[j] = make_float2(-FLT_MAX, 0.f);
+      z[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c <= last && !(sparse && part_of(all, c, p.ctas) == part_of(all, c + 1, p.ctas))) {
+        const int64_t at = (int64_t)(c * 2 + (c == first)) * C::kRows + r;
+        s[j] = __ldcg(reinterpret_cast<const float2 *>(ml + at * 2));
+        z[j] = __ldcg(reinterpret_cast<const float4 *>(p.part + at * C::D + dd));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) top = fmaxf(top, s[j].x);
+    const float f = ptx::ex2_approx(m - top);
+    m = top;
+    l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const float w = ptx::ex2_approx(s[j].x - m);
+      l = fmaf(s[j].y, w, l);
+      o.x = fmaf(z[j].x, w, o.x), o.y = fmaf(z[j].y, w, o.y);
+      o.z = fmaf(z[j].z, w, o.z), o.w = fmaf(z[j].w, w, o.w);
+    }
+  }
+}
+
+// Values dd.. of an output row from its sums.
+template <class C>
+__device__ __forceinline__ void store_sums(const Params &p, int64_t b, int64_t h, int r, int n,
+                                           int dd, float l, float4 o) {
+  bool live;
+  uint8_t *to = out_row(p, b, h, r, n, C::kF32 ? 4 : 2, live);
+  if (!to) return;
+  const bool some = live && l != 0.f;
+  const float inv = 1.f / l;
+  store_out4<C::kF32>(p, to, dd,
+                      some ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv)
+                           : make_float4(0.f, 0.f, 0.f, 0.f));
 }
 
 // Counts this CTA's part of a segment, which its threads have written, as
 // arrived, and joins the parts if it is the last: thread groups take a float4
-// column of a row each and every kth part, eight in flight, and meet in `room`
-// (4 KB of shared memory).  Not inlined: a CTA comes here twice at most, and the
-// loads in flight would cost the main loop its registers.
+// column of a row each and every kth part, and meet in `room` (4 KB of shared
+// memory).  Not inlined: a CTA comes here twice at most, and the loads in flight
+// would cost the main loop its registers.
 template <class C>
 __device__ __noinline__ void join(const Params &p, int b, int h, int tile, int n, int first,
                                   int last, int parts, int64_t all, uint8_t *room) {
   __shared__ int is_last;
-  rows_barrier();
+  __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
     is_last = atomicInc(p.arrived + first, parts - 1) == (unsigned)(parts - 1);
     __threadfence();
   }
-  rows_barrier();
+  __syncthreads();
   if (!is_last) return;
-  constexpr int kCols = C::D / 4, kAtOnce = 8;
-  const int rows = min(C::kRows, p.R - tile * C::kRows);
-  const float *ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D;
-  const int items = rows * kCols;
-  const int groups = items >= kThreads ? 1 : kThreads / items;  // 1, 2, 4, 8 or fewer
+  constexpr int kCols = C::D / 4;
+  const int items = min(C::kRows, p.R - tile * C::kRows) * kCols;
+  const int groups = items >= kThreads ? 1 : kThreads / items;
   const int group = items >= kThreads ? 0 : threadIdx.x / items;
-  const bool sparse = all < p.ctas;  // some CTAs have no unit
 #pragma unroll 1
   for (int x = items >= kThreads ? threadIdx.x : threadIdx.x % items; x < items; x += kThreads) {
     const int r = x / kCols, dd = x % kCols * 4;
     float m = -FLT_MAX, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (group < groups) {
-#pragma unroll 1
-      for (int c0 = first + group; c0 <= last; c0 += groups * kAtOnce) {
-        float2 s[kAtOnce];
-        float4 z[kAtOnce];
-        float top = m;
-#pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) {
-          const int c = c0 + j * groups;
-          s[j] = make_float2(-FLT_MAX, 0.f);
-          z[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (c <= last && !(sparse && all * c / p.ctas == all * (c + 1) / p.ctas)) {
-            const int64_t at = (int64_t)(c * 2 + (c == first)) * C::kRows + r;
-            s[j] = __ldcg(reinterpret_cast<const float2 *>(ml + at * 2));
-            z[j] = __ldcg(reinterpret_cast<const float4 *>(p.part + at * C::D + dd));
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) top = fmaxf(top, s[j].x);
-        const float f = ptx::ex2_approx(m - top);
-        m = top;
-        l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-#pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) {
-          const float w = ptx::ex2_approx(s[j].x - m);
-          l = fmaf(s[j].y, w, l);
-          o.x = fmaf(z[j].x, w, o.x), o.y = fmaf(z[j].y, w, o.y);
-          o.z = fmaf(z[j].z, w, o.z), o.w = fmaf(z[j].w, w, o.w);
-        }
-      }
-    }
+    if (group < groups) add_parts<C>(p, r, dd, first, last, group, groups, all, m, l, o);
     if (groups > 1) {  // one pass: items < kThreads
       float4 *sums = reinterpret_cast<float4 *>(room);
       float2 *mls = reinterpret_cast<float2 *>(room + kThreads * sizeof(float4));
@@ -1096,7 +1123,7 @@ __device__ __noinline__ void join(const Params &p, int b, int h, int tile, int n
         sums[threadIdx.x] = o;
         mls[threadIdx.x] = make_float2(m, l);
       }
-      rows_barrier();
+      __syncthreads();
       if (group > 0) return;
       for (int y = 1; y < groups; ++y) m = fmaxf(m, mls[y * items + x].x);
       const float f = ptx::ex2_approx(mls[x].x - m);
@@ -1111,13 +1138,7 @@ __device__ __noinline__ void join(const Params &p, int b, int h, int tile, int n
       }
     }
     if (group > 0) return;
-    bool live;
-    uint8_t *to = out_row(p, b, h, tile * C::kRows + r, n, C::kF32 ? 4 : 2, live);
-    const bool some = live && l != 0.f;
-    const float inv = 1.f / l;
-    store_out4<C::kF32>(p, to, dd,
-                        some ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv)
-                             : make_float4(0.f, 0.f, 0.f, 0.f));
+    store_sums<C>(p, b, h, tile * C::kRows + r, n, dd, l, o);
   }
 }
 
@@ -1282,7 +1303,6 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
     float *part = p.part + (int64_t)(blockIdx.x * 2 + slot) * C::kRows * C::D;
     float *part_ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D +
                      (int64_t)(blockIdx.x * 2 + slot) * C::kRows * 2;
-    constexpr int kSize = C::kF32 ? 4 : 2;
     // The warps' sums meet in the stage just read: rows of O, and beside them
     // maximum and sum.  (With all the keys in one warp this only turns the
     // fragments into rows.)
@@ -1329,16 +1349,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
         o.z = fmaf(z.z, f, o.z), o.w = fmaf(z.w, f, o.w);
       }
       if (whole) {
-        bool live;
-        uint8_t *to =
-            out_row(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, kSize, live);
-        if (to) {
-          const bool some = live && l != 0.f;
-          const float inv = 1.f / l;
-          store_out4<C::kF32>(p, to, dd,
-                              some ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv)
-                                   : make_float4(0.f, 0.f, 0.f, 0.f));
-        }
+        store_sums<C>(p, cur.b, cur.h, cur.tile * C::kRows + r, cur.s.n, dd, l, o);
       } else {
         *reinterpret_cast<float4 *>(part + r * C::D + dd) = o;
         if (dd == 0) *reinterpret_cast<float2 *>(part_ml + 2 * r) = make_float2(m, l);
@@ -1370,7 +1381,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
 template <class C>
 size_t workspace_bytes() {
   static_assert(C::kCtas * kMaxSms <= kCounters, "a counter a CTA");
-  return kCounters * sizeof(unsigned int) +
+  return kCounters * sizeof(unsigned int) + kMaxSms * C::kCtas * sizeof(Split) +
          (size_t)kMaxSms * C::kCtas * 2 * C::kRows * (C::D + 2) * sizeof(float);
 }
 
@@ -1388,7 +1399,8 @@ void prepare(Params &p, void *workspace, const DeviceInfo &dev) {
   const int64_t most = (dev.sm_count < kMaxSms ? dev.sm_count : kMaxSms) * C::kCtas;
   p.ctas = (int)imin64(most, units > most ? most : units * imin64(segs, most));
   p.arrived = static_cast<unsigned int *>(workspace);
-  p.part = reinterpret_cast<float *>(p.arrived + kCounters);
+  p.split = reinterpret_cast<Split *>(p.arrived + kCounters);
+  p.part = reinterpret_cast<float *>(p.split + kMaxSms * C::kCtas);
 }
 
 template <class C>
