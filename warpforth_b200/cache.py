@@ -25,7 +25,7 @@ import struct
 import torch
 
 from . import _lib
-from .warpforth import _DTYPES, DecodeWorkspace, _ptr, _require_cuda, _stream_handle
+from .warpforth import _DTYPES, DecodeWorkspace, _ptr, _raw_stream, _require_cuda
 
 _FORMATS = {"f32": (_lib.CACHE_F32, torch.float32), "bf16": (_lib.CACHE_BF16, torch.bfloat16),
             "e4m3": (_lib.CACHE_E4M3, torch.float8_e4m3fn), "int4": (_lib.CACHE_INT4, torch.uint8)}
@@ -123,8 +123,12 @@ class KVCache:
         self._c = _lib.Cache(_FORMATS[fmt][0], self.head_dim, batch, heads, max_len, sb, sh,
                              _ptr(k), _ptr(v), _ptr(k_scale) if scaled else None,
                              _ptr(v_scale) if scaled else None)
+        # what every call needs, looked up once
+        self._lib = _lib.load()
         self._at = ctypes.addressof(self._c)
-        self._batch_shape = torch.Size((batch,))
+        self._index = k.get_device()
+        self._batch_shape = (batch,)
+        self._new = {t: torch.empty(0, dtype=t, device=k.device).new_empty for t in _DTYPES}
         self._tree_bytes: dict[tuple, int] = {}  # workspace sizes by call shape
 
 
@@ -134,11 +138,12 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 
 def _run(cache: KVCache, fn, *args) -> None:
     """fn(cache, *args, stream) with the cache's device current."""
-    if cache.device.index == _current_device():
-        status = fn(cache._at, *args, _stream_handle(cache.device))
+    index = cache._index
+    if index == _current_device():
+        status = fn(cache._at, *args, _raw_stream(index))
     else:
-        with torch.cuda.device(cache.device):
-            status = fn(cache._at, *args, _stream_handle(cache.device))
+        with torch.cuda.device(index):
+            status = fn(cache._at, *args, _raw_stream(index))
     if status:
         _lib.check(status)
 
@@ -146,8 +151,8 @@ def _run(cache: KVCache, fn, *args) -> None:
 def _ints(name: str, t: torch.Tensor, shape, cache: KVCache,
           dtype: torch.dtype = torch.int32) -> int:
     """The address of integers with a unit last stride on the cache's device."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != cache.device or \
-            t.shape != shape:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or \
+            t.get_device() != cache._index or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)} on {cache.device}")
     if t.stride(-1) != 1 and shape[-1] > 1:
         raise ValueError(f"{name} must have a unit last stride")
@@ -156,9 +161,9 @@ def _ints(name: str, t: torch.Tensor, shape, cache: KVCache,
 
 def _rows(name: str, t: torch.Tensor, shape, dtype, cache: KVCache) -> bytes:
     """The strides of f32 or bf16 rows of this shape on the cache's device."""
-    if not isinstance(t, torch.Tensor) or t.shape != shape or t.device != cache.device:
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.get_device() != cache._index:
         raise ValueError(f"{name} must be of shape {tuple(shape)} on {cache.device}")
-    if t.dtype != dtype or dtype not in _DTYPES:
+    if t.dtype is not dtype or dtype not in _DTYPES:
         raise ValueError(f"{name} must be float32 or bfloat16, as its companions (got {t.dtype})")
     a, b, c, d = t.stride()
     if d != 1:
@@ -179,7 +184,7 @@ def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, starts: torch.
     dtype, n = k.dtype, k.shape[2]
     shape = (cache.batch, cache.heads, n, cache.head_dim)
     ks, vs = _rows("k", k, shape, dtype, cache), _rows("v", v, shape, dtype, cache)
-    _run(cache, _lib.load().wfattn_cache_write, _DTYPES[dtype], n, k.data_ptr(), ks, v.data_ptr(),
+    _run(cache, cache._lib.wfattn_cache_write, _DTYPES[dtype], n, k.data_ptr(), ks, v.data_ptr(),
          vs, _ints("starts", starts, cache._batch_shape, cache),
          None if counts is None else _ints("counts", counts, cache._batch_shape, cache))
 
@@ -199,14 +204,14 @@ def cache_read(cache: KVCache, starts: torch.Tensor, rows: int, *,
         dtype = dtype or (torch.float32 if cache.fmt == "f32" else torch.bfloat16)
         if dtype not in _DTYPES:
             raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
-        k = torch.empty(shape, dtype=dtype, device=cache.device)
+        k = cache._new[dtype](shape)
         v = torch.empty_like(k)
         ks = vs = None  # contiguous
     else:
         k, v = out
         dtype = dtype or k.dtype
         ks, vs = (_rows(name, t, shape, dtype, cache) for name, t in (("out[0]", k), ("out[1]", v)))
-    _run(cache, _lib.load().wfattn_cache_read, _DTYPES[dtype], shape[2], k.data_ptr(), ks,
+    _run(cache, cache._lib.wfattn_cache_read, _DTYPES[dtype], shape[2], k.data_ptr(), ks,
          v.data_ptr(), vs, _ints("starts", starts, cache._batch_shape, cache),
          None if counts is None else _ints("counts", counts, cache._batch_shape, cache),
          out is None)
@@ -230,7 +235,7 @@ def cache_keep(cache: KVCache, lens: torch.Tensor, path: torch.Tensor, *,
     steps = _ints("path", path, (cache.batch, depth), cache)
     if out is None:
         out = torch.empty_like(lens)
-    _run(cache, _lib.load().wfattn_cache_keep, at, depth, steps, path.stride(0),
+    _run(cache, cache._lib.wfattn_cache_keep, at, depth, steps, path.stride(0),
          None if counts is None else _ints("counts", counts, cache._batch_shape, cache),
          _ints("out", out, cache._batch_shape, cache))
     return out
@@ -259,7 +264,7 @@ def tree_decode(q: torch.Tensor, cache: KVCache, kv_lens: torch.Tensor, *,
     _, hq, n, _ = shape
     qs = _rows("q", q, (cache.batch, hq, n, cache.head_dim), dtype, cache)
     if out is None:
-        out, os = q.new_empty(shape), None  # contiguous
+        out, os = cache._new[dtype](shape), None  # contiguous
     else:
         os = _rows("out", out, shape, dtype, cache)
     at = _ints("kv_lens", kv_lens, cache._batch_shape, cache)
@@ -269,7 +274,7 @@ def tree_decode(q: torch.Tensor, cache: KVCache, kv_lens: torch.Tensor, *,
         words = _ints("tree", tree, (n,) if one else (cache.batch, n), cache, torch.int64)
         words_stride = 0 if one else tree.stride(0)
     count = None if nodes is None else _ints("nodes", nodes, cache._batch_shape, cache)
-    lib = _lib.load()
+    lib = cache._lib
     nbytes = cache._tree_bytes.get((dtype, hq, n))
     if nbytes is None:
         nbytes = lib.wfattn_tree_decode_workspace_size(cache._at, _DTYPES[dtype], hq, n)
