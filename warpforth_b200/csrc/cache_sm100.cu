@@ -201,21 +201,29 @@ __device__ __forceinline__ void cache_store8(uint8_t *codes, uint8_t *scale, boo
     // the largest bf16; a NaN or an infinity among the values, or a span past f32
     const bool bad = !(s <= 3.38953139e38f);
     // u = rint(fl(a / s)), a = fl(x - m) >= 0.  a <= 15 s (1 + 2^-23), so u is in
-    // 0..15 without a clamp.  t = a (1 / s) + 1.5 2^23 holds rint(a (1 / s)) in
-    // its low bits; a (1 / s) is within 1e-5 of a / s, so only values that near
-    // a half need the division itself.
+    // 0..15 without a clamp.  y + 1.5 2^23 holds rint(y) in its low bits, and
+    // a / s and its rounding lie between a (1 / s) (1 -+ 2^-21): where both ends
+    // round alike that is u, and only else the division itself is needed.
     constexpr float kMagic = 12582912.f;
     const float inv = __frcp_rn(s);
-    float a[8], t[8], far = 0.f;
+    const float below = inv * (1.f - 0x1p-21f), above = inv * (1.f + 0x1p-21f);
+    const uint64_t m2 = ptx::f2_pack(-m, -m), magic2 = ptx::f2_pack(kMagic, kMagic);
+    const uint64_t below2 = ptx::f2_pack(below, below), above2 = ptx::f2_pack(above, above);
+    float t[8];
+    uint32_t apart = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      a[i] = __fsub_rn(f[i], m);
-      t[i] = fmaf(a[i], inv, kMagic);
-      far = fmaxf(far, fabsf(fmaf(a[i], inv, kMagic - t[i])));
+    for (int i = 0; i < 8; i += 2) {
+      const uint64_t a = ptx::f2_add(ptx::f2_pack(f[i], f[i + 1]), m2);
+      float y0, y1;
+      ptx::f2_unpack(ptx::f2_fma(a, below2, magic2), t[i], t[i + 1]);
+      ptx::f2_unpack(ptx::f2_fma(a, above2, magic2), y0, y1);
+      apart |= (__float_as_uint(t[i]) ^ __float_as_uint(y0)) |
+               (__float_as_uint(t[i + 1]) ^ __float_as_uint(y1));
     }
-    if (!(far < 0.49999f) || !(inv < 1e38f)) {  // or 1 / s overflows
+    if (apart || !(inv < 1e38f)) {  // or 1 / s overflows
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = kMagic + (s > 0.f ? rintf(__fdiv_rn(a[i], s)) : 0.f);
+      for (int i = 0; i < 8; ++i)
+        t[i] = kMagic + (s > 0.f ? rintf(__fdiv_rn(__fsub_rn(f[i], m), s)) : 0.f);
     }
     uint32_t w = 0;
 #pragma unroll

@@ -135,17 +135,10 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
                                       uint32_t row_tmem, uint32_t sp, int key0, bool odd,
                                       uint64_t word, float qf, float qsum, const float *k_scale,
                                       const float *k_mid, const float *v_scale, const float *v_mid,
-                                      bool first, float &m, float &l, float &om, float &vinv,
+                                      float vtop, bool first, float &m, float &l, float &om, float &vinv,
                                       Wait wait_o) {
   uint32_t s[64];
   ptx::tmem_ld_32x32b_x64(sp, s);
-  const int lane = threadIdx.x & 31;
-  float vtop = 0.f;
-  if constexpr (C::kScaled) {
-    vtop = fmaxf(v_scale[lane], v_scale[lane + 32]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, x));
-  }
   ptx::tmem_wait_ld();
   // ---- scores before qf, which is positive
   const uint64_t qsum2 = ptx::f2_pack(qsum, qsum);
@@ -319,6 +312,7 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
     alignas(16) float k_mid[2][C::kKeys];
     alignas(16) float v_scale[2][C::kKeys];
     alignas(16) float v_mid[2][C::kKeys];
+    float v_top[2][2];  // the largest scale of V's rows 0-31 and 32-63
   } sh;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   if (ptx::timeout_flagged(p.status)) return;  // until the host clears it
@@ -555,6 +549,10 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
           sh.k_mid[buf][t] = fmaf(8.f, ks, ptx::bf16_hi(held_k));
           sh.v_mid[buf][t] = fmaf(8.f, vs, ptx::bf16_hi(held_v));
         }
+        // scales are not negative: their bits order like them; NaN does not count
+        uint32_t top = C::kFmt == WFATTN_CACHE_E4M3 ? held_v : held_v << 16;
+        top = __reduce_max_sync(0xffffffffu, top > 0x7f800000u ? 0u : top);
+        if (t % 32 == 0) sh.v_top[buf][t / 32] = __uint_as_float(top);
       }
       return odd;
     };
@@ -654,6 +652,7 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
         const bool odd = sh.odd[buf] == (int)(i & 0x7fffffff);
         // a wait ends the same way for a warp, whose loads and stores are common
         if (!idle && __all_sync(0xffffffffu, !failed)) {
+          const float vtop = C::kScaled ? fmaxf(sh.v_top[buf][0], sh.v_top[buf][1]) : 0.f;
           auto wait_o = [&]() {
             if (i > 0) wait(sh.o_done[buf ^ 1], (uint32_t)((i - 1) >> 1) & 1);
             ptx::tc_fence_after();
@@ -662,11 +661,11 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
           if ((cur.u + 1) * C::kKeys > cur.s.len)
             weigh<C, true>(p, cur, row_tmem, row_tmem + C::kColS + 64 * buf, cur.u * C::kKeys, odd,
                            word, qf, qsum, sh.k_scale[buf], sh.k_mid[buf], sh.v_scale[buf],
-                           sh.v_mid[buf], first, m, l, om, vinv, wait_o);
+                           sh.v_mid[buf], vtop, first, m, l, om, vinv, wait_o);
           else
             weigh<C, false>(p, cur, row_tmem, row_tmem + C::kColS + 64 * buf, cur.u * C::kKeys,
                             odd, word, qf, qsum, sh.k_scale[buf], sh.k_mid[buf], sh.v_scale[buf],
-                            sh.v_mid[buf], first, m, l, om, vinv, wait_o);
+                            sh.v_mid[buf], vtop, first, m, l, om, vinv, wait_o);
         }
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(sh.p_full[buf]));
