@@ -70,11 +70,22 @@ __device__ __forceinline__ void cache_values8(const uint32_t *w, uint32_t scale,
     }
   } else {
     const float s = ptx::bf16_lo(scale), m = ptx::bf16_hi(scale);
-    // 2^23 + u has the code in its low bits; s u is exact in f32 (8 and 4
-    // bits), so one rounding is left
+    // A code left where it is in its half of the word, under 2^23, is 16^i u;
+    // s 16^-i is exact (for s >= 2^-130), as is s u (8 and 4 bits): one rounding
+    // is left.
+    const float s1 = s * 0x1p-4f, s2 = s * 0x1p-8f, s3 = s * 0x1p-12f;
+    const uint64_t s01 = ptx::f2_pack(s, s1), s23 = ptx::f2_pack(s2, s3);
+    const uint64_t m2 = ptx::f2_pack(m, m), less = ptx::f2_pack(-8388608.f, -8388608.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      f[i] = fmaf(s, __uint_as_float((w[0] >> (4 * i) & 15u) | 0x4b000000u) - 8388608.f, m);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t h = i ? w[0] >> 16 : w[0];
+      const uint64_t a = ptx::f2_pack(__uint_as_float((h & 0xfu) | 0x4b000000u),
+                                      __uint_as_float((h & 0xf0u) | 0x4b000000u));
+      const uint64_t b = ptx::f2_pack(__uint_as_float((h & 0xf00u) | 0x4b000000u),
+                                      __uint_as_float((h & 0xf000u) | 0x4b000000u));
+      ptx::f2_unpack(ptx::f2_fma(s01, ptx::f2_add(a, less), m2), f[4 * i], f[4 * i + 1]);
+      ptx::f2_unpack(ptx::f2_fma(s23, ptx::f2_add(b, less), m2), f[4 * i + 2], f[4 * i + 3]);
+    }
   }
 }
 

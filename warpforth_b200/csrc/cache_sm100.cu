@@ -201,29 +201,40 @@ __device__ __forceinline__ void cache_store8(uint8_t *codes, uint8_t *scale, boo
     // the largest bf16; a NaN or an infinity among the values, or a span past f32
     const bool bad = !(s <= 3.38953139e38f);
     // u = rint(fl(a / s)), a = fl(x - m) >= 0.  a <= 15 s (1 + 2^-23), so u is in
-    // 0..15 without a clamp.  y + 1.5 2^23 holds rint(y) in its low bits, and
-    // a / s and its rounding lie between a (1 / s) (1 -+ 2^-21): where both ends
-    // round alike that is u, and only else the division itself is needed.
+    // 0..15 without a clamp.  t = a (1 / s) + 1.5 2^23 holds a whole number r next
+    // to a / s in its low bits, and e = a - r s is exact (r s has 12 bits) where
+    // it matters: r is u while |e| stays below s / 2 by more than a quotient's
+    // rounding; |e| = s / 2 is a tie, which a and s of few bits meet often, and
+    // its quotient is exact; only else the division itself is needed.
     constexpr float kMagic = 12582912.f;
-    const float inv = __frcp_rn(s);
-    const float below = inv * (1.f - 0x1p-21f), above = inv * (1.f + 0x1p-21f);
+    const float inv = __frcp_rn(s), half = 0.5f * s, sure = half * (1.f - 0x1p-18f);
     const uint64_t m2 = ptx::f2_pack(-m, -m), magic2 = ptx::f2_pack(kMagic, kMagic);
-    const uint64_t below2 = ptx::f2_pack(below, below), above2 = ptx::f2_pack(above, above);
-    float t[8];
-    uint32_t apart = 0;
+    const uint64_t inv2 = ptx::f2_pack(inv, inv), less2 = ptx::f2_pack(-kMagic, -kMagic);
+    const uint64_t s2 = ptx::f2_pack(-s, -s);
+    float t[8], e[8], far = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       const uint64_t a = ptx::f2_add(ptx::f2_pack(f[i], f[i + 1]), m2);
-      float y0, y1;
-      ptx::f2_unpack(ptx::f2_fma(a, below2, magic2), t[i], t[i + 1]);
-      ptx::f2_unpack(ptx::f2_fma(a, above2, magic2), y0, y1);
-      apart |= (__float_as_uint(t[i]) ^ __float_as_uint(y0)) |
-               (__float_as_uint(t[i + 1]) ^ __float_as_uint(y1));
+      const uint64_t y = ptx::f2_fma(a, inv2, magic2);
+      ptx::f2_unpack(y, t[i], t[i + 1]);
+      ptx::f2_unpack(ptx::f2_fma(ptx::f2_add(y, less2), s2, a), e[i], e[i + 1]);
+      far = ptx::fmax3(far, fabsf(e[i]), fabsf(e[i + 1]));
     }
-    if (apart || !(inv < 1e38f)) {  // or 1 / s overflows
+    if (!(far < sure) || !(inv < 1e38f)) {  // or 1 / s overflows, or s is 0
+      bool divide = !(inv < 1e38f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        t[i] = kMagic + (s > 0.f ? rintf(__fdiv_rn(__fsub_rn(f[i], m), s)) : 0.f);
+      for (int i = 0; i < 8; ++i) {
+        const float d = fabsf(e[i]);
+        if (d == half)  // to the even neighbour
+          t[i] += __float_as_uint(t[i]) & 1 ? copysignf(1.f, e[i]) : 0.f;
+        else
+          divide = divide || !(d < sure);
+      }
+      if (divide) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          t[i] = kMagic + (s > 0.f ? rintf(__fdiv_rn(__fsub_rn(f[i], m), s)) : 0.f);
+      }
     }
     uint32_t w = 0;
 #pragma unroll

@@ -32,10 +32,11 @@
 // its units through a ring of cp.async stages without regard to where a
 // segment (one sequence, head and tile) ends; a segment that lies in one CTA
 // is written out directly.  Of the others every CTA writes its part (maximum,
-// sum, unnormalised output) to the workspace, and the CTA whose part is the last
-// to arrive, by a counter, joins them in their order: the same bits every time
-// (one launch less than a second kernel, which tree_decode_wide.cuh has for its
-// 128 rows).
+// sum, unnormalised output) to the workspace, and they are joined in their order:
+// the same bits every time.  With one or two rows the CTA whose part is the last
+// to arrive, by a counter, does that, without another launch; more rows would
+// keep that CTA busy (8 rows of 128 values in 27 parts 15 us, 60 rows in 7 parts
+// 40 us), so there a second kernel does.
 // Four warps split the keys of a unit or, with more rows, the rows.
 #pragma once
 
@@ -66,6 +67,7 @@ struct Params {
   int R, G, T;   // query rows a head = G heads x T nodes
   uint32_t over_T;  // ceil(2^32 / T)
   bool q_vec, o_vec;  // rows of q (o) are aligned for vector loads (stores)
+  bool apart;         // parts are joined by a second kernel
   int ctas;      // of the grid
   const uint8_t *q;
   uint8_t *o;
@@ -101,13 +103,13 @@ struct Cfg {
   // keys of a unit: about 16 to 32 KB of K and V
   static constexpr int kKeys = kRowBytes == 32    ? 256
                                : kRowBytes == 64  ? (kNT * D > 128 ? 256 : 128)
-                               : kRowBytes == 128 && D == 64 ? 128
-                                                             : 64;
+                               : kRowBytes == 128 && (D == 64 || kNT == 2) ? 128
+                                                                           : 64;
   // 16-key tiles taken together: two independent chains of products hide their
   // latency.  Rows of 128 values have two chains each, and smaller units leave
   // more of the stages in flight (e4m3, one token, 342k keys of 8 heads: 128 us
   // against 160 with two tiles and 128 keys).
-  static constexpr int kKT = kRowBytes <= 64 || (kRowBytes == 128 && D == 64) ? 2 : 1;
+  static constexpr int kKT = kRowBytes <= 64 || (kRowBytes == 128 && (D == 64 || kNT == 2)) ? 2 : 1;
   static constexpr int kGroups = kKeys / (16 * kKT * kKW);  // of a warp in a unit
   static constexpr int kKBytes = kKeys * kRowBytes;
   static constexpr int kMerge = kWarps * 8 * kNT * D * 4;  // sums of O, in a used stage
@@ -331,6 +333,21 @@ struct Cursor {
 // no segment has more than kShort units the shares are whole segments: a few
 // units' difference in load costs less than joining parts.
 constexpr int kShort = 4;
+
+// What the joining kernel needs to know of the segment at c, which begins with
+// unit s0 and goes on to the CTA of its last unit: unit s lies in the last CTA x
+// with total x / ctas <= s.
+template <int kKeys>
+__device__ __forceinline__ Split split_of(const Params &p, const Cursor<kKeys> &c, int64_t s0,
+                                          int64_t all) {
+  Split s;
+  s.all = all;
+  s.b = c.b;
+  s.h = c.h;
+  s.tile = c.tile;
+  s.last = (int)(((s0 + c.s.units) * p.ctas - 1) / all);
+  return s;
+}
 
 // total * x / parts, x <= parts <= kCounters; 64-bit divisions are long.
 __device__ __forceinline__ int64_t part_of(int64_t total, int x, int parts) {
@@ -1154,6 +1171,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
   int64_t begin, end, all;
   Cursor<C::kKeys> cur = share<C::kKeys>(p, begin, end, all), ahead = cur;
   const int64_t units = end - begin;
+  if (p.apart && threadIdx.x == 0) p.split[blockIdx.x].b = -1;
   if (units <= 0) return;
 
   // Who loads what of a unit: where every warp reads keys of its own, each warp
@@ -1355,13 +1373,14 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
         if (dd == 0) *reinterpret_cast<float2 *>(part_ml + 2 * r) = make_float2(m, l);
       }
     }
-    if (!whole) {
-      // Units s.. of the segment lie in CTAs x with all x / ctas <= s: the
-      // one of s is ((s + 1) ctas - 1) / all.  CTAs without units are passed
-      // over; there are none, or no CTA has two.
+    if (p.apart) {
+      if (!done && headed && threadIdx.x == 0)
+        p.split[blockIdx.x] = split_of(p, cur, begin + i - cur.u, all);
+    } else if (!whole) {
+      // CTAs without units are passed over; there are none, or no CTA has two
       const int64_t s0 = begin + i - cur.u;
       const int first_cta = headed ? (int)blockIdx.x : (int)(((s0 + 1) * p.ctas - 1) / all);
-      const int last_cta = (int)(((s0 + cur.s.units) * p.ctas - 1) / all);
+      const int last_cta = split_of(p, cur, s0, all).last;
       const int parts = min(last_cta - first_cta + 1, cur.s.units);
       join<C>(p, cur.b, cur.h, cur.tile, cur.s.n, first_cta, last_cta, parts, all, smem + st);
     }
@@ -1385,6 +1404,39 @@ size_t workspace_bytes() {
          (size_t)kMaxSms * C::kCtas * 2 * C::kRows * (C::D + 2) * sizeof(float);
 }
 
+// Joins the parts of the segments that more than one CTA worked on: block (x, y)
+// rows y kJoinRows.. of the one that begins in CTA x.
+constexpr int kJoinRows = 16;
+
+template <class C>
+__global__ void __launch_bounds__(kThreads) tree_join_kernel(const __grid_constant__ Params p) {
+  // after a wait ran out the records may be another call's
+  if (C::kWide && ptx::timeout_flagged(p.status)) return;
+  const Split s = p.split[blockIdx.x];
+  if (s.b < 0) return;
+  const Seq seq = sequence<C::kKeys>(p, s.b, false);
+  constexpr int kCols = C::D / 4;
+#pragma unroll 1
+  for (int x = threadIdx.x; x < kJoinRows * kCols; x += kThreads) {
+    const int r = blockIdx.y * kJoinRows + x / kCols, dd = x % kCols * 4;
+    if (s.tile * C::kRows + r >= p.R) return;
+    float m = -FLT_MAX, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    add_parts<C>(p, r, dd, blockIdx.x, s.last, 0, 1, s.all, m, l, o);
+    store_sums<C>(p, s.b, s.h, s.tile * C::kRows + r, seq.n, dd, l, o);
+  }
+}
+
+template <class C>
+cudaError_t launch_join(const Params &p, cudaStream_t stream) {
+  const cudaError_t err = cudaGetLastError();  // of the launch before
+  // segments of at most kShort units are dealt whole
+  if (err != cudaSuccess || p.c.L <= kShort * C::kKeys) return err;
+  const unsigned rows = p.R < C::kRows ? p.R : C::kRows;
+  tree_join_kernel<C><<<dim3(p.ctas, (rows + kJoinRows - 1) / kJoinRows), kThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
 // The parameters that go with the configuration.
 template <class C>
 void prepare(Params &p, void *workspace, const DeviceInfo &dev) {
@@ -1394,6 +1446,7 @@ void prepare(Params &p, void *workspace, const DeviceInfo &dev) {
   constexpr int kVec = C::kF32 ? 4 : 8;  // values in 16 bytes
   p.q_vec = q16 % 16 == 0 && p.qs.b % kVec == 0 && p.qs.h % kVec == 0 && p.qs.s % kVec == 0;
   p.o_vec = o16 % 16 == 0 && p.os.b % kVec == 0 && p.os.h % kVec == 0 && p.os.s % kVec == 0;
+  p.apart = p.R > 2;
   const int64_t segs = p.c.B * p.c.H * p.RT;
   const int64_t units = (p.c.L + C::kKeys - 1) / C::kKeys;  // of a segment, at most
   const int64_t most = (dev.sm_count < kMaxSms ? dev.sm_count : kMaxSms) * C::kCtas;
@@ -1411,7 +1464,7 @@ cudaError_t launch(Params p, void *workspace, const DeviceInfo &dev, cudaStream_
       reinterpret_cast<const void *>(tree_decode_kernel<C>), C::kSmem, dev.device);
   if (err != cudaSuccess) return err;
   tree_decode_kernel<C><<<p.ctas, kThreads, C::kSmem, stream>>>(p);
-  return cudaGetLastError();
+  return p.apart ? launch_join<C>(p, stream) : cudaGetLastError();
 }
 
 }  // namespace tree

@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
   } sh;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   if (ptx::timeout_flagged(p.status)) return;  // until the host clears it
-  if (tid == 0) p.split[blockIdx.x].b = -1;
+  if (tid == 0) p.split[blockIdx.x].b = -1;  // for the joining kernel
 
   int64_t begin, end, all;
   Cursor<C::kKeys> cur = share<C::kKeys>(p, begin, end, all);
@@ -720,15 +720,8 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
         }
       }
       ptx::tc_fence_before();  // O may be written again after this thread's next p_full
-      if (!done && headed && tid == 0) {  // goes on to the CTA of its last unit
-        Split s;
-        s.all = all;
-        s.b = cur.b;
-        s.h = cur.h;
-        s.tile = cur.tile;
-        s.last = (int)(((begin + i + cur.s.units - cur.u) * p.ctas - 1) / all);
-        p.split[blockIdx.x] = s;
-      }
+      if (!done && headed && tid == 0)
+        p.split[blockIdx.x] = split_of(p, cur, begin + i - cur.u, all);
       headed = true;
       cur.next(p);
       ++i;
@@ -743,29 +736,6 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
   }
 }
 
-// Joins the parts of the segments that more than one CTA worked on: block (x, y)
-// rows y kJoinRows.. of the one that begins in CTA x.  (In the kernel itself the
-// last CTA alone took 50 to 90 us for 60 rows of a segment in 7 to 37 parts.)
-constexpr int kJoinRows = 16;
-
-template <class C>
-__global__ void __launch_bounds__(kThreads) tree_join_kernel(const __grid_constant__ Params p) {
-  if (ptx::timeout_flagged(p.status)) return;
-  const Split s = p.split[blockIdx.x];
-  if (s.b < 0) return;
-  const Seq seq = sequence<C::kKeys>(p, s.b, false);
-  constexpr int kCols = C::D / 4;
-#pragma unroll 1
-  for (int x = threadIdx.x; x < kJoinRows * kCols; x += kThreads) {
-    const int r = blockIdx.y * kJoinRows + x / kCols, dd = x % kCols * 4;
-    if (s.tile * C::kRows + r >= p.R) return;
-    float m = -FLT_MAX, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    add_parts<C>(p, r, dd, blockIdx.x, s.last, 0, 1, s.all, m, l, o);
-    store_sums<C>(p, s.b, s.h, s.tile * C::kRows + r, seq.n, dd, l, o);
-  }
-}
-
 // ------------------------------------------------------------------ launch
 
 template <class C>
@@ -775,12 +745,7 @@ cudaError_t launch_wide(Params p, void *workspace, const DeviceInfo &dev, cudaSt
       reinterpret_cast<const void *>(tree_decode_wide_kernel<C>), C::kSmem, dev.device);
   if (err != cudaSuccess) return err;
   tree_decode_wide_kernel<C><<<p.ctas, kWideThreads, C::kSmem, stream>>>(p);
-  const cudaError_t launched = cudaGetLastError();
-  // segments of at most kShort units are dealt whole
-  if (launched != cudaSuccess || p.c.L <= kShort * C::kKeys) return launched;
-  const unsigned rows = p.R < C::kRows ? p.R : C::kRows;
-  tree_join_kernel<C><<<dim3(p.ctas, (rows + kJoinRows - 1) / kJoinRows), kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_join<C>(p, stream);
 }
 
 }  // namespace tree
