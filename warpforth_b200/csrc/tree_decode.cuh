@@ -329,11 +329,6 @@ struct Cursor {
   }
 };
 
-// Finds this CTA's share [begin, end) of the units and where it begins.  Where
-// no segment has more than kShort units the shares are whole segments: a few
-// units' difference in load costs less than joining parts.
-constexpr int kShort = 4;
-
 // What the joining kernel needs to know of the segment at c, which begins with
 // unit s0 and goes on to the CTA of its last unit: unit s lies in the last CTA x
 // with total x / ctas <= s.
@@ -355,6 +350,11 @@ __device__ __forceinline__ int64_t part_of(int64_t total, int x, int parts) {
   return total * x / parts;
 }
 
+constexpr int kShort = 4;
+
+// Finds this CTA's share [begin, end) of the units and where it begins.  Where
+// no segment has more than kShort units the shares are whole segments: a few
+// units' difference in load costs less than joining parts.
 template <int kKeys>
 __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, int64_t &end,
                                                int64_t &all) {
