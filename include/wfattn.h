@@ -274,7 +274,7 @@ WFATTN_API wfattn_status_t wfattn_decode_noalloc(int64_t batch, int64_t heads, i
  * (head_stride >= max_len and batch_stride >= the rows of a batch entry, or
  * the other way round; a stride over a size of 1 is not looked at).  k and v
  * are 16-byte aligned, the scales 4-byte aligned.  head_dim is 64 or 128;
- * batch * heads * max_len is at most 2^31 - 1 rows.
+ * batch * heads * max_len is at most 2^31 - 1024 rows.
  *
  * Lengths and positions are DEVICE int32 arrays.  An entry that points outside
  * the cache reads and writes nothing there, and wfattn_device_status() then
@@ -330,8 +330,8 @@ WFATTN_API wfattn_status_t wfattn_cache_read(const wfattn_cache_t *cache, int dt
  * was before the call (rows as stored, scales with them; any order of the
  * path, repeated entries too), and new_lens[b] = lens[b] + counts[b].  path is
  * [batch, depth] with rows path_stride entries apart, depth at most 64; counts
- * NULL: depth for every b.  new_lens is another array than lens
- * (WFATTN_INVALID_ARG): every head reads lens.
+ * NULL: depth for every b.  new_lens overlaps none of lens, path
+ * and counts (WFATTN_INVALID_ARG): every head reads them.
  * A sequence with a negative length, a count outside 0..depth, or a source or
  * destination row outside the cache moves nothing and keeps its length.
  */
@@ -349,6 +349,8 @@ WFATTN_API wfattn_status_t wfattn_cache_keep(const wfattn_cache_t *cache, const 
  *         F32, E4M3 or INT4 one.  Scores, softmax and sums are held in f32; F32
  *         outputs keep the f32 path's accuracy (~1e-6 of the values).
  * lens:   rows before the tree, lens[b] >= 0: every node sees them all.
+ *         At most 2^20 query rows (query heads times nodes) of one cache head.
+ *         o may be q.
  * nodes:  1..64 nodes; node j of sequence b is row lens[b] + j of the cache
  *         (written by wfattn_cache_write before this call).
  * tree:   64-bit words [batch, nodes], tree_stride words from one sequence to

@@ -28,8 +28,8 @@ def _read(cache, dtype=_lib.DTYPE_BF16, n=4, k=16, v=16, starts=16, strides=None
     return _lib.load().wfattn_cache_read(cache, dtype, n, k, st, v, st, starts, None, 0, None)
 
 
-def _keep(cache, lens=1024, depth=4, path=16, path_stride=4, new_lens=4096):
-    return _lib.load().wfattn_cache_keep(cache, lens, depth, path, path_stride, None, new_lens,
+def _keep(cache, lens=1024, depth=4, path=16, path_stride=4, new_lens=4096, counts=None):
+    return _lib.load().wfattn_cache_keep(cache, lens, depth, path, path_stride, counts, new_lens,
                                          None)
 
 
@@ -94,7 +94,9 @@ def test_no_rows_is_no_work():
 
 @pytest.mark.parametrize("bad", [{"lens": None}, {"path": None}, {"new_lens": None}, {"depth": 0},
                                  {"depth": 65}, {"path_stride": -4}, {"new_lens": 1024},
-                                 {"new_lens": 1028}, {"new_lens": 1020}])
+                                 {"new_lens": 1028}, {"new_lens": 1020}, {"path": 4092},
+                                 {"path": 4100}, {"path": 4096 - 7 * 4, "path_stride": 5},
+                                 {"counts": 4096}, {"counts": 4100}, {"counts": 4092}])
 def test_bad_paths_are_refused(bad):
     assert _keep(_cache(), **bad) == _lib.INVALID_ARG
 
@@ -123,6 +125,21 @@ def test_workspace_size_of_refused_shapes_is_zero():
     assert lib.wfattn_tree_decode_workspace_size(_cache(), _lib.DTYPE_BF16, 7, 4) == 0
     assert lib.wfattn_tree_decode_workspace_size(_cache(), _lib.DTYPE_BF16, 6, 65) == 0
     assert lib.wfattn_tree_decode_workspace_size(None, _lib.DTYPE_BF16, 6, 4) == 0
+
+
+def test_outgrown_workspaces_stay():
+    """A captured graph goes on using the buffer that it was captured with."""
+    from warpforth_b200 import DecodeWorkspace
+
+    ws, cpu = DecodeWorkspace(), torch.device("cpu")
+    small = ws.get_tree(5000, cpu)
+    assert small.numel() == 5000 and not small[:_lib.TREE_DECODE_ZEROED].any()
+    assert ws.get_tree(4096, cpu) is small
+    small[0] = 7
+    big = ws.get_tree(9000, cpu)
+    assert big.numel() == 9000 and not big[:_lib.TREE_DECODE_ZEROED].any()
+    assert ws.get_tree(5000, cpu) is big
+    assert any(b is small for b in ws.tree_buffers[cpu])
 
 
 def test_caches_need_cuda_tensors():

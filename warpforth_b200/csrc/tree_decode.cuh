@@ -10,8 +10,8 @@
 //
 // with mma.sync: rows of K and V go from shared memory through a conversion in
 // registers (codes to f16; nothing is written back), which tcgen05 operands in
-// shared or tensor memory would need a round trip for, and a step has 8 to 64
-// query rows where a tcgen05 tile has 128.  Products:
+// shared or tensor memory would need a round trip for, and there are up to 32
+// query rows where a tcgen05 tile has 128 (more: tree_decode_wide.cuh).  Products:
 //  * e4m3 / int4 rows: the codes (int4: u - 8) are exact in f16; scale and
 //    minimum of a row are applied to the f32 score and to the f32 weight;
 //  * bf16 rows: bf16 products, the weights as two bf16 terms (16 bits);
@@ -28,16 +28,20 @@
 // Work: a unit is kKeys keys of one (sequence, cache head, tile of query
 // rows); the units of all sequences in order are dealt in equal contiguous
 // shares to a grid of kCtas CTAs an SM, whatever the lengths (short segments
-// whole).  A CTA streams
-// its units through a ring of cp.async stages without regard to where a
-// segment (one sequence, head and tile) ends; a segment that lies in one CTA
-// is written out directly.  Of the others every CTA writes its part (maximum,
+// whole).  A CTA streams its units through a ring of cp.async stages without
+// regard to where a segment (one sequence, head and tile) ends; a segment that
+// lies in one CTA is written out directly.  Of the others every CTA writes its part (maximum,
 // sum, unnormalised output) to the workspace, and they are joined in their order:
 // the same bits every time.  With one or two rows the CTA whose part is the last
 // to arrive, by a counter, does that, without another launch; more rows would
 // keep that CTA busy (8 rows of 128 values in 27 parts 15 us, 60 rows in 7 parts
 // 40 us), so there a second kernel does.
 // Four warps split the keys of a unit or, with more rows, the rows.
+//
+// HBM bounds it where the conversion is short, issue slots where it is not.  One
+// token, ragged lengths: bf16 rows of 64 values 5.9 TB/s, e4m3 rows of 128 5.6,
+// e4m3 rows of 64 4.7 (64 x 25 heads, 145,600 keys of each head: 104 us), 4-bit
+// rows of 128 under 8 query heads 3.8 (32 x 8 heads, 342,100 keys: 98 us).
 #pragma once
 
 #include <float.h>
@@ -1400,6 +1404,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
 template <class C>
 size_t workspace_bytes() {
   static_assert(C::kCtas * kMaxSms <= kCounters, "a counter a CTA");
+  static_assert(C::kCtas * kMaxSms * sizeof(Split) % 16 == 0, "parts are read 16 bytes at a time");
   return kCounters * sizeof(unsigned int) + kMaxSms * C::kCtas * sizeof(Split) +
          (size_t)kMaxSms * C::kCtas * 2 * C::kRows * (C::D + 2) * sizeof(float);
 }

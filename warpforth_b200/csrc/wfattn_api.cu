@@ -540,8 +540,8 @@ wfattn_status_t check_cache(const wfattn_cache_t *c, CacheView *out) {
     return fail(WFATTN_INVALID_ARG, "cache sizes must be >= 1");
   int64_t bh = 0, rows = 0;
   if (__builtin_mul_overflow(c->batch, c->heads, &bh) ||
-      __builtin_mul_overflow(bh, c->max_len, &rows) || rows > INT32_MAX)
-    return fail(WFATTN_INVALID_ARG, "a cache holds at most 2^31-1 rows");
+      __builtin_mul_overflow(bh, c->max_len, &rows) || rows > kMaxCacheRows)
+    return fail(WFATTN_INVALID_ARG, "a cache holds at most 2^31-1024 rows");
   const bool scaled = c->format == WFATTN_CACHE_E4M3 || c->format == WFATTN_CACHE_INT4;
   if (!c->k || !c->v || (scaled && (!c->k_scale || !c->v_scale)))
     return fail(WFATTN_INVALID_ARG, "null cache pointer");
@@ -665,13 +665,18 @@ wfattn_status_t wfattn_cache_keep(const wfattn_cache_t *cache, const int32_t *le
   wfattn_status_t st = check_cache(cache, &a.c);
   if (st != WFATTN_OK) return st;
   if (!lens || !path || !new_lens) return fail(WFATTN_INVALID_ARG, "null tensor pointer");
-  const char *from = reinterpret_cast<const char *>(lens), *to = reinterpret_cast<char *>(new_lens);
-  if (from < to + 4 * a.c.B && to < from + 4 * a.c.B)
-    return fail(WFATTN_INVALID_ARG, "new_lens must be another array than lens");
   if (depth < 1 || depth > kMaxTreeNodes)
     return fail(WFATTN_INVALID_ARG, "depth must be in [1, %d] (got %lld)", kMaxTreeNodes,
                 (long long)depth);
   if (path_stride < 0) return fail(WFATTN_INVALID_ARG, "negative stride");
+  // every head's blocks read these while one writes new_lens
+  auto meets = [&](const int32_t *p, int64_t n) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(new_lens);
+    return x < y + 4 * (uintptr_t)a.c.B && y < x + 4 * (uintptr_t)n;
+  };
+  if (path_stride > (int64_t(1) << 40) || meets(lens, a.c.B) || (counts && meets(counts, a.c.B)) ||
+      meets(path, (a.c.B - 1) * path_stride + depth))
+    return fail(WFATTN_INVALID_ARG, "new_lens must be another array than lens, path and counts");
   a.lens = lens;
   a.path = path;
   a.counts = counts;

@@ -98,6 +98,10 @@ cudaError_t decode_noalloc_scratch(void **ptr);
 
 // ---- key/value caches (row formats: include/wfattn.h)
 
+// Rows of a cache, and so positions in it: a position rounded up to a unit of
+// keys still fits 32 bits.
+constexpr int64_t kMaxCacheRows = (int64_t(1) << 31) - 1024;
+
 struct CacheView {
   int format;  // wfattn_cache_format_t
   int D;       // 64 or 128

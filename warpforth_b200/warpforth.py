@@ -190,16 +190,19 @@ class DecodeWorkspace:
 
     def __init__(self) -> None:
         self.buffer: torch.Tensor | None = None
-        self.tree_buffer: torch.Tensor | None = None
+        self.tree_buffers: dict[torch.device, list[torch.Tensor]] = {}
 
     def get_tree(self, nbytes: int, device: torch.device) -> torch.Tensor:
-        """``tree_decode``'s own scratch: it begins with counters that only its calls may write."""
-        buffer = self.tree_buffer
-        if buffer is None or buffer.numel() < nbytes or buffer.device != device:
+        """``tree_decode``'s own scratch: it begins with counters that only its calls may write.
+        An outgrown buffer stays, for the captured graphs that use it."""
+        buffers = self.tree_buffers.get(device)
+        if buffers is None:
+            buffers = self.tree_buffers[device] = []
+        if not buffers or buffers[-1].numel() < nbytes:
             buffer = torch.empty(nbytes, dtype=torch.uint8, device=device)
             buffer[:_lib.TREE_DECODE_ZEROED].zero_()
-            self.tree_buffer = buffer
-        return buffer
+            buffers.append(buffer)
+        return buffers[-1]
 
     def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
         if self.buffer is None or self.buffer.numel() < nbytes or self.buffer.device != device:
