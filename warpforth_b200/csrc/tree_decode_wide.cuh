@@ -2,7 +2,7 @@
 // products on tcgen05 tensor cores.
 //
 // A CTA takes up to 128 query rows of one cache head (one TMEM lane, and one
-// thread, a row) and walks its keys in units of 64:
+// thread or two, a row) and walks its keys in units of 64:
 //
 //   S [128 x 64]   = Q [128 x D] K^T         both operands in shared memory
 //   O [128 x D]   += P [128 x 64] V          P in tensor memory
@@ -14,29 +14,34 @@
 // maximum and the split of work are those of tree_decode.cuh; bf16 weights take
 // two products (two terms).
 //
-// Warps 0-3 turn scores into weights, warps 4 and 5 bring the rows of the units,
-// warp 6 issues Q K^T and warp 7 P V (a product leaves a warp every 75 clocks or
-// so, which one warp's other work would add to).  K and V have two buffers, and so
-// have S and P, which share theirs (a thread has read its row of S before it
-// writes P): while the weights of unit i are made, Q K^T of i + 1 is done and
-// the rows of i + 2 follow P V of i.  TMEM columns: twice 64 for S and P, 64 or
-// 128 for O; 256 a CTA, two CTAs an SM.
+// Warps 0-3 (4-bit rows: 0-7, half a row's keys a thread) turn scores into
+// weights, the next two bring the rows of the units, one issues Q K^T and the last
+// P V (a product leaves a warp every 75 clocks or so, which one warp's other work
+// would add to).  K and V have two buffers, and so have S and P, which share
+// theirs (a thread, or both of a row, has read S before it writes P): while the
+// weights of unit i are made, Q K^T of i + 1 is done and the rows of i + 2 follow
+// P V of i.  TMEM columns: twice 64 for S and P, 64 or 128 for O; 256 a CTA, two
+// CTAs an SM.
 //
 // Measured: 61-node trees of 4 query heads a cache head over two e4m3 caches of
-// 65,000 and 131,000 keys, 8 heads of 128: 418 us, 469 TFLOP/s; a unit takes a CTA
-// about 3,500 clocks, 2,000 of them the weights (512 to issue 64 exponentials a
-// row) and 700 barriers.  15-node trees over 37,840 bf16 keys of 8 heads: 66 us.
+// 65,000 and 131,000 keys, 8 heads of 128: 410 us, 478 TFLOP/s.  A unit takes a
+// CTA about 4,000 clocks; rows are placed in 1,350, S is there 1,500 after Q K^T
+// begins, weights take 2,400 and P V 840.  No one of them is the bound: without
+// weights it would be 286 us, without conversion 349, with half the products 390.
+// 15-node trees over 37,840 keys of 8 heads: 65 us (bf16), 69 (4 bits).
 //
 // Every wait has a limit.  After one that runs out the warps that make weights
-// go on to the end without waiting.
+// go on to the end without waiting; the two of a row meet as often as ever.
 #pragma once
+
+#include <type_traits>
 
 #include "tree_decode.cuh"
 
 namespace wfattn {
 namespace tree {
 
-constexpr int kWideThreads = 2 * kThreads, kLoaders = 64;
+constexpr int kLoaders = 64;
 
 template <int kFmt_, int D_>
 struct WideCfg {
@@ -45,6 +50,14 @@ struct WideCfg {
   static constexpr bool kBf16Rows = kFmt == WFATTN_CACHE_BF16;
   static constexpr bool kScaled = !kBf16Rows;
   static constexpr int kRowBytes = CacheRow<kFmt, D>::kBytes;
+  // Threads of a query row.  4-bit rows take two, as their minima make the weights
+  // dearer: 15-node trees, 4 query heads on 8, 69 us against 79 (64 values a row: 52
+  // against 58); 61-node trees over 196,000 keys 417 against 434 (319 against 302).
+  // The others lose more by having 80 registers a thread: bf16 74 against 66, e4m3
+  // 91 against 81.
+  static constexpr int kHalves = kFmt == WFATTN_CACHE_INT4 ? 2 : 1;
+  static constexpr int kWeighers = kHalves * kThreads, kWideThreads = kWeighers + kThreads;
+  static constexpr int kMine = kKeys / kHalves, kDims = D / kHalves;  // of a thread's row
   static constexpr int kSlabs = D / 64;               // 128-byte wide slabs of an operand
   static constexpr int kSlab = kKeys * 128;           // bytes of a slab of K or V
   static constexpr int kQSlab = kRows * 128;
@@ -132,24 +145,40 @@ __device__ __forceinline__ float v_in_memory(const uint8_t *row, int d) {
   return ptx::f16x2_to_f32(ptx::e4m3x2_to_f16x2(row[d])).x;
 }
 
-// A thread's row of S to weights in tensor memory, at `sp`: maximum, sum and
-// (int4) the sum of weights times minima go on in m, l and om.  wait_o() waits
-// for the products added to O so far, and is called where O is changed.
-template <class C, bool kTail, class Wait>
-__device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &cur,
+// The other half's value of a row's pair of threads (`at` and `other` are their
+// places, `pair` their two warps' barrier).  Two sets of places take turns: one
+// is written again after the other's barrier, when it has been read.
+__device__ __forceinline__ float swap_halves(float x, float *at, const float *other, int pair) {
+  *at = x;
+  asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+  return *other;
+}
+
+// A thread's keys of its row of S, C::kMine * half and on, to weights in tensor
+// memory; sp is the row's.  Maximum, sum and (int4) the sum of weights times
+// minima go on in m, which both halves know, and l and om, which are this half's.
+// swap() gives the other half's value: its thread has read S when it returns, and
+// P may take its place.  wait_o() waits for the products added to O so far, and is
+// called where O is changed, C::kDims columns by each.
+template <class C, bool kTail, class Swap, class Wait>
+__device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &cur, int half,
                                       uint32_t row_tmem, uint32_t sp, int key0, bool odd,
                                       uint64_t word, float qf, float qsum, const float *k_scale,
                                       const float *k_mid, const float *v_scale, const float *v_mid,
-                                      float vtop, bool first, float &m, float &l, float &om, float &vinv,
-                                      Wait wait_o) {
-  uint32_t s[64];
-  ptx::tmem_ld_32x32b_x64(sp, s);
+                                      float vtop, bool first, float &m, float &l, float &om,
+                                      float &vinv, Swap swap, Wait wait_o) {
+  constexpr int kMine = C::kMine;
+  uint32_t s[kMine];
+  if constexpr (kMine == 64)
+    ptx::tmem_ld_32x32b_x64(sp, s);
+  else
+    ptx::tmem_ld32(sp + kMine * half, s);
   ptx::tmem_wait_ld();
   // ---- scores before qf, which is positive
   const uint64_t qsum2 = ptx::f2_pack(qsum, qsum);
   if constexpr (C::kScaled) {
 #pragma unroll
-    for (int k = 0; k < 64; k += 4) {
+    for (int k = 0; k < kMine; k += 4) {
       const ulonglong2 ks = *reinterpret_cast<const ulonglong2 *>(k_scale + k);
       uint64_t y0 = ptx::f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1]));
       uint64_t y1 = ptx::f2_pack(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3]));
@@ -168,7 +197,8 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
       for (int e = 0; e < 4; ++e) s[k + e] = __float_as_uint(x[e]);
     }
   }
-  uint64_t hidden = 0;  // keys this row does not see
+  uint64_t hidden = 0;  // keys of the unit this row does not see
+  std::conditional_t<kMine == 64, uint64_t, uint32_t> mine = 0;  // of this thread's
   if constexpr (kTail) {
     // key k is node k - at: bits of the row's word, or before the tree
     const int at = cur.s.len - key0;  // at most 63
@@ -176,16 +206,18 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
     const uint64_t seen = word & nodes;
     hidden = at >= 0 ? ~(at > 0 ? seen << at | ((uint64_t(1) << at) - 1) : seen)
                      : ~(at > -64 ? seen >> -at : 0);
+    mine = kMine == 64 ? hidden : hidden >> 32 * half;
 #pragma unroll
-    for (int k = 0; k < 64; ++k)
-      if (hidden >> k & 1) s[k] = 0xff800000u;
+    for (int k = 0; k < kMine; ++k)
+      if (mine >> k & 1) s[k] = 0xff800000u;
   }
   float high4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int k = 0; k < 64; k += 2)
+  for (int k = 0; k < kMine; k += 2)
     high4[k / 2 % 4] =
         ptx::fmax3(high4[k / 2 % 4], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-  const float high = fmaxf(fmaxf(high4[0], high4[1]), fmaxf(high4[2], high4[3]));
+  float high = fmaxf(fmaxf(high4[0], high4[1]), fmaxf(high4[2], high4[3]));
+  if constexpr (C::kHalves == 2) high = fmaxf(high, swap(high));
   if (__any_sync(0xffffffffu, fmaf(high, qf, -m) > 4.f || vtop * vinv > 2048.f)) {
     float ratio = 1.f;
     if (C::kScaled && vtop * vinv > 2048.f) {
@@ -202,7 +234,7 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
     if (!first) {
       wait_o();
 #pragma unroll 1
-      for (int c = 0; c < C::D; c += 16) {
+      for (int c = C::kDims * half; c < C::kDims * (half + 1); c += 16) {
         uint32_t o[16];
         tmem_ld16(row_tmem + C::kColO + c, o);
         ptx::tmem_wait_ld();
@@ -217,10 +249,10 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
   const uint64_t vinv2 = ptx::f2_pack(vinv, vinv);
   uint64_t l2[2] = {0, 0}, om2[2] = {0, 0};
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {  // 16 registers of weights at a time
+  for (int part = 0; part < kMine / 32; ++part) {  // 16 registers of weights at a time
     uint32_t hi[16], lo[C::kBf16Rows ? 16 : 1];
 #pragma unroll
-    for (int k = 32 * half; k < 32 * half + 32; k += 4) {
+    for (int k = 32 * part; k < 32 * part + 32; k += 4) {
       ulonglong2 vs = {0, 0}, mid = {0, 0};
       if constexpr (C::kScaled) vs = *reinterpret_cast<const ulonglong2 *>(v_scale + k);
       if constexpr (C::kFmt == WFATTN_CACHE_INT4)
@@ -236,8 +268,8 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
         b = ptx::ex2_approx(b);
         const uint64_t w = ptx::f2_pack(a, b);
         l2[e] = ptx::f2_add(l2[e], w);
-        const bool hide_a = kTail && (hidden >> kk & 1), hide_b = kTail && (hidden >> kk & 2);
-        const int to = (kk - 32 * half) / 2;
+        const bool hide_a = kTail && (mine >> kk & 1), hide_b = kTail && (mine >> kk & 2);
+        const int to = (kk - 32 * part) / 2;
         if constexpr (C::kScaled) {
           uint64_t vm = e ? mid.y : mid.x;
           if constexpr (C::kFmt == WFATTN_CACHE_INT4) {
@@ -259,8 +291,9 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
       }
     }
     // S is read: P takes its place
-    ptx::tmem_st16(sp + 16 * half, hi);
-    if constexpr (C::kBf16Rows) ptx::tmem_st16(sp + 32 + 16 * half, lo);
+    const uint32_t to = sp + kMine / 2 * half + 16 * part;
+    ptx::tmem_st16(to, hi);
+    if constexpr (C::kBf16Rows) ptx::tmem_st16(to + 32, lo);
   }
   float a, b;
   ptx::f2_unpack(ptx::f2_add(l2[0], l2[1]), a, b);
@@ -278,7 +311,7 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
       const int keys = min(64, cur.s.total - key0);
       wait_o();
 #pragma unroll 1
-      for (int c = 0; c < C::D; c += 16) {
+      for (int c = C::kDims * half; c < C::kDims * (half + 1); c += 16) {
         uint32_t o[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[e] = 0;
@@ -296,6 +329,7 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
             if (!(fabsf(y) <= FLT_MAX)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
           }
         }
+        __syncwarp();
         ptx::tmem_st16(row_tmem + C::kColO + c, o);
       }
     }
@@ -304,7 +338,7 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
 }
 
 template <class C>
-__global__ void __launch_bounds__(kWideThreads, C::kCtas)
+__global__ void __launch_bounds__(C::kWideThreads, C::kCtas)
     tree_decode_wide_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t raw_smem[];
   __shared__ struct {
@@ -318,9 +352,11 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
     alignas(16) float v_scale[2][C::kKeys];
     alignas(16) float v_mid[2][C::kKeys];
     float v_top[2][2];  // the largest scale of V's rows 0-31 and 32-63
+    float swap[2][C::kHalves == 2 ? C::kWeighers : 1];
   } sh;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  if (ptx::timeout_flagged(p.status)) return;  // until the host clears it
+  // until the host clears it; one answer for all, as warps wait for one another below
+  if (__syncthreads_or(ptx::timeout_flagged(p.status))) return;
   if (tid == 0) p.split[blockIdx.x].b = -1;  // for the joining kernel
 
   int64_t begin, end, all;
@@ -334,12 +370,12 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(bar(sh.kv_full[i]), kLoaders);
       ptx::mbar_init(bar(sh.s_full[i]), 2);  // the products, and their issuer
-      ptx::mbar_init(bar(sh.p_full[i]), kThreads);
+      ptx::mbar_init(bar(sh.p_full[i]), C::kWeighers);
       ptx::mbar_init(bar(sh.o_done[i]), 1);
       ptx::mbar_init(bar(sh.drain[i]), 1);
       sh.odd[i] = -1;
     }
-    ptx::mbar_init(bar(sh.q_full), kThreads);
+    ptx::mbar_init(bar(sh.q_full), C::kWeighers);
     ptx::fence_barrier_init();
   }
   if (warp == 0) {
@@ -350,8 +386,9 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  constexpr int kRest = C::kWeighers / 32;  // the first warp that makes no weights
 
-  if (warp >= 6) {
+  if (warp >= kRest + 2) {
     // -------------------------------------------------------------- products
     // The warp waits in step; lane 0 issues.
     const uint32_t leader = (tid & 31) == 0;
@@ -359,7 +396,7 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
       return __all_sync(0xffffffffu, ptx::mbar_wait(bar(b), parity, p.status)) != 0;
     };
     bool ok = true;
-    if (warp == 6) {
+    if (warp == kRest + 2) {
       const uint32_t idesc = idesc_wide(C::kBf16Rows, 64, false);
       uint32_t segment = 0;
 #pragma unroll 1
@@ -412,12 +449,12 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
       }
     }
     if (!ok) {  // every product issued has to end before the memory goes
-      commit_warp(leader, bar(sh.drain[warp - 6]));
-      ptx::mbar_wait_drain(bar(sh.drain[warp - 6]), 0);
+      commit_warp(leader, bar(sh.drain[warp - kRest - 2]));
+      ptx::mbar_wait_drain(bar(sh.drain[warp - kRest - 2]), 0);
     }
-  } else if (warp >= 4) {
+  } else if (warp >= kRest) {
     // --------------------------------------------------------- rows of K and V
-    const int t = tid - kThreads;
+    const int t = tid - C::kWeighers;
     constexpr int kRowPieces = C::kRowBytes / 16;
     Cursor<C::kKeys> ahead = cur;
     uint4 held[C::kBf16Rows ? 1 : 2 * C::kPieces];  // codes of K, then of V
@@ -583,7 +620,15 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
     if constexpr (C::kBf16Rows) cp_async_wait<0>();
   } else {
     // ---------------------------------------------------- weights, and results
-    const uint32_t row_tmem = tmem + ((uint32_t)(warp * 32) << 16);  // this thread's lane
+    // Threads of a TMEM lane, 128 apart, have a row; each of two half of its keys and columns.
+    const int row = tid % kThreads, half = tid / kThreads, quad = warp % 4;
+    const uint32_t row_tmem = tmem + ((uint32_t)(quad * 32) << 16);
+    int turn = 0;
+    // Every pass through here is the same for both: it depends on no wait.
+    auto swap = [&](float x) {
+      turn ^= 1;
+      return swap_halves(x, &sh.swap[turn][tid], &sh.swap[turn][tid ^ kThreads], 1 + quad);
+    };
     bool headed = cur.u == 0, failed = false;
     auto wait = [&](uint64_t &b, uint32_t parity) {
       if (!failed && !ptx::mbar_wait(bar(b), parity, p.status)) failed = true;
@@ -592,40 +637,42 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
 #pragma unroll 1
     while (i < units) {  // a segment, or the part of it in this share
       // ---- the query row of this thread as an operand, scaled into f16's range
-      const int r = cur.tile * C::kRows + tid;
-      const bool idle = cur.tile * C::kRows + warp * 32 >= p.R;  // the whole warp
+      const int r = cur.tile * C::kRows + row;
+      const bool idle = cur.tile * C::kRows + quad * 32 >= p.R;  // both warps
       float qf = p.scale_log2, qsum = 0.f;
       uint64_t word = 0;
       {
         const int hg = over_T(p, r), node = r - hg * p.T;
         const uint16_t *q = reinterpret_cast<const uint16_t *>(p.q) + cur.b * p.qs.b +
-                            ((int64_t)cur.h * p.G + hg) * p.qs.h + node * p.qs.s;
-        uint32_t w[C::D / 2];
+                            ((int64_t)cur.h * p.G + hg) * p.qs.h + node * p.qs.s + C::kDims * half;
+        uint32_t w[C::kDims / 2];
 #pragma unroll
-        for (int c = 0; c < C::D / 2; ++c) w[c] = 0;
+        for (int c = 0; c < C::kDims / 2; ++c) w[c] = 0;
         if (r < p.R) {
           word = p.tree ? p.tree[cur.b * p.tree_stride + node] : (2ull << node) - 1;
           if (p.q_vec) {
 #pragma unroll
-            for (int c = 0; c < C::D / 8; ++c) {
+            for (int c = 0; c < C::kDims / 8; ++c) {
               const uint4 y = reinterpret_cast<const uint4 *>(q)[c];
               w[4 * c] = y.x, w[4 * c + 1] = y.y, w[4 * c + 2] = y.z, w[4 * c + 3] = y.w;
             }
           } else {
 #pragma unroll
-            for (int c = 0; c < C::D / 2; ++c) w[c] = q[2 * c] | (uint32_t)q[2 * c + 1] << 16;
+            for (int c = 0; c < C::kDims / 2; ++c) w[c] = q[2 * c] | (uint32_t)q[2 * c + 1] << 16;
           }
         }
         if constexpr (!C::kBf16Rows) {
           uint32_t top = 0;
 #pragma unroll
-          for (int c = 0; c < C::D / 2; ++c) top = __vmaxu2(top, w[c] & 0x7fff7fffu);
-          const int e = (int)(max(top >> 16, top & 0xffffu) >> 7);  // exponent field
-          const int f = min(max(268 - e, 1), 253);                  // 2^14 <= top * mul < 2^15
+          for (int c = 0; c < C::kDims / 2; ++c) top = __vmaxu2(top, w[c] & 0x7fff7fffu);
+          top = max(top >> 16, top & 0xffffu) >> 7;  // exponent field
+          int e = (int)top;
+          if constexpr (C::kHalves == 2) e = max(e, __float_as_int(swap(__int_as_float(e))));
+          const int f = min(max(268 - e, 1), 253);  // 2^14 <= top * mul < 2^15
           const float mul = __uint_as_float((uint32_t)f << 23);
           qf = p.scale_log2 * __uint_as_float((uint32_t)(254 - f) << 23);
 #pragma unroll
-          for (int c = 0; c < C::D / 8; ++c) {
+          for (int c = 0; c < C::kDims / 8; ++c) {
             float x[8];
 #pragma unroll
             for (int v = 0; v < 8; ++v) {
@@ -637,10 +684,11 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
 #pragma unroll
             for (int v = 0; v < 4; ++v) w[4 * c + v] = pack_f16x2(x[2 * v], x[2 * v + 1]);
           }
+          if constexpr (C::kHalves == 2) qsum += swap(qsum);
         }
 #pragma unroll
-        for (int c = 0; c < C::D / 8; ++c)
-          sts128(q_at + piece(tid, c, C::kQSlab),
+        for (int c = 0; c < C::kDims / 8; ++c)
+          sts128(q_at + piece(row, C::kDims / 8 * half + c, C::kQSlab),
                  make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
       }
       ptx::fence_proxy_async_smem();
@@ -655,22 +703,26 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
         wait(sh.s_full[buf], parity);
         ptx::tc_fence_after();
         const bool odd = sh.odd[buf] == (int)(i & 0x7fffffff);
-        // a wait ends the same way for a warp, whose loads and stores are common
-        if (!idle && __all_sync(0xffffffffu, !failed)) {
+        __syncwarp();
+        // after a wait that failed as before it: the other half's warp counts on this one
+        if (!idle) {
           const float vtop = C::kScaled ? fmaxf(sh.v_top[buf][0], sh.v_top[buf][1]) : 0.f;
+          const int k0 = C::kMine * half;
           auto wait_o = [&]() {
             if (i > 0) wait(sh.o_done[buf ^ 1], (uint32_t)((i - 1) >> 1) & 1);
             ptx::tc_fence_after();
             __syncwarp();
           };
           if ((cur.u + 1) * C::kKeys > cur.s.len)
-            weigh<C, true>(p, cur, row_tmem, row_tmem + C::kColS + 64 * buf, cur.u * C::kKeys, odd,
-                           word, qf, qsum, sh.k_scale[buf], sh.k_mid[buf], sh.v_scale[buf],
-                           sh.v_mid[buf], vtop, first, m, l, om, vinv, wait_o);
+            weigh<C, true>(p, cur, half, row_tmem, row_tmem + C::kColS + 64 * buf,
+                           cur.u * C::kKeys, odd, word, qf, qsum, sh.k_scale[buf] + k0,
+                           sh.k_mid[buf] + k0, sh.v_scale[buf] + k0, sh.v_mid[buf] + k0, vtop,
+                           first, m, l, om, vinv, swap, wait_o);
           else
-            weigh<C, false>(p, cur, row_tmem, row_tmem + C::kColS + 64 * buf, cur.u * C::kKeys,
-                            odd, word, qf, qsum, sh.k_scale[buf], sh.k_mid[buf], sh.v_scale[buf],
-                            sh.v_mid[buf], vtop, first, m, l, om, vinv, wait_o);
+            weigh<C, false>(p, cur, half, row_tmem, row_tmem + C::kColS + 64 * buf,
+                            cur.u * C::kKeys, odd, word, qf, qsum, sh.k_scale[buf] + k0,
+                            sh.k_mid[buf] + k0, sh.v_scale[buf] + k0, sh.v_mid[buf] + k0, vtop,
+                            first, m, l, om, vinv, swap, wait_o);
         }
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(sh.p_full[buf]));
@@ -685,16 +737,20 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
       wait(sh.o_done[i & 1], (uint32_t)(i >> 1) & 1);
       ptx::tc_fence_after();
       const bool whole = done && headed;
+      if constexpr (C::kHalves == 2) {
+        l += swap(l);
+        om += swap(om);
+      }
       const int64_t slot = (int64_t)blockIdx.x * 2 + (headed ? 1 : 0);
       if (!idle && __all_sync(0xffffffffu, !failed)) {
         bool live = false;
         uint8_t *to = out_row(p, cur.b, cur.h, r, cur.s.n, 2, live);
-        float *part = p.part + (slot * C::kRows + tid) * C::D;
+        float *part = p.part + (slot * C::kRows + row) * C::D;
         const float back = C::kScaled ? 1.f / vinv : 1.f;
         const bool some = live && l != 0.f;
         const float inv = 1.f / l;
 #pragma unroll 1
-        for (int c = 0; c < C::D; c += 32) {
+        for (int c = C::kDims * half; c < C::kDims * (half + 1); c += 32) {
           uint32_t o[32];
           ptx::tmem_ld32(row_tmem + C::kColO + c, o);
           ptx::tmem_wait_ld();
@@ -718,8 +774,8 @@ __global__ void __launch_bounds__(kWideThreads, C::kCtas)
                   make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
           }
         }
-        if (to && !whole) {
-          float *ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D + (slot * C::kRows + tid) * 2;
+        if (to && !whole && half == 0) {
+          float *ml = p.part + (int64_t)p.ctas * 2 * C::kRows * C::D + (slot * C::kRows + row) * 2;
           ml[0] = m;
           ml[1] = l;
         }
@@ -749,7 +805,7 @@ cudaError_t launch_wide(Params p, void *workspace, const DeviceInfo &dev, cudaSt
   const cudaError_t err = ensure_smem_attr(
       reinterpret_cast<const void *>(tree_decode_wide_kernel<C>), C::kSmem, dev.device);
   if (err != cudaSuccess) return err;
-  tree_decode_wide_kernel<C><<<p.ctas, kWideThreads, C::kSmem, stream>>>(p);
+  tree_decode_wide_kernel<C><<<p.ctas, C::kWideThreads, C::kSmem, stream>>>(p);
   return launch_join<C>(p, stream);
 }
 
