@@ -660,6 +660,34 @@ def test_captured_steps_replay_with_new_lengths(wf, fmt, dtype):
         check(got, ref, tol)
 
 
+@pytest.mark.parametrize("n", [1, 16])
+def test_a_captured_step_outlives_its_workspace(wf, n):
+    """A larger call through the same workspace gets a larger buffer; a graph
+    captured before replays with the one that it has."""
+    d, ws = 64, wf.DecodeWorkspace()
+    small = make_cache(wf, "e4m3", 1, 1, 200 + n, d, 24)
+    large = make_cache(wf, "e4m3", 10, 8, 516, 128, 25)
+    gen = torch.Generator().manual_seed(26)
+    q = torch.randn(1, 4, n, d, generator=gen).bfloat16().cuda()
+    lens, out = ints([200]), torch.zeros_like(q)
+    want = wf.tree_decode(q, small, lens, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        wf.tree_decode(q, small, lens, out=out, workspace=ws)
+    before = ws.get_tree(1, q.device)
+    big = torch.randn(10, 32, 16, 128, generator=gen).bfloat16().cuda()
+    all_lens = ints([500 - 7 * i for i in range(10)])
+    want_big = wf.tree_decode(big, large, all_lens)
+    for _ in range(2):
+        got_big = wf.tree_decode(big, large, all_lens, workspace=ws)
+        graph.replay()
+        assert torch.equal(got_big, want_big)
+        assert torch.equal(out, want)
+        out.zero_()
+    assert ws.get_tree(1, q.device).numel() > before.numel()
+
+
 def test_calls_on_two_streams_at_once(wf):
     d, n, length = 128, 8, 3000
     caches = [make_cache(wf, "e4m3", 1, 2, length + n, d, 19 + i) for i in range(2)]
