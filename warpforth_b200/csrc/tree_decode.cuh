@@ -1412,8 +1412,9 @@ size_t workspace_bytes() {
 // Joins the parts of the segments that more than one CTA worked on.  A thread takes
 // four values of a row and, where there are few rows, every kth of its parts: all
 // the loads there are should be in flight at once, as a round of them takes a
-// microsecond.  One 15-node tree over 4,000 bf16 rows (8 heads, 37 parts each, 60
-// rows): 5 us, against 30 with four rows a thread one after the other.
+// microsecond.  One 15-node tree over 4,000 bf16 rows, 8 heads of 37 parts each: a
+// call takes 25 us, against 43 with four rows a thread one after the other and
+// all of a row's parts; with one cache head of 63 parts 17 against 63.
 constexpr int kJoinThreads = 256, kJoinBlocks = 3 * kMaxSms;
 
 template <class C>
@@ -1429,10 +1430,17 @@ __global__ void __launch_bounds__(kJoinThreads, 3)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // after a wait ran out the records may be another call's
   if (C::kWide && __syncthreads_or(ptx::timeout_flagged(p.status))) return;
+  constexpr int kTimes = (kMaxSms * C::kCtas + kJoinThreads - 1) / kJoinThreads;
+  bool goes_on[kTimes];
+#pragma unroll
+  for (int t = 0; t < kTimes; ++t) {
+    const int x = t * kJoinThreads + tid;
+    goes_on[t] = x < p.ctas && p.split[x].b >= 0;
+  }
   int segments = 0;
-#pragma unroll 1
-  for (int x0 = 0; x0 < p.ctas; x0 += kJoinThreads) {  // in order, the same in every block
-    const bool live = x0 + tid < p.ctas && p.split[x0 + tid].b >= 0;
+#pragma unroll
+  for (int t = 0; t < kTimes; ++t) {  // in order, the same in every block
+    const bool live = goes_on[t];
     const unsigned mask = __ballot_sync(0xffffffffu, live);
     if (lane == 0) counts[warp] = __popc(mask);
     __syncthreads();
@@ -1442,7 +1450,7 @@ __global__ void __launch_bounds__(kJoinThreads, 3)
       if (w < warp) at += counts[w];
       segments += counts[w];
     }
-    if (live) heads[at] = x0 + tid;
+    if (live) heads[at] = t * kJoinThreads + tid;
     __syncthreads();
   }
   const int rows = min(C::kRows, p.R), total = segments * rows;
@@ -1455,6 +1463,7 @@ __global__ void __launch_bounds__(kJoinThreads, 3)
     const int i = i0 + team, head = heads[min(i, total - 1) / rows], r = i % rows;
     const Split s = p.split[head];
     const bool live = i < total && s.tile * C::kRows + r < p.R;
+    const int n = sequence<C::kKeys>(p, s.b, false).n;
     float m = -FLT_MAX, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live) add_parts<C>(p, r, dd, head, s.last, group, k, s.all, m, l, o);
@@ -1478,10 +1487,8 @@ __global__ void __launch_bounds__(kJoinThreads, 3)
       }
       __syncthreads();
     }
-    if (live && group == 0) {
-      const Seq seq = sequence<C::kKeys>(p, s.b, false);
-      store_sums<C>(p, s.b, s.h, s.tile * C::kRows + r, seq.n, dd, l, o);
-    }
+    if (live && group == 0)
+      store_sums<C>(p, s.b, s.h, s.tile * C::kRows + r, n, dd, l, o);
   }
 }
 
