@@ -389,6 +389,29 @@ def test_tree_decode_over_long_rows(wf, fmt, dtype):
 
 
 @pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("b,longest", [(33, 1100), (129, 600), (300, 300)])
+@pytest.mark.parametrize("g,n", [(2, 1), (3, 4), (8, 5)])
+def test_tree_decode_of_many_sequences(wf, fmt, dtype, b, longest, g, n):
+    """More sequences than a warp, and than a block, has threads to share them out; the longest are
+    dealt in units (4-bit rows of few queries: with 33 sequences only) and many are empty."""
+    d, gen = 64, torch.Generator().manual_seed(b)
+    rng = np.random.default_rng(b)
+    lens = [int(x) for x in rng.integers(0, 40, b)]
+    for i in range(0, b, 7):
+        lens[i] = 0
+    lens[3] = lens[b - 2] = longest
+    cache = wf.KVCache(b, 1, longest + n, d, fmt=fmt)
+    x = torch.randn(2, b, 1, longest + n, d, generator=gen).cuda()
+    wf.cache_write(cache, x[0], x[1], ints([0] * b))
+    q = torch.randn(b, g, n, d, generator=gen).to(TYPES[dtype])
+    words = wf.tree_words(random_trees(b, n, b))
+    nodes = [int(x) for x in rng.integers(0, n + 1, b)]
+    out = wf.tree_decode(q.cuda(), cache, ints(lens), tree=words.cuda(), nodes=ints(nodes))
+    ref, tol = attend(fmt, cache, q, lens, words.tolist(), nodes)
+    check(out, ref, tol)
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
 def test_masked_and_missing_rows_never_reach_an_output(wf, fmt, dtype):
     """Rows past the end hold NaN; node 2 holds NaN and infinities, and nodes 2 and 4 see it."""
     b, h, d, n, lmax = 2, 2, 64, 6, 80

@@ -52,7 +52,7 @@
 namespace wfattn {
 namespace tree {
 
-constexpr int kThreads = 128, kWarps = 4;
+constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kMaxSms = 148;  // CTAs are dealt for at most this many SMs
 
 // Counters of arrived parts, at the start of the workspace: zero before the
@@ -358,11 +358,12 @@ constexpr int kShort = 4;
 
 // Finds this CTA's share [begin, end) of the units and where it begins.  Where
 // no segment has more than kShort units the shares are whole segments: a few
-// units' difference in load costs less than joining parts.
+// units' difference in load costs less than joining parts.  All the block's warps
+// call it; the sequences are shared out over its first kThreads threads.
 template <int kKeys>
 __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, int64_t &end,
                                                int64_t &all) {
-  __shared__ int64_t warp_sum[8], offset, stop;
+  __shared__ int64_t warp_sum[kWarps], offset, stop;
   __shared__ Cursor<kKeys> found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int B = (int)p.c.B, per = (B + kThreads - 1) / kThreads;
@@ -382,10 +383,11 @@ __device__ __forceinline__ Cursor<kKeys> share(const Params &p, int64_t &begin, 
     const int64_t y = __shfl_up_sync(0xffffffffu, upto, x);
     if (lane >= x) upto += y;
   }
-  if (lane == 31) warp_sum[warp] = upto;
+  if (lane == 31 && warp < kWarps) warp_sum[warp] = upto;
   const bool whole = !__syncthreads_or(longest > kShort);
   all = 0;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) {
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
     if (w < warp) upto += warp_sum[w];
     all += warp_sum[w];
   }
