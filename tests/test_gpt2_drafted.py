@@ -37,6 +37,86 @@ def test_acceptance_walks_the_chosen_tokens():
     assert accepted_path([3], [-1], [3]) == [0]
 
 
+class PlainCache:
+    """A KVCache's rows in plain tensors."""
+
+    def __init__(self, batch, heads, max_len, head_dim, *, fmt, device):
+        self.k, self.v = (torch.zeros(batch, heads, max_len, head_dim) for _ in range(2))
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """warpforth_b200.gpt2 with the cache calls in plain operations, for one f32 sequence."""
+    from warpforth_b200 import gpt2
+
+    def write(cache, k, v, starts):
+        at = slice(int(starts), int(starts) + k.shape[2])
+        cache.k[:, :, at], cache.v[:, :, at] = k, v
+
+    def read(cache, starts, rows, dtype):
+        return cache.k[:, :, :rows], cache.v[:, :, :rows]
+
+    def keep(cache, lens, path):
+        for t in (cache.k, cache.v):
+            t[:, :, int(lens):int(lens) + path.shape[1]] = t[:, :, int(lens) + path[0].long()]
+        return lens + path.shape[1]
+
+    def attend(q, k, v, mask, scale):
+        return (q @ k.mT * scale).masked_fill(~mask, -torch.inf).softmax(-1) @ v
+
+    def tree(q, cache, lens, tree, scale, workspace):
+        rows, n = int(lens), q.shape[2]
+        sees = (tree[:, None] >> torch.arange(n) & 1).bool()
+        mask = torch.cat([torch.ones(n, rows, dtype=torch.bool), sees], 1)
+        return attend(q, cache.k[:, :, :rows + n], cache.v[:, :, :rows + n], mask, scale)
+
+    def causal(q, k, v, causal, scale):
+        n, rows = q.shape[2], k.shape[2]
+        return attend(q, k, v, torch.ones(n, rows, dtype=torch.bool).tril(rows - n), scale)
+
+    for name, f in (("KVCache", PlainCache), ("cache_write", write), ("cache_read", read),
+                    ("cache_keep", keep), ("tree_decode", tree), ("attention", causal)):
+        monkeypatch.setattr(gpt2, name, f)
+    return gpt2
+
+
+def _small_gpt2(seed=0, attention="eager", **kw):
+    from transformers import GPT2Config, GPT2LMHeadModel
+
+    torch.manual_seed(seed)
+    model = GPT2LMHeadModel(GPT2Config(n_layer=3, n_embd=128, n_head=2, vocab_size=50,
+                                       n_positions=64, initializer_range=0.2, **kw)).eval()
+    if attention:
+        model.set_attn_implementation(attention)
+    return model
+
+
+def _greedy(model, prompt, count):
+    ids = prompt
+    with torch.no_grad():
+        for _ in range(count):
+            ids = torch.cat([ids, model(ids, use_cache=False).logits[:, -1:].argmax(-1)], 1)
+    return ids
+
+
+@pytest.mark.parametrize("nodes,chunk", [(1, 512), (9, 512), (64, 3)])
+def test_small_models_generate_the_greedy_tokens(on_cpu, nodes, chunk):
+    model, prompt = _small_gpt2(), torch.arange(10).remainder(4)[None]
+    want = _greedy(model, prompt, 20)
+    got, _ = on_cpu.generate_drafted(model, prompt, 20, nodes=nodes, prompt_chunk=chunk)
+    assert got.tolist() == want.tolist()
+
+
+@pytest.mark.parametrize("kw", [dict(attention=None), dict(attention="sdpa"),
+                                dict(reorder_and_upcast_attn=True)])
+def test_models_that_pass_the_cache_by_are_refused(on_cpu, kw):
+    model = _small_gpt2(**kw)
+    with pytest.raises(RuntimeError, match="eager"):
+        on_cpu.generate_drafted(model, torch.arange(10)[None], 5)
+    # and the model attends as it did before
+    _greedy(model, torch.arange(10)[None], 1)
+
+
 @pytest.fixture(scope="module")
 def gpt2():
     if not torch.cuda.is_available():

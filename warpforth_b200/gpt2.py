@@ -125,9 +125,22 @@ class _CachedAttention:
         self.length = 0  # the same on the host
         self.words: torch.Tensor | None = None  # of the drafted tree; None in the prompt
         self.workspace = DecodeWorkspace()
+        self.reached: list[int] = []  # layers whose attention ran here in this forward
+
+    def forward(self, model, ids: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        """The model's logits, every layer having attended over its cache."""
+        self.reached.clear()
+        logits = model(ids, position_ids=positions, use_cache=False).logits
+        if self.reached != list(range(len(self.caches))):
+            raise RuntimeError(
+                "the model's attention does not run over the cache (layers reached: "
+                f"{self.reached}): generate_drafted needs eager attention "
+                '(model.set_attn_implementation("eager")) without reorder_and_upcast_attn')
+        return logits
 
     def __call__(self, module, query, key, value, attention_mask=None, scaling=None, dropout=0.0,
                  **kwargs):
+        self.reached.append(module.layer_idx)
         cache = self.caches[module.layer_idx]
         cache_write(cache, key, value, self.lens)
         if self.words is not None:
@@ -204,7 +217,8 @@ def generate_drafted(model, prompt: torch.Tensor, max_new_tokens: int, *, nodes:
                      cache: str = "f32", prompt_chunk: int = 512) -> tuple[torch.Tensor, int]:
     """Greedy generation with drafted trees of up to ``nodes`` tokens over a ``cache`` of that format.
 
-    prompt: [1, n].  A prompt longer than ``prompt_chunk`` is read in parts.  Over an f32 cache the
+    model: a GPT2LMHeadModel in eager mode (RuntimeError where its attention does not run over the
+    cache).  prompt: [1, n].  A prompt longer than ``prompt_chunk`` is read in parts.  Over an f32 cache the
     tokens are those of ``generate`` (but for ties); the other formats round what is attended to.
     Returns the tokens [1, n + max_new_tokens] and how many times the model ran after the prompt.
     """
@@ -224,7 +238,7 @@ def generate_drafted(model, prompt: torch.Tensor, max_new_tokens: int, *, nodes:
         for at in range(0, ids.shape[1], prompt_chunk):
             part = ids[:, at:at + prompt_chunk]
             positions = torch.arange(at, at + part.shape[1], device=device)[None]
-            logits = model(part, position_ids=positions, use_cache=False).logits
+            logits = state.forward(model, part, positions)
             state.lens = state.lens + part.shape[1]
             state.length += part.shape[1]
         tokens.append(int(logits[0, -1].argmax()))
@@ -242,8 +256,7 @@ def generate_drafted(model, prompt: torch.Tensor, max_new_tokens: int, *, nodes:
                 parents = [renamed.get(parent, -1) for parent in parents]
             state.words = tree_words(parents).to(device)
             positions = torch.tensor([[state.length + depth for depth in depths]], device=device)
-            logits = model(torch.tensor([drafted], device=device), position_ids=positions,
-                           use_cache=False).logits
+            logits = state.forward(model, torch.tensor([drafted], device=device), positions)
             runs += 1
             chosen = logits[0].argmax(-1).tolist()
             path = accepted_path(drafted, parents, chosen)
