@@ -117,6 +117,34 @@ def test_models_that_pass_the_cache_by_are_refused(on_cpu, kw):
     _greedy(model, torch.arange(10)[None], 1)
 
 
+def test_other_models_and_threads_attend_as_ever_meanwhile(on_cpu, monkeypatch):
+    """While one model generates: another one runs in the same thread, the same one in another, and
+    a second generation begins and ends in a third."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    import transformers.models.gpt2.modeling_gpt2 as gpt2_module
+
+    stock = gpt2_module.eager_attention_forward
+    model, other = _small_gpt2(0), _small_gpt2(1)
+    prompt = torch.arange(10).remainder(4)[None]
+    want, want_other = _greedy(model, prompt, 12), _greedy(other, prompt, 12)
+    tree, seen = on_cpu.tree_decode, []
+
+    def meddled(*args, **kwargs):
+        monkeypatch.setattr(on_cpu, "tree_decode", tree)  # once
+        seen.append(_greedy(other, prompt, 12))
+        with ThreadPoolExecutor(1) as pool:
+            seen.append(pool.submit(_greedy, model, prompt, 12).result())
+            seen.append(pool.submit(on_cpu.generate_drafted, other, prompt, 12).result()[0])
+        return tree(*args, **kwargs)
+
+    monkeypatch.setattr(on_cpu, "tree_decode", meddled)
+    got, _ = on_cpu.generate_drafted(model, prompt, 12)
+    assert got.tolist() == want.tolist()
+    assert [x.tolist() for x in seen] == [x.tolist() for x in (want_other, want, want_other)]
+    assert gpt2_module.eager_attention_forward is stock
+
+
 @pytest.fixture(scope="module")
 def gpt2():
     if not torch.cuda.is_available():

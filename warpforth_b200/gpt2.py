@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import argparse
 import contextlib
+import threading
 import time
 from collections.abc import Callable
 
@@ -125,6 +126,7 @@ class _CachedAttention:
         self.length = 0  # the same on the host
         self.words: torch.Tensor | None = None  # of the drafted tree; None in the prompt
         self.workspace = DecodeWorkspace()
+        self.modules = set(model.modules())
         self.reached: list[int] = []  # layers whose attention ran here in this forward
 
     def forward(self, model, ids: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
@@ -200,16 +202,45 @@ def accepted_path(drafted: list[int], parents: list[int], chosen: list[int]) -> 
         path.append(following[0])
 
 
+# Generations that run now, one a thread: transformers looks its eager attention up in the module
+# that all models share, so what stands there sends a layer to the generation of its own thread and
+# model, and every other to the function that stood there before.
+_generating = threading.local()
+_routing = threading.Lock()
+_routed = 0
+
+
+def _route(otherwise: Callable) -> Callable:
+    def routed_attention(module, *args, **kwargs):
+        state = getattr(_generating, "state", None)
+        if state is not None and module in state.modules:
+            return state(module, *args, **kwargs)
+        return otherwise(module, *args, **kwargs)
+
+    routed_attention.otherwise = otherwise
+    return routed_attention
+
+
 @contextlib.contextmanager
-def _eager_attention(function):
+def _attention_of(state: _CachedAttention):
+    """This thread's calls of the model's layers go to `state`."""
+    global _routed
     import transformers.models.gpt2.modeling_gpt2 as gpt2_module
 
-    original = gpt2_module.eager_attention_forward
-    gpt2_module.eager_attention_forward = function
+    with _routing:
+        _routed += 1
+        if not hasattr(gpt2_module.eager_attention_forward, "otherwise"):
+            gpt2_module.eager_attention_forward = _route(gpt2_module.eager_attention_forward)
+    before, _generating.state = getattr(_generating, "state", None), state
     try:
         yield
     finally:
-        gpt2_module.eager_attention_forward = original
+        _generating.state = before
+        with _routing:
+            _routed -= 1
+            now = gpt2_module.eager_attention_forward
+            if _routed == 0 and hasattr(now, "otherwise"):
+                gpt2_module.eager_attention_forward = now.otherwise
 
 
 @torch.no_grad()
@@ -234,7 +265,7 @@ def generate_drafted(model, prompt: torch.Tensor, max_new_tokens: int, *, nodes:
         raise ValueError(f"the model has {limit} positions, {end} are asked for")
     state = _CachedAttention(model, end + nodes, cache)
     runs = 0
-    with _eager_attention(state):
+    with _attention_of(state):
         for at in range(0, ids.shape[1], prompt_chunk):
             part = ids[:, at:at + prompt_chunk]
             positions = torch.arange(at, at + part.shape[1], device=device)[None]
