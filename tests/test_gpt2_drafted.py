@@ -117,6 +117,15 @@ def test_models_that_pass_the_cache_by_are_refused(on_cpu, kw):
     _greedy(model, torch.arange(10)[None], 1)
 
 
+@pytest.mark.parametrize("dtype,cache", [(torch.bfloat16, "f32"), (torch.float32, "bf16"),
+                                         (torch.float16, "f32"), (torch.float32, "e5m2")])
+def test_caches_that_the_queries_do_not_take_are_refused_first(on_cpu, monkeypatch, dtype, cache):
+    model = _small_gpt2().to(dtype)
+    monkeypatch.setattr(model, "forward", None)  # never called
+    with pytest.raises(ValueError, match="bfloat16 models .*'bf16'"):
+        on_cpu.generate_drafted(model, torch.arange(10)[None], 5, cache=cache)
+
+
 def test_other_models_and_threads_attend_as_ever_meanwhile(on_cpu, monkeypatch):
     """While one model generates: another one runs in the same thread, the same one in another, and
     a second generation begins and ends in a third."""

@@ -243,21 +243,31 @@ def _attention_of(state: _CachedAttention):
                 gpt2_module.eager_attention_forward = now.otherwise
 
 
+# caches that tree_decode takes with a model's queries
+_CACHES = {torch.float32: ("f32", "e4m3", "int4"), torch.bfloat16: ("bf16", "e4m3", "int4")}
+
+
 @torch.no_grad()
 def generate_drafted(model, prompt: torch.Tensor, max_new_tokens: int, *, nodes: int = 12,
                      cache: str = "f32", prompt_chunk: int = 512) -> tuple[torch.Tensor, int]:
     """Greedy generation with drafted trees of up to ``nodes`` tokens over a ``cache`` of that format.
 
     model: a GPT2LMHeadModel in eager mode (RuntimeError where its attention does not run over the
-    cache).  prompt: [1, n].  A prompt longer than ``prompt_chunk`` is read in parts.  Over an f32 cache the
-    tokens are those of ``generate`` (but for ties); the other formats round what is attended to.
+    cache), in f32 (caches "f32", "e4m3", "int4") or bf16 ("bf16", "e4m3", "int4").  prompt: [1, n];
+    one longer than ``prompt_chunk`` is read in parts.  Over an f32 cache the tokens are those of
+    ``generate`` (but for ties); the other formats round what is attended to.
     Returns the tokens [1, n + max_new_tokens] and how many times the model ran after the prompt.
     """
     if prompt.dim() != 2 or prompt.shape[0] != 1 or prompt.shape[1] < 1:
         raise ValueError(f"prompt must be [1, n], got {tuple(prompt.shape)}")
     if max_new_tokens < 1 or not 1 <= nodes <= 64 or prompt_chunk < 1:
         raise ValueError("max_new_tokens and prompt_chunk must be >= 1, nodes in 1..64")
-    device = next(model.parameters()).device
+    weight = next(model.parameters())
+    device = weight.device
+    takes = _CACHES.get(weight.dtype)
+    if takes is None or cache not in takes:
+        raise ValueError(f"cache={cache!r} for a model of {weight.dtype}: float32 models take "
+                         f"{_CACHES[torch.float32]}, bfloat16 models {_CACHES[torch.bfloat16]}")
     ids = prompt.to(device)
     tokens, end = prompt[0].tolist(), prompt.shape[1] + max_new_tokens
     limit = model.config.n_positions
