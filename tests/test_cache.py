@@ -142,6 +142,24 @@ def test_outgrown_workspaces_stay():
     assert any(b is small for b in ws.tree_buffers[cpu])
 
 
+def test_a_buffer_made_in_a_capture_is_not_kept(monkeypatch):
+    """Its counters are zero only when the graph has run."""
+    from warpforth_b200 import DecodeWorkspace, warpforth
+
+    ws, cpu, capturing = DecodeWorkspace(), torch.device("cpu"), [True]
+    monkeypatch.setattr(warpforth, "_capturing", lambda device: capturing[0], raising=False)
+    first = ws.get_tree(5000, cpu)
+    assert first.numel() == 5000 and ws.get_tree(5000, cpu) is not first
+    capturing[0] = False
+    kept = ws.get_tree(5000, cpu)
+    assert kept is not first and ws.get_tree(5000, cpu) is kept
+    capturing[0] = True
+    assert ws.get_tree(4500, cpu) is kept  # zeroed before the capture
+    assert ws.get_tree(5001, cpu).numel() == 5001
+    capturing[0] = False
+    assert ws.get_tree(5000, cpu) is kept
+
+
 def test_caches_need_cuda_tensors():
     from warpforth_b200 import KVCache
 

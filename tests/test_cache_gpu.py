@@ -711,6 +711,31 @@ def test_a_captured_step_outlives_its_workspace(wf, n):
     assert ws.get_tree(1, q.device).numel() > before.numel()
 
 
+@pytest.mark.parametrize("n", [1, 16, 40])
+def test_a_workspace_first_used_in_a_capture(wf, n):
+    """Calls outside it, before the graph's first replay and between two, join their parts by
+    counters of their own; so does a second graph that is replayed first."""
+    d, ws, length = 64, wf.DecodeWorkspace(), 6000
+    cache = make_cache(wf, "e4m3", 1, 1, length + n, d, 27)
+    q = torch.randn(1, 1, n, d, generator=torch.Generator().manual_seed(27)).bfloat16().cuda()
+    lens = ints([length])
+    want = wf.tree_decode(q, cache, lens)
+    outs, graphs = [torch.zeros_like(q) for _ in range(2)], []
+    torch.cuda.synchronize()
+    for out in outs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            wf.tree_decode(q, cache, lens, out=out, workspace=ws)
+            wf.tree_decode(q, cache, lens, out=out, workspace=ws)
+    for _ in range(2):
+        for graph, out in reversed(list(zip(graphs, outs))):
+            got = torch.zeros_like(q)
+            wf.tree_decode(q, cache, lens, out=got, workspace=ws)
+            graph.replay()
+            assert torch.equal(got, want) and torch.equal(out, want)
+            out.zero_()
+
+
 def test_calls_on_two_streams_at_once(wf):
     d, n, length = 128, 8, 3000
     caches = [make_cache(wf, "e4m3", 1, 2, length + n, d, 19 + i) for i in range(2)]

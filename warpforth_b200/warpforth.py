@@ -184,6 +184,14 @@ def attention_multicast_ptr(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o
         1 if causal else 0, _stream_handle(q.device)))
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the device's current stream is being captured into a graph."""
+    if device.type != "cuda":
+        return False
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class DecodeWorkspace:
     """Caller-owned scratch for ``decode`` and ``tree_decode`` (grown on demand, reused across
     calls; calls that share one must be ordered on one stream)."""
@@ -194,13 +202,17 @@ class DecodeWorkspace:
 
     def get_tree(self, nbytes: int, device: torch.device) -> torch.Tensor:
         """``tree_decode``'s own scratch: it begins with counters that only its calls may write.
-        An outgrown buffer stays, for the captured graphs that use it."""
+        An outgrown buffer stays, for the captured graphs that use it (sizes go by the kernel, not
+        by lengths: a few dozen MB at most, and few of them).  One that a capture would have to make
+        is not kept: its counters are zeroed when the graph runs, and the graph alone uses it."""
         buffers = self.tree_buffers.get(device)
         if buffers is None:
             buffers = self.tree_buffers[device] = []
         if not buffers or buffers[-1].numel() < nbytes:
             buffer = torch.empty(nbytes, dtype=torch.uint8, device=device)
             buffer[:_lib.TREE_DECODE_ZEROED].zero_()
+            if _capturing(device):
+                return buffer
             buffers.append(buffer)
         return buffers[-1]
 
