@@ -496,6 +496,26 @@ def test_values_of_very_different_sizes(wf, fmt):
     check(out, ref, tol)
 
 
+@pytest.mark.parametrize("fmt,dtype", [k for k in KINDS if k[0] not in TYPES])
+@pytest.mark.parametrize("g,n", [(1, 2), (2, 4), (4, 4), (4, 8), (5, 8), (3, 64)])
+@pytest.mark.parametrize("power", [30, 90])
+def test_values_of_unseen_nodes_may_be_huge(wf, fmt, dtype, g, n, power):
+    """Node 1's values are 2^power times the others'; those who do not see it keep their bits."""
+    lens, d, h = [0, 3, 50, 300], 64, 2
+    b = len(lens)
+    cache = wf.KVCache(b, h, 300 + n, d, fmt=fmt)
+    gen = torch.Generator().manual_seed(n)
+    x = torch.randn(2, b, h, 300 + n, d, generator=gen)
+    for i in range(b):
+        x[1, i, :, lens[i] + 1] *= 2.0 ** power
+    wf.cache_write(cache, x[0].cuda(), x[1].cuda(), ints([0] * b))
+    q = torch.randn(b, g * h, n, d, generator=gen).to(TYPES[dtype])
+    words = wf.tree_words([-1, 0, 0, 1, 2, 0, 3, 4][:n] + [i // 2 for i in range(8, n)])
+    out = wf.tree_decode(q.cuda(), cache, ints(lens), tree=words.cuda())
+    ref, tol = attend(fmt, cache, q, lens, [words.tolist()] * b, [n] * b)
+    check(out, ref, tol)
+
+
 def test_strided_queries_outputs_and_caches(wf):
     b, h, d, n = 3, 4, 128, 5
     big = make_cache(wf, "int4", 2 * b, h, 99, d, 13)

@@ -18,8 +18,8 @@
 //  * f32 rows: tf32 products of two-term splits (hi hi, hi lo, lo hi), and
 //    with f32 queries over quantised rows Q and P as two f16 terms: ~2^-21.
 // Queries are scaled by a power of two into f16's upper range, weights are
-// taken as p <= 2^4 times the row's scale over the running largest scale, also
-// in f16's range; sums, maxima and all other arithmetic are f32.
+// taken as p <= 2^4 times the row's scale over the running largest one that the
+// query sees, also in f16's range; sums, maxima and all other arithmetic are f32.
 //
 // Softmax is online with a lazy maximum: weights are 2^(s - m) for a reference
 // m that is raised (and the sums rescaled) only when a score passes m + 4, so
@@ -437,7 +437,15 @@ struct Warp {
   float qf[C::kNT][2], qsum[C::kNT][2];  // score = product * qf; sum of q (int4)
   uint64_t word[C::kNT][2];
   float m[C::kNT][2], l[C::kNT][2], om[C::kNT][2];
-  float vinv;  // f16 weights carry scale * vinv
+  // f16 weights carry scale * vinv.  Among a tree's nodes it is each query's own, so
+  // that a scale that it does not see leaves its weights their bits; only tails
+  // need those, so they lie in shared memory, as what to add to the bits of vinv.
+  float vinv;
+  int *own;  // of the warp's 8 kNT queries
+
+  __device__ __forceinline__ float own_vinv(int nt, int i) const {
+    return __int_as_float(__float_as_int(vinv) + own[8 * nt + 2 * (threadIdx.x & 3) + i]);
+  }
 
   // The values of one query row that this lane multiplies, step by step.  Any
   // order along a row will do as long as K's fragments have the same.
@@ -574,6 +582,7 @@ struct Warp {
         for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
     }
     vinv = __uint_as_float(253u << 23);  // 2^126
+    if (C::kScaled && g < 2 * C::kNT) own[4 * g + t] = 0;
   }
 
   // c = K Q^T of the 16 keys at k.
@@ -862,11 +871,56 @@ struct Warp {
     }
   }
 
+  // 2^7 <= top * vinv < 2^8: weights of 2^4 times scales up to 2^11 stay below
+  // 2^16, and a weight has all its 11 bits down to 2^-21.
+  static __device__ __forceinline__ float vinv_of(float top) {
+    const int f = min(max(261 - (int)(__float_as_uint(top) >> 23), 1), 253);
+    return __uint_as_float((uint32_t)f << 23);
+  }
+
+  // A tail's weights: each query's vinv follows the scales that it sees, and what
+  // it does not see has weight 0 whatever its scale.
+  __device__ __forceinline__ void tail_weights(const float (&d)[C::kKT][C::kNT][4],
+                                               const float (&vs)[C::kKT][2],
+                                               float (&pv)[C::kKT][C::kNT][4]) {
+#pragma unroll
+    for (int nt = 0; nt < C::kNT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mine = own_vinv(nt, i), top = 0.f;
+#pragma unroll
+        for (int j = 0; j < C::kKT; ++j)
+#pragma unroll
+          for (int e = i; e < 4; e += 2)
+            if (d[j][nt][e] != -INFINITY) top = fmaxf(top, vs[j][e >> 1]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const bool change = top * mine > 2048.f;  // the same for all that hold the query
+        if (__any_sync(0xffffffffu, change)) {
+          const float now = change ? vinv_of(top) : mine, ratio = now / mine;
+          mine = now;
+#pragma unroll
+          for (int mt = 0; mt < C::kMt; ++mt) o[nt][mt][i] *= ratio, o[nt][mt][2 + i] *= ratio;
+          if ((threadIdx.x & 31) < 4)
+            own[8 * nt + 2 * threadIdx.x % 8 + i] = __float_as_int(now) - __float_as_int(vinv);
+          __syncwarp();
+        }
+#pragma unroll
+        for (int j = 0; j < C::kKT; ++j)
+#pragma unroll
+          for (int e = i; e < 4; e += 2)
+            pv[j][nt][e] = d[j][nt][e] == -INFINITY
+                               ? 0.f
+                               : ptx::ex2_approx(d[j][nt][e]) * (vs[j][e >> 1] * mine);
+      }
+  }
+
   // Attends to the 16 kKT keys of rows tr.. of the stage `st`, key0 their
-  // position.  tail: some of them are nodes of the tree, or no keys.
+  // position.  kTail: some of them are nodes of the tree, or no keys.
+  template <bool kTail>
   __device__ __forceinline__ void group(uint32_t st, int tr, int key0, const Seq &seq) {
     const int lane = threadIdx.x & 31, g = lane >> 2;
-    const bool tail = key0 + 16 * C::kKT > seq.len;
     const uint32_t k = st + tr * C::kRowBytes;  // rows 16 apart have the same swizzle
     const uint32_t scales = st + 2 * C::kKBytes + 4 * (tr + g);
     float c[C::kKT][C::kNT][4], vs[C::kKT][2], vm[C::kKT][2];
@@ -912,7 +966,7 @@ struct Warp {
           d[j][nt][e] = fmaf(c[j][nt][e], qf[nt][e & 1], -m[nt][e & 1]);
       if constexpr (C::kScaled) vtop = fmaxf(vtop, fmaxf(vs[j][0], vs[j][1]));
     }
-    if (tail) {
+    if constexpr (kTail) {
 #pragma unroll
       for (int j = 0; j < C::kKT; ++j)
 #pragma unroll
@@ -932,19 +986,16 @@ struct Warp {
       for (int nt = 0; nt < C::kNT; ++nt)
         high = fmaxf(high, fmaxf(ptx::fmax3(d[j][nt][0], d[j][nt][1], d[j][nt][2]), d[j][nt][3]));
     bool raise = high > 4.f;
-    if constexpr (C::kScaled) raise = raise || vtop * vinv > 2048.f;
+    if constexpr (C::kScaled) raise = raise || (!kTail && vtop * vinv > 2048.f);
     if (__any_sync(0xffffffffu, raise)) {
       float ratio = 1.f;
-      if constexpr (C::kScaled) {
+      if constexpr (C::kScaled && !kTail) {
         float top = vtop;
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
         if (top * vinv > 2048.f) {  // the same in the whole warp
-          // 2^7 <= top * vinv < 2^8: weights of 2^4 times scales up to 2^11
-          // stay below 2^16, and a weight has all its 11 bits down to 2^-21
-          const int f = min(max(261 - (int)(__float_as_uint(top) >> 23), 1), 253);
-          const float now = __uint_as_float((uint32_t)f << 23);
+          const float now = vinv_of(top);
           ratio = now / vinv;
           vinv = now;
         }
@@ -993,14 +1044,15 @@ struct Warp {
           pv[j][nt][e] = C::kScaled ? x * w[e >> 1] : x;
           if constexpr (C::kFmt == WFATTN_CACHE_INT4) {
             float y = x * vm[j][e >> 1];
-            if (tail && d[j][nt][e] == -INFINITY) y = 0.f;  // a scale may be NaN
+            if (kTail && d[j][nt][e] == -INFINITY) y = 0.f;  // a scale may be NaN
             om[nt][e & 1] += y;
           }
-          if (C::kScaled && tail && d[j][nt][e] == -INFINITY) pv[j][nt][e] = 0.f;
         }
-      operands(pv[j], pr[j]);
     }
-    if (!tail) {
+    if constexpr (C::kScaled && kTail) tail_weights(d, vs, pv);
+#pragma unroll
+    for (int j = 0; j < C::kKT; ++j) operands(pv[j], pr[j]);
+    if constexpr (!kTail) {
 #pragma unroll
       for (int j = 0; j < C::kKT; ++j)
         values<false>(k + C::kKBytes + 16 * j * C::kRowBytes, pr[j]);
@@ -1169,6 +1221,7 @@ template <class C>
 __global__ void __launch_bounds__(kThreads, C::kCtas) 
     tree_decode_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int own[kWarps][8 * C::kNT];  // of Warp
   float *stats = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
   const uint32_t ring = ptx::smem_u32(smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1276,6 +1329,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
 #pragma unroll 1
   while (i < units) {  // a segment, or the part of it in this share
     Warp<C> w;
+    w.own = own[warp];
     w.load_q(p, cur.b, cur.h, cur.tile * C::kRows + rw * 8 * C::kNT);
     bool done;
 #pragma unroll 1
@@ -1292,7 +1346,10 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
       for (int j = 0; j < C::kGroups; ++j) {
         const int tr = 16 * C::kKT * (kw + C::kKW * j);
         if (tr >= cur.s.total - key0) break;
-        w.group(ring + st, tr, key0 + tr, cur.s);
+        if (key0 + tr + 16 * C::kKT > cur.s.len)
+          w.template group<true>(ring + st, tr, key0 + tr, cur.s);
+        else
+          w.template group<false>(ring + st, tr, key0 + tr, cur.s);
       }
       done = cur.u + 1 == cur.s.units;
       if (done || i + 1 == units) break;
@@ -1303,7 +1360,6 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
 
     const bool whole = done && headed;
     const int g = lane >> 2, t = lane & 3;
-    const float back = C::kScaled ? 1.f / w.vinv : 1.f;
 #pragma unroll
     for (int nt = 0; nt < C::kNT; ++nt)
 #pragma unroll
@@ -1315,6 +1371,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
             w.om[nt][e] += __shfl_xor_sync(0xffffffffu, w.om[nt][e], x);
         }
         if constexpr (C::kScaled) {
+          const float back = 1.f / w.own_vinv(nt, e);
 #pragma unroll
           for (int mt = 0; mt < C::kMt; ++mt) {
             w.o[nt][mt][e] = w.o[nt][mt][e] * back + w.om[nt][e];

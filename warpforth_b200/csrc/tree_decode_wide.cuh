@@ -154,6 +154,29 @@ __device__ __forceinline__ float swap_halves(float x, float *at, const float *ot
   return *other;
 }
 
+// Keys of a unit that a query with this word does not see; key k is node k - at of
+// n: bits of the word, or before the tree.
+__device__ __forceinline__ uint64_t hidden_keys(int at, int n, uint64_t word) {  // at <= 63
+  const uint64_t nodes = n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
+  const uint64_t seen = word & nodes;
+  return at >= 0 ? ~(at > 0 ? seen << at | ((uint64_t(1) << at) - 1) : seen)
+                 : ~(at > -64 ? seen >> -at : 0);
+}
+
+// The largest of a thread's scales that its query sees: one that it does not see
+// has to leave its weights their bits.  Not inlined: tails alone come here, and
+// the rest would be short of registers.
+template <class C>
+__device__ __noinline__ float seen_top(int at, int n, int half, uint64_t word,
+                                       const float *v_scale) {
+  const uint64_t hidden = hidden_keys(at, n, word) >> C::kMine * half;
+  float top = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < C::kMine; ++k)
+    if (!(hidden >> k & 1)) top = fmaxf(top, v_scale[k]);
+  return top;
+}
+
 // A thread's keys of its row of S, C::kMine * half and on, to weights in tensor
 // memory; sp is the row's.  Maximum, sum and (int4) the sum of weights times
 // minima go on in m, which both halves know, and l and om, which are this half's.
@@ -168,6 +191,12 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
                                       float vtop, bool first, float &m, float &l, float &om,
                                       float &vinv, Swap swap, Wait wait_o) {
   constexpr int kMine = C::kMine;
+  if constexpr (kTail && C::kScaled) {
+    if (C::kHalves == 2 || __any_sync(0xffffffffu, vtop * vinv > 2048.f)) {
+      vtop = seen_top<C>(cur.s.len - key0, cur.s.n, half, word, v_scale);
+      if constexpr (C::kHalves == 2) vtop = fmaxf(vtop, swap(vtop));
+    }
+  }
   uint32_t s[kMine];
   if constexpr (kMine == 64)
     ptx::tmem_ld_32x32b_x64(sp, s);
@@ -200,12 +229,7 @@ __device__ __forceinline__ void weigh(const Params &p, const Cursor<C::kKeys> &c
   uint64_t hidden = 0;  // keys of the unit this row does not see
   std::conditional_t<kMine == 64, uint64_t, uint32_t> mine = 0;  // of this thread's
   if constexpr (kTail) {
-    // key k is node k - at: bits of the row's word, or before the tree
-    const int at = cur.s.len - key0;  // at most 63
-    const uint64_t nodes = cur.s.n >= 64 ? ~uint64_t(0) : (uint64_t(1) << cur.s.n) - 1;
-    const uint64_t seen = word & nodes;
-    hidden = at >= 0 ? ~(at > 0 ? seen << at | ((uint64_t(1) << at) - 1) : seen)
-                     : ~(at > -64 ? seen >> -at : 0);
+    hidden = hidden_keys(cur.s.len - key0, cur.s.n, word);
     mine = kMine == 64 ? hidden : hidden >> 32 * half;
 #pragma unroll
     for (int k = 0; k < kMine; ++k)
