@@ -516,6 +516,21 @@ def test_values_of_unseen_nodes_may_be_huge(wf, fmt, dtype, g, n, power):
     check(out, ref, tol)
 
 
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("g,n", [(1, 4), (3, 4), (5, 8)])
+@pytest.mark.parametrize("scale", [None, 1e-3, 1e-12, 1e-38])
+def test_zero_queries_and_small_scales(wf, fmt, dtype, g, n, scale):
+    """Scores next to 0: a node's output is the mean of what it sees, and of nothing else."""
+    lens, d, h = [0, 5, 130], 64, 1
+    cache = make_cache(wf, fmt, 3, h, 130 + n, d, 28)
+    q = torch.randn(3, g * h, n, d, generator=torch.Generator().manual_seed(28)).to(TYPES[dtype])
+    q[:, :, ::2] = 0
+    words = wf.tree_words([i - 2 if i > 1 else -1 for i in range(n)])
+    out = wf.tree_decode(q.cuda(), cache, ints(lens), tree=words.cuda(), scale=scale)
+    ref, tol = attend(fmt, cache, q, lens, [words.tolist()] * 3, [n] * 3, scale)
+    check(out, ref, tol)
+
+
 def test_strided_queries_outputs_and_caches(wf):
     b, h, d, n = 3, 4, 128, 5
     big = make_cache(wf, "int4", 2 * b, h, 99, d, 13)

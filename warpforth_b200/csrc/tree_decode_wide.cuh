@@ -694,7 +694,9 @@ __global__ void __launch_bounds__(C::kWideThreads, C::kCtas)
           if constexpr (C::kHalves == 2) e = max(e, __float_as_int(swap(__int_as_float(e))));
           const int f = min(max(268 - e, 1), 253);  // 2^14 <= top * mul < 2^15
           const float mul = __uint_as_float((uint32_t)f << 23);
-          qf = p.scale_log2 * __uint_as_float((uint32_t)(254 - f) << 23);
+          // not 0, as a hidden score of -inf times that is NaN
+          qf = fmaxf(p.scale_log2 * __uint_as_float((uint32_t)(254 - f) << 23),
+                     __uint_as_float(1));
 #pragma unroll
           for (int c = 0; c < C::kDims / 8; ++c) {
             float x[8];
