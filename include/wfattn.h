@@ -256,15 +256,15 @@ WFATTN_API wfattn_status_t wfattn_decode_noalloc(int64_t batch, int64_t heads, i
  *
  * Row formats (head_dim = D):
  *  WFATTN_CACHE_F32, WFATTN_CACHE_BF16: D values; no scales.
- *  WFATTN_CACHE_E4M3: D e4m3 codes, and one f32 scale a row in k_scale /
- *    v_scale.  A value is code * scale.  wfattn_cache_write takes as scale the
- *    smallest power of two s >= 2^-126 with max|x| <= 448 s, so x / s is exact
- *    and each value is rounded once (to nearest even).
+ *  WFATTN_CACHE_E4M3: D e4m3 codes, and one f32 scale a row (of either sign)
+ *    in k_scale / v_scale.  A value is code * scale.  wfattn_cache_write takes
+ *    as scale the smallest power of two s >= 2^-126 with max|x| <= 448 s, so
+ *    x / s is exact and each value is rounded once (to nearest even).
  *  WFATTN_CACHE_INT4: D 4-bit codes u (value 2i in the low half of byte i), and
- *    two bf16 numbers (s, m) a row in k_scale / v_scale.  A value is m + s u.
- *    wfattn_cache_write takes as m the largest bf16 <= min(x), as s the
- *    smallest bf16 >= (max(x) - m) / 15 (in f32), and as u (x - m) / s in f32
- *    rounded to nearest even, in 0..15 (0 where s = 0).
+ *    two bf16 numbers (s, m), of either sign, a row in k_scale / v_scale.  A
+ *    value is m + s u.  wfattn_cache_write takes as m the largest bf16 <=
+ *    min(x), as s the smallest bf16 >= (max(x) - m) / 15 (in f32), and as u
+ *    (x - m) / s in f32 rounded to nearest even, in 0..15 (0 where s = 0).
  * A row that holds a NaN or an infinity (or, for INT4, spans more than f32
  * does) is stored by the last two with a NaN scale and codes 0: it reads back
  * as NaN in every value.

@@ -531,6 +531,28 @@ def test_zero_queries_and_small_scales(wf, fmt, dtype, g, n, scale):
     check(out, ref, tol)
 
 
+@pytest.mark.parametrize("fmt,dtype", [k for k in KINDS if k[0] not in TYPES])
+@pytest.mark.parametrize("g,n", [(1, 1), (2, 4), (4, 4), (4, 8), (5, 8)])
+def test_scales_of_either_sign(wf, fmt, dtype, g, n):
+    """A program's own cache may hold them: a value is code * scale, or minimum + scale * code."""
+    lens, d, h = [0, 7, 300], 64, 2
+    cache = make_cache(wf, fmt, 3, h, 300 + n, d, 29)
+    gen = torch.Generator().manual_seed(29)
+    for s in (cache.k_scale, cache.v_scale):
+        sign = (1 - 2 * torch.randint(0, 2, s.shape[:3], generator=gen)).cuda()
+        sign[1] = -1
+        (s if fmt == "e4m3" else s[..., 0]).mul_(sign)
+    q = torch.randn(3, g * h, n, d, generator=gen).to(TYPES[dtype])
+    words = wf.tree_words(random_trees(1, n, 29)[0])
+    out = wf.tree_decode(q.cuda(), cache, ints(lens), tree=words.cuda())
+    ref, tol = attend(fmt, cache, q, lens, [words.tolist()] * 3, [n] * 3)
+    check(out, ref, tol)
+    for t, codes, scale in zip(wf.cache_read(cache, ints([0] * 3), 300, dtype=torch.float32),
+                               (cache.k, cache.v), (cache.k_scale, cache.v_scale)):
+        want = values(fmt, codes.cpu(), scale.cpu())[:, :, :300].astype(np.float32)
+        assert np.array_equal(t.cpu().numpy(), want)
+
+
 def test_strided_queries_outputs_and_caches(wf):
     b, h, d, n = 3, 4, 128, 5
     big = make_cache(wf, "int4", 2 * b, h, 99, d, 13)

@@ -892,7 +892,7 @@ struct Warp {
         for (int j = 0; j < C::kKT; ++j)
 #pragma unroll
           for (int e = i; e < 4; e += 2)
-            if (d[j][nt][e] != -INFINITY) top = fmaxf(top, vs[j][e >> 1]);
+            if (d[j][nt][e] != -INFINITY) top = fmaxf(top, fabsf(vs[j][e >> 1]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -964,7 +964,7 @@ struct Warp {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           d[j][nt][e] = fmaf(c[j][nt][e], qf[nt][e & 1], -m[nt][e & 1]);
-      if constexpr (C::kScaled) vtop = fmaxf(vtop, fmaxf(vs[j][0], vs[j][1]));
+      if constexpr (C::kScaled) vtop = fmaxf(vtop, fmaxf(fabsf(vs[j][0]), fabsf(vs[j][1])));
     }
     if constexpr (kTail) {
 #pragma unroll

@@ -173,7 +173,7 @@ __device__ __noinline__ float seen_top(int at, int n, int half, uint64_t word,
   float top = 0.f;
 #pragma unroll 4
   for (int k = 0; k < C::kMine; ++k)
-    if (!(hidden >> k & 1)) top = fmaxf(top, v_scale[k]);
+    if (!(hidden >> k & 1)) top = fmaxf(top, fabsf(v_scale[k]));
   return top;
 }
 
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(C::kWideThreads, C::kCtas)
     alignas(16) float k_mid[2][C::kKeys];
     alignas(16) float v_scale[2][C::kKeys];
     alignas(16) float v_mid[2][C::kKeys];
-    float v_top[2][2];  // the largest scale of V's rows 0-31 and 32-63
+    float v_top[2][2];  // the largest magnitude of a scale of V's rows 0-31 and 32-63
     float swap[2][C::kHalves == 2 ? C::kWeighers : 1];
   } sh;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -615,8 +615,8 @@ __global__ void __launch_bounds__(C::kWideThreads, C::kCtas)
           sh.k_mid[buf][t] = fmaf(8.f, ks, ptx::bf16_hi(held_k));
           sh.v_mid[buf][t] = fmaf(8.f, vs, ptx::bf16_hi(held_v));
         }
-        // scales are not negative: their bits order like them; NaN does not count
-        uint32_t top = C::kFmt == WFATTN_CACHE_E4M3 ? held_v : held_v << 16;
+        // the bits of magnitudes order like them; NaN does not count
+        uint32_t top = (C::kFmt == WFATTN_CACHE_E4M3 ? held_v : held_v << 16) & 0x7fffffffu;
         top = __reduce_max_sync(0xffffffffu, top > 0x7f800000u ? 0u : top);
         if (t % 32 == 0) sh.v_top[buf][t / 32] = __uint_as_float(top);
       }
