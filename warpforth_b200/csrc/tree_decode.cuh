@@ -1165,13 +1165,13 @@ __device__ __forceinline__ void store_sums(const Params &p, int64_t b, int64_t h
 }
 
 // Counts this CTA's part of a segment, which its threads have written, as
-// arrived, and joins the parts if it is the last: thread groups take a float4
-// column of a row each and every kth part, and meet in `room` (4 KB of shared
-// memory).  Not inlined: a CTA comes here twice at most, and the loads in flight
-// would cost the main loop its registers.
+// arrived, and joins the parts if it is the last: of one or two query rows, a
+// thread takes a float4 column and every groups-th part, and they meet in `room`
+// (3 KB of shared memory).  Not inlined: a CTA comes here twice at most, and the
+// loads in flight would cost the main loop its registers.
 template <class C>
-__device__ __noinline__ void join(const Params &p, int b, int h, int tile, int n, int first,
-                                  int last, int parts, int64_t all, uint8_t *room) {
+__device__ __noinline__ void join(const Params &p, int b, int h, int n, int first, int last,
+                                  int parts, int64_t all, uint8_t *room) {
   __shared__ int is_last;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -1182,39 +1182,31 @@ __device__ __noinline__ void join(const Params &p, int b, int h, int tile, int n
   __syncthreads();
   if (!is_last) return;
   constexpr int kCols = C::D / 4;
-  const int items = min(C::kRows, p.R - tile * C::kRows) * kCols;
-  const int groups = items >= kThreads ? 1 : kThreads / items;
-  const int group = items >= kThreads ? 0 : threadIdx.x / items;
-#pragma unroll 1
-  for (int x = items >= kThreads ? threadIdx.x : threadIdx.x % items; x < items; x += kThreads) {
-    const int r = x / kCols, dd = x % kCols * 4;
-    float m = -FLT_MAX, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (group < groups) add_parts<C>(p, r, dd, first, last, group, groups, all, m, l, o);
-    if (groups > 1) {  // one pass: items < kThreads
-      float4 *sums = reinterpret_cast<float4 *>(room);
-      float2 *mls = reinterpret_cast<float2 *>(room + kThreads * sizeof(float4));
-      if (group < groups) {
-        sums[threadIdx.x] = o;
-        mls[threadIdx.x] = make_float2(m, l);
-      }
-      __syncthreads();
-      if (group > 0) return;
-      for (int y = 1; y < groups; ++y) m = fmaxf(m, mls[y * items + x].x);
-      const float f = ptx::ex2_approx(mls[x].x - m);
-      l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-      for (int y = 1; y < groups; ++y) {
-        const float2 s = mls[y * items + x];
-        const float4 z = sums[y * items + x];
-        const float w = ptx::ex2_approx(s.x - m);
-        l = fmaf(s.y, w, l);
-        o.x = fmaf(z.x, w, o.x), o.y = fmaf(z.y, w, o.y);
-        o.z = fmaf(z.z, w, o.z), o.w = fmaf(z.w, w, o.w);
-      }
-    }
-    if (group > 0) return;
-    store_sums<C>(p, b, h, tile * C::kRows + r, n, dd, l, o);
+  static_assert(kThreads % (2 * kCols) == 0 && kThreads > 2 * kCols, "whole groups, two at least");
+  const int items = p.R * kCols, groups = kThreads / items;
+  const int group = threadIdx.x / items, x = threadIdx.x % items;
+  const int r = x / kCols, dd = x % kCols * 4;
+  float m = -FLT_MAX, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  add_parts<C>(p, r, dd, first, last, group, groups, all, m, l, o);
+  float4 *sums = reinterpret_cast<float4 *>(room);
+  float2 *mls = reinterpret_cast<float2 *>(room + kThreads * sizeof(float4));
+  sums[threadIdx.x] = o;
+  mls[threadIdx.x] = make_float2(m, l);
+  __syncthreads();
+  if (group > 0) return;
+  for (int y = 1; y < groups; ++y) m = fmaxf(m, mls[y * items + x].x);
+  const float f = ptx::ex2_approx(mls[x].x - m);
+  l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+  for (int y = 1; y < groups; ++y) {
+    const float2 s = mls[y * items + x];
+    const float4 z = sums[y * items + x];
+    const float w = ptx::ex2_approx(s.x - m);
+    l = fmaf(s.y, w, l);
+    o.x = fmaf(z.x, w, o.x), o.y = fmaf(z.y, w, o.y);
+    o.z = fmaf(z.z, w, o.z), o.w = fmaf(z.w, w, o.w);
   }
+  store_sums<C>(p, b, h, r, n, dd, l, o);
 }
 
 template <class C>
@@ -1436,16 +1428,20 @@ __global__ void __launch_bounds__(kThreads, C::kCtas)
         if (dd == 0) *reinterpret_cast<float2 *>(part_ml + 2 * r) = make_float2(m, l);
       }
     }
-    if (p.apart) {
+    constexpr bool kJoins = C::kRows == 8;  // the configuration of one or two query rows
+    if (!kJoins || p.apart) {
       if (!done && headed && threadIdx.x == 0)
         p.split[blockIdx.x] = split_of(p, cur, begin + i - cur.u, all);
     } else if (!whole) {
-      // CTAs without units are passed over; there are none, or no CTA has two
-      const int64_t s0 = begin + i - cur.u;
-      const int first_cta = headed ? (int)blockIdx.x : (int)(((s0 + 1) * p.ctas - 1) / all);
-      const int last_cta = split_of(p, cur, s0, all).last;
-      const int parts = min(last_cta - first_cta + 1, cur.s.units);
-      join<C>(p, cur.b, cur.h, cur.tile, cur.s.n, first_cta, last_cta, parts, all, smem + st);
+      if constexpr (kJoins) {
+        // CTAs without units are passed over; there are none, or no CTA has two
+        const int64_t s0 = begin + i - cur.u;
+        const int first_cta =
+            headed ? (int)blockIdx.x : (int)(((s0 + 1) * p.ctas - 1) / all);
+        const int last_cta = split_of(p, cur, s0, all).last;
+        const int parts = min(last_cta - first_cta + 1, cur.s.units);
+        join<C>(p, cur.b, cur.h, cur.s.n, first_cta, last_cta, parts, all, smem + st);
+      }
     }
     // the stage may be refilled once all have read it (with common loads the
     // next unit's barrier says so)
@@ -1600,7 +1596,8 @@ cudaError_t launch(Params p, void *workspace, const DeviceInfo &dev, cudaStream_
       reinterpret_cast<const void *>(tree_decode_kernel<C>), C::kSmem, dev.device);
   if (err != cudaSuccess) return err;
   tree_decode_kernel<C><<<p.ctas, kThreads, C::kSmem, stream>>>(p);
-  return p.apart ? launch_join<C>(p, stream) : cudaGetLastError();
+  if (C::kRows == 8 && !p.apart) return cudaGetLastError();
+  return launch_join<C>(p, stream);
 }
 
 }  // namespace tree
