@@ -359,6 +359,8 @@ WFATTN_API wfattn_status_t wfattn_cache_keep(const wfattn_cache_t *cache, const 
  * counts: nodes of each sequence, 0..nodes (NULL: all); the rest is padding.
  *         Padding nodes, and nodes that see nothing, give zeros.
  * Rows that a node does not see do not reach its output, whatever they hold.
+ * One that it sees with a value (or scale) that is not finite makes its output
+ * not finite, NaN where the formula may give an infinity.
  * Over E4M3 and INT4 caches errors are relative to the largest value that the
  * node sees: a weight times its row's scale is off by 2^-11 of itself (F32
  * queries: 2^-22) or 2^-32 of the largest scale seen, whichever is more.

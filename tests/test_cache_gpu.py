@@ -553,6 +553,21 @@ def test_scales_of_either_sign(wf, fmt, dtype, g, n):
         assert np.array_equal(t.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("fmt,dtype", [k for k in KINDS if k[0] not in TYPES])
+@pytest.mark.parametrize("g,n", [(1, 2), (3, 4), (5, 8)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_keys_that_are_not_finite_are_not_passed_over(wf, fmt, dtype, g, n, bad):
+    """A scale of K that is not finite, in a row before the tree (head 0) and in node 0 (head 1)."""
+    lens, d, h = [4, 130], 64, 2
+    cache = make_cache(wf, fmt, 2, h, 130 + n, d, 38)
+    scale = cache.k_scale if fmt == "e4m3" else cache.k_scale[..., 0]
+    for i in range(2):
+        scale[i, 0, 2] = scale[i, 1, lens[i]] = bad
+    q = torch.randn(2, g * h, n, d, generator=torch.Generator().manual_seed(38)).to(TYPES[dtype])
+    out = wf.tree_decode(q.cuda(), cache, ints(lens))
+    assert torch.isnan(out).all()
+
+
 def test_strided_queries_outputs_and_caches(wf):
     b, h, d, n = 3, 4, 128, 5
     big = make_cache(wf, "int4", 2 * b, h, 99, d, 13)

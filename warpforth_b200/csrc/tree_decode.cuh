@@ -935,21 +935,23 @@ struct Warp {
         for (int i = 0; i < 2; ++i) {
           const uint32_t at = scales + 4 * (16 * j + 8 * i);
           const uint32_t ks = lds32(at), vw = lds32(at + 4 * C::kKeys);
+          // 0, or NaN where the scale is not finite: a score of -inf would hide the key
           if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
+            const float s = __uint_as_float(ks), odd = s - s;
             vs[j][i] = __uint_as_float(vw);
 #pragma unroll
             for (int nt = 0; nt < C::kNT; ++nt) {
-              c[j][nt][2 * i] *= __uint_as_float(ks);
-              c[j][nt][2 * i + 1] *= __uint_as_float(ks);
+              c[j][nt][2 * i] = fmaf(c[j][nt][2 * i], s, odd);
+              c[j][nt][2 * i + 1] = fmaf(c[j][nt][2 * i + 1], s, odd);
             }
           } else {
-            const float s = ptx::bf16_lo(ks), mid = fmaf(8.f, s, ptx::bf16_hi(ks));
+            const float s = ptx::bf16_lo(ks), mid = fmaf(8.f, s, ptx::bf16_hi(ks)), odd = s - s;
             vs[j][i] = ptx::bf16_lo(vw);
             vm[j][i] = fmaf(8.f, vs[j][i], ptx::bf16_hi(vw));
 #pragma unroll
             for (int nt = 0; nt < C::kNT; ++nt) {
-              c[j][nt][2 * i] = fmaf(c[j][nt][2 * i], s, mid * qsum[nt][0]);
-              c[j][nt][2 * i + 1] = fmaf(c[j][nt][2 * i + 1], s, mid * qsum[nt][1]);
+              c[j][nt][2 * i] = fmaf(c[j][nt][2 * i], s, fmaf(mid, qsum[nt][0], odd));
+              c[j][nt][2 * i + 1] = fmaf(c[j][nt][2 * i + 1], s, fmaf(mid, qsum[nt][1], odd));
             }
           }
         }

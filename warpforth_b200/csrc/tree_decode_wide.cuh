@@ -605,12 +605,14 @@ __global__ void __launch_bounds__(C::kWideThreads, C::kCtas)
                                 int4_f16x2<false>(w[e] >> 8), int4_f16x2<true>(w[e] >> 8)));
           }
         }
+        // K's scale is NaN where it is not finite: a score of -inf would hide the key
         if constexpr (C::kFmt == WFATTN_CACHE_E4M3) {
-          sh.k_scale[buf][t] = __uint_as_float(held_k);
+          const float ks = __uint_as_float(held_k);
+          sh.k_scale[buf][t] = ks + (ks - ks);
           sh.v_scale[buf][t] = __uint_as_float(held_v);
         } else {
           const float ks = ptx::bf16_lo(held_k), vs = ptx::bf16_lo(held_v);
-          sh.k_scale[buf][t] = ks;
+          sh.k_scale[buf][t] = ks + (ks - ks);
           sh.v_scale[buf][t] = vs;
           sh.k_mid[buf][t] = fmaf(8.f, ks, ptx::bf16_hi(held_k));
           sh.v_mid[buf][t] = fmaf(8.f, vs, ptx::bf16_hi(held_v));
