@@ -667,6 +667,169 @@ def test_bad_tensors_are_refused(wf):
             wf.KVCache.wrap(*bad)
 
 
+# ------------------------------------- many query rows a cache head (products on tcgen05)
+
+WIDE = [k for k in KINDS if k[1] == "bf16"]
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_unseen_rows_of_large_trees(wf, fmt, dtype, d):
+    """60 and 132 query rows a head; rows past the end hold NaN, node 2 NaN and infinities, its
+    unit being the first, the middle of one and the last of one."""
+    lens, nodes, n, h = [0, 61, 126, 190], [6, 5, 6, 3], 6, 2
+    b, lmax = len(lens), 200
+    words = wf.tree_words([-1, 0, 0, 1, 2, 0])
+    sees = torch.tensor([w >> 2 & 1 == 1 for w in words.tolist()])
+    for g in (10, 22):
+        cache = make_cache(wf, fmt, b, h, lmax, d, 30)
+        clean = wf.KVCache.wrap(*(None if t is None else t.clone() for t in
+                                  (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+        for t in (cache.k, cache.v):
+            for i in range(b):
+                end, node = lens[i] + nodes[i], lens[i] + 2
+                if fmt in TYPES:
+                    t[i, :, end:] = math.nan
+                    t[i, 0, node, ::7] = math.nan
+                    t[i, 1, node, 1::2] = math.inf
+                elif fmt == "e4m3":
+                    t.view(torch.uint8)[i, :, end:] = 0x7F
+                    t.view(torch.uint8)[i, 1, node, 1::2] = 0xFF
+        for t in (cache.k_scale, cache.v_scale):
+            for i in range(b):
+                if t is not None:
+                    t[i, :, lens[i] + nodes[i]:] = math.nan
+                    t[i, 0, lens[i] + 2] = math.nan
+                    if fmt == "int4":
+                        t[i, 1, lens[i] + 2, 0] = math.inf
+        q = torch.randn(b, g * h, n, d, generator=torch.Generator().manual_seed(30))
+        q = q.to(TYPES[dtype])
+        out = wf.tree_decode(q.cuda(), cache, ints(lens), tree=words.cuda(), nodes=ints(nodes))
+        for i in range(b):
+            live = sees & (torch.arange(n) < nodes[i])
+            assert not torch.isfinite(out[i][:, live].float()).all(-1).any()
+        ref, tol = attend(fmt, clean, q, lens, [words.tolist()] * b, nodes)
+        check(out[:, :, ~sees], ref[:, :, ~sees], tol[:, :, ~sees])
+
+
+@pytest.mark.parametrize("fmt,dtype", WIDE[:2])
+def test_what_is_not_finite_stays_in_its_column(wf, fmt, dtype):
+    """Only V's values at one place of a seen node are not finite: the others are as ever."""
+    d, n, lens = 64, 34, [0, 64, 100]
+    cache = make_cache(wf, fmt, 3, 1, 140, d, 31)
+    clean = wf.KVCache.wrap(*(None if t is None else t.clone() for t in
+                              (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+    for i in range(3):
+        if fmt == "e4m3":
+            cache.v.view(torch.uint8)[i, 0, lens[i] + 3, 5] = 0x7F
+        else:
+            cache.v[i, 0, lens[i] + 3, 5] = math.inf
+    q = torch.randn(3, 1, n, d, generator=torch.Generator().manual_seed(31)).to(TYPES[dtype])
+    words = wf.tree_words(random_trees(1, n, 31)[0])
+    out = wf.tree_decode(q.cuda(), cache, ints(lens), tree=words.cuda())
+    ref, tol = attend(fmt, clean, q, lens, [words.tolist()] * 3, [n] * 3)
+    odd = torch.zeros(n, d, dtype=torch.bool)
+    odd[[i for i, w in enumerate(words.tolist()) if w >> 3 & 1], 5] = True
+    got = out[:, 0].cpu()
+    assert (torch.isnan if fmt == "e4m3" else torch.isposinf)(got[:, odd]).all()
+    check(out[:, 0][:, ~odd], ref[:, 0][:, ~odd], tol[:, 0][:, ~odd])
+
+
+@pytest.mark.parametrize("fmt,dtype", WIDE)
+def test_many_nodes_that_see_nothing_give_zeros(wf, fmt, dtype):
+    cache = make_cache(wf, fmt, 2, 1, 70, 64, 32)
+    q = torch.randn(2, 20, 3, 64, generator=torch.Generator().manual_seed(32)).to(TYPES[dtype])
+    words = torch.tensor([[0, 2, 0], [0, 0, 7]])
+    out = wf.tree_decode(q.cuda(), cache, ints([0, 67]), tree=words.cuda(), nodes=ints([2, 3]))
+    ref, tol = attend(fmt, cache, q, [0, 67], words.tolist(), [2, 3])
+    assert not out[0, :, 0].any() and not out[0, :, 2].any()
+    check(out, ref, tol)
+
+
+@pytest.mark.parametrize("fmt,dtype", WIDE)
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_rising_scores_of_many_rows(wf, fmt, dtype, d):
+    h, g, n, length = 2, 20, 2, 1500
+    cache = wf.KVCache(1, h, length, d, fmt=fmt)
+    ramp = torch.linspace(-1, 1, length)[:, None] + 0.02 * torch.randn(
+        length, d, generator=torch.Generator().manual_seed(33))
+    x = ramp.expand(1, h, length, d).contiguous().cuda()
+    wf.cache_write(cache, x, x.flip(-1), ints([0]))
+    q = (8 * torch.ones(1, h * g, n, d)).to(TYPES[dtype])
+    q[..., 1, :] *= -1
+    q[:, ::3] *= 0.01
+    for scale in (None, 0.5):
+        out = wf.tree_decode(q.cuda(), cache, ints([length - n]), scale=scale)
+        ref, tol = attend(fmt, cache, q, [length - n], [[1, 3]], [n], scale)
+        check(out, ref, tol)
+
+
+@pytest.mark.parametrize("fmt,dtype", WIDE)
+def test_many_rows_over_values_of_very_different_sizes(wf, fmt, dtype):
+    # the largest rows of V have almost no weight, and come last
+    d, length, g = 64, 600, 40
+    rng = np.random.default_rng(34)
+    cache = wf.KVCache(1, 1, length, d, fmt=fmt)
+    k = rng.standard_normal((1, 1, length, d)).astype(np.float32)
+    v = rng.standard_normal((1, 1, length, d)).astype(np.float32)
+    k[..., 300::50, :] = -3.0
+    v[..., 300::50, :] *= 4096
+    wf.cache_write(cache, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), ints([0]))
+    q = torch.linspace(0.5, 1, g).reshape(1, g, 1, 1).expand(1, g, 1, d).to(TYPES[dtype])
+    out = wf.tree_decode(q.cuda(), cache, ints([length - 1]))
+    ref, tol = attend(fmt, cache, q, [length - 1], [[1]], [1])
+    check(out, ref, tol)
+
+
+@pytest.mark.parametrize("fmt,dtype", WIDE)
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_rows_of_strided_queries_outputs_and_caches(wf, fmt, dtype, d):
+    b, n, hq, lens = 3, 7, 12, [0, 90, 33]
+    big = make_cache(wf, fmt, 2 * b, 4, 99, d, 35)
+    part = wf.KVCache.wrap(*(None if t is None else t[1::2, 1:3] for t in
+                             (big.k, big.v, big.k_scale, big.v_scale)))
+    q = torch.randn(b, n, hq, d + 3, generator=torch.Generator().manual_seed(35))
+    q = q.to(TYPES[dtype])[..., 1:1 + d].transpose(1, 2)
+    qc = torch.empty(b, n, hq, d + 3, dtype=q.dtype, device="cuda")[..., 1:1 + d].transpose(1, 2)
+    qc.copy_(q)
+    store = torch.full((b, hq, n, d + 9), 5.0, dtype=q.dtype, device="cuda")
+    out = store[..., 7:7 + d]
+    words = wf.tree_words(random_trees(b, n, 35))
+    assert wf.tree_decode(qc, part, ints(lens), tree=words.cuda(), out=out) is out
+    ref, tol = attend(fmt, part, q, lens, words.tolist(), [n] * b)
+    check(out, ref, tol)
+    assert (store[..., :7] == 5).all() and (store[..., 7 + d:] == 5).all()
+    # the output in the place of the queries, one query head for all of a group
+    wf.tree_decode(qc, part, ints(lens), tree=words.cuda(), out=qc)
+    assert torch.equal(qc, out)
+
+
+@pytest.mark.parametrize("fmt,dtype", WIDE)
+def test_lengths_of_many_rows_are_clamped_and_reported(wf, fmt, dtype):
+    from warpforth_b200 import _lib, warpforth
+
+    cache = make_cache(wf, fmt, 4, 1, 40, 64, 36)
+    q = torch.randn(4, 10, 4, 64, generator=torch.Generator().manual_seed(36)).to(TYPES[dtype])
+    out = wf.tree_decode(q.cuda(), cache, ints([-5, 38, 1000, 10]), nodes=ints([4, 4, 4, 9]))
+    with pytest.raises(_lib.WfattnError, match="length"):
+        warpforth.device_status()
+    ref, tol = attend(fmt, cache, q, [0, 38, 40, 10], [[1, 3, 7, 15]] * 4, [4, 2, 0, 4])
+    check(out, ref, tol)
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("d,g,n", [(64, 1, 2), (128, 4, 12), (64, 8, 61)])
+def test_trees_over_one_long_sequence(wf, fmt, dtype, d, g, n):
+    # one cache head dealt to the whole GPU: 8,000 keys, up to 488 query rows
+    length = 8000
+    cache = make_cache(wf, fmt, 1, 1, length + n, d, 37)
+    q = torch.randn(1, g, n, d, generator=torch.Generator().manual_seed(37)).to(TYPES[dtype])
+    words = wf.tree_words(random_trees(1, n, 37)[0])
+    out = wf.tree_decode(q.cuda(), cache, ints([length]), tree=words.cuda())
+    ref, tol = attend(fmt, cache, q, [length], [words.tolist()], [n])
+    check(out, ref, tol)
+
+
 # ---------------------------------------------------------------------- used together
 
 
