@@ -82,6 +82,22 @@ def test_bad_rows_are_refused(call, bad):
     assert call(_cache(), **bad) == _lib.INVALID_ARG
 
 
+@pytest.mark.parametrize("call", ["write", "read"])
+@pytest.mark.parametrize("starts,counts", [(18, 16), (16, 18), (17, None), (16, 19)])
+def test_positions_off_their_alignment_are_refused(call, starts, counts):
+    lib, rows = _lib.load(), (_cache(), _lib.DTYPE_BF16, 4, 16, None, 16, None, starts, counts)
+    status = lib.wfattn_cache_write(*rows, None) if call == "write" else \
+        lib.wfattn_cache_read(*rows, 0, None)
+    assert status == _lib.INVALID_ARG and b"aligned" in lib.wfattn_last_error()
+
+
+@pytest.mark.parametrize("bad", [{"lens": 1026}, {"path": 18}, {"counts": 2049},
+                                 {"new_lens": 8193}])
+def test_paths_off_their_alignment_are_refused(bad):
+    assert _keep(_cache(), **bad) == _lib.INVALID_ARG
+    assert b"aligned" in _lib.load().wfattn_last_error()
+
+
 def test_reading_into_broadcast_rows_is_refused():
     assert _read(_cache(), strides=(1000, 300, 0)) == _lib.INVALID_ARG
     assert b"broadcast" in _lib.load().wfattn_last_error()

@@ -610,6 +610,8 @@ wfattn_status_t prepare_rows(const wfattn_cache_t *cache, int dtype, int64_t n_r
   a->ks = resolve_strides(k_strides, a->c.H, n_rows, a->c.D);
   a->vs = resolve_strides(v_strides, a->c.H, n_rows, a->c.D);
   if (!strides_ok(a->ks) || !strides_ok(a->vs)) return fail(WFATTN_INVALID_ARG, "negative stride");
+  if (!aligned(starts, 4) || !aligned(counts, 4))
+    return fail(WFATTN_INVALID_ARG, "starts and counts must be aligned to their elements");
   a->starts = starts;
   a->counts = counts;
   return WFATTN_OK;
@@ -669,6 +671,9 @@ wfattn_status_t wfattn_cache_keep(const wfattn_cache_t *cache, const int32_t *le
     return fail(WFATTN_INVALID_ARG, "depth must be in [1, %d] (got %lld)", kMaxTreeNodes,
                 (long long)depth);
   if (path_stride < 0) return fail(WFATTN_INVALID_ARG, "negative stride");
+  if (!aligned(lens, 4) || !aligned(path, 4) || !aligned(counts, 4) || !aligned(new_lens, 4))
+    return fail(WFATTN_INVALID_ARG,
+                "lens, path, counts and new_lens must be aligned to their elements");
   // every head's blocks read these while one writes new_lens
   auto meets = [&](const int32_t *p, int64_t n) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(new_lens);
