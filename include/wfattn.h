@@ -266,8 +266,8 @@ WFATTN_API wfattn_status_t wfattn_decode_noalloc(int64_t batch, int64_t heads, i
  *    min(x), as s the smallest bf16 >= (max(x) - m) / 15 (in f32), and as u
  *    (x - m) / s in f32 rounded to nearest even, in 0..15 (0 where s = 0).
  * A row that holds a NaN or an infinity (or, for INT4, spans more than f32
- * does) is stored by the last two with a NaN scale and codes 0: it reads back
- * as NaN in every value.
+ * does or has a value below the lowest bf16) is stored by the last two with a
+ * NaN scale and codes 0: it reads back as NaN in every value.
  *
  * Row (b, h, t) of K, of V and of their scales is number
  * b * batch_stride + h * head_stride + t of its array; rows do not overlap
@@ -303,7 +303,8 @@ typedef struct wfattn_cache {
  * {batch, head, row}; any alignment of the element).  counts NULL: n_rows for
  * every b.  Other rows are left as they are.  Row positions below 0 or past
  * max_len are not written; a count outside 0..n_rows is clamped (both are
- * recorded, see above).  n_rows 0 does nothing.
+ * recorded, see above).  n_rows 0 does nothing.  k and v share no memory with
+ * the rows that are written.
  */
 WFATTN_API wfattn_status_t wfattn_cache_write(const wfattn_cache_t *cache, int dtype,
                                               int64_t n_rows, const void *k,
@@ -316,7 +317,8 @@ WFATTN_API wfattn_status_t wfattn_cache_write(const wfattn_cache_t *cache, int d
  * of k and v ([batch, heads, n_rows, head_dim] of `dtype`) take the values of
  * rows starts[b] .. starts[b]+counts[b]-1, computed in f32 and rounded once.
  * The other rows of k and v, and those whose position is outside the cache,
- * are left as they are, or set to zero where zero_rest is not 0.
+ * are left as they are, or set to zero where zero_rest is not 0.  k and v share
+ * no memory with one another or with the rows that are read.
  */
 WFATTN_API wfattn_status_t wfattn_cache_read(const wfattn_cache_t *cache, int dtype,
                                              int64_t n_rows, void *k, const int64_t *k_strides,
@@ -359,8 +361,8 @@ WFATTN_API wfattn_status_t wfattn_cache_keep(const wfattn_cache_t *cache, const 
  * counts: nodes of each sequence, 0..nodes (NULL: all); the rest is padding.
  *         Padding nodes, and nodes that see nothing, give zeros.
  * Rows that a node does not see do not reach its output, whatever they hold.
- * One that it sees with a value (or scale) that is not finite makes its output
- * not finite, NaN where the formula may give an infinity.
+ * Where one that it sees has a value or scale that is not finite, the output is
+ * what the formula gives, or NaN.
  * Over E4M3 and INT4 caches errors are relative to the largest value that the
  * node sees: a weight times its row's scale is off by 2^-11 of itself (F32
  * queries: 2^-22) or 2^-32 of the largest scale seen, whichever is more.

@@ -177,7 +177,7 @@ def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, starts: torch.
 
     k, v: [batch, heads, n, head_dim] f32 or bf16, any batch/head/row strides; the first
     ``counts[b]`` rows of sequence b are taken (all n without ``counts``).  The other rows of the
-    cache stay as they are.
+    cache stay as they are.  k and v share no memory with the rows that are written.
     """
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise ValueError("k must be a [batch, heads, n, head_dim] tensor")
@@ -197,7 +197,8 @@ def cache_read(cache: KVCache, starts: torch.Tensor, rows: int, *,
 
     Returns (k, v), each [batch, heads, rows, head_dim] of ``dtype`` (float32 for an f32 cache,
     else bfloat16, by default).  Rows from ``counts[b]`` on are zero in new tensors, and left as
-    they are in ``out``, whose strides may be any with a unit last one.
+    they are in ``out``, whose strides may be any with a unit last one, and whose memory is neither
+    shared between the two nor with the rows that are read.
     """
     shape = (cache.batch, cache.heads, int(rows), cache.head_dim)
     if out is None:
@@ -254,7 +255,8 @@ def tree_decode(q: torch.Tensor, cache: KVCache, kv_lens: torch.Tensor, *,
     ``tree[b, i]`` is set (``tree_words``; int64 [batch, n], or [n] for one tree of all; without
     it, nodes 0..i).  ``nodes`` (int32 [batch]) is how many of the n nodes each sequence has; the
     rest is padding, and gives zeros like a node that sees nothing.  What a node does not see does
-    not reach its output, whatever it holds.
+    not reach its output, whatever it holds.  Over e4m3 and int4 rows errors are relative to the
+    largest value that a node sees.
 
     Returns [batch, heads_q, n, head_dim] of q's dtype (``out`` where given).
     """

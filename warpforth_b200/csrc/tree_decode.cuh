@@ -2,8 +2,8 @@
 // instantiation a row format, head size, query type and number of query rows.
 //
 // The rows of queries that share one cache head, R = heads_q / heads * nodes,
-// are attended together, so every cache row is read once for all of them.  The
-// kernel works on transposed products, whose narrow side (8) holds queries:
+// are attended together, up to 32 in a tile: every cache row is read once a tile.
+// The kernel works on transposed products, whose narrow side (8) holds queries:
 //
 //   S^T [16 keys x 8 queries] = K [16 x D] Q^T [D x 8]
 //   O^T [D x 8 queries]      += V^T [D x 16 keys] P^T [16 x 8]
@@ -38,10 +38,12 @@
 // 40 us), so there a second kernel does.
 // Four warps split the keys of a unit or, with more rows, the rows.
 //
-// HBM bounds it where the conversion is short, issue slots where it is not.  One
-// token, ragged lengths: bf16 rows of 64 values 5.9 TB/s, e4m3 rows of 128 5.6,
-// e4m3 rows of 64 4.7 (64 x 25 heads, 145,600 keys of each head: 104 us), 4-bit
-// rows of 128 under 8 query heads 3.8 (32 x 8 heads, 342,100 keys: 98 us).
+// HBM bounds it where the conversion is short; where it is not, the latency of
+// unpacking, product, exponential and product with the 12 to 16 warps an SM that
+// the registers leave (half the issue slots stay empty).  One token, ragged lengths:
+// rows of 64 values, 64 x 25 heads, 145,700 keys of each, bf16 6.4 TB/s (145 us),
+// e4m3 4.6 (107); rows of 128, 8 heads, 326,100 keys of each, e4m3 5.8 (119), 4 bits
+// under 8 query heads 3.9 (90).
 #pragma once
 
 #include <float.h>

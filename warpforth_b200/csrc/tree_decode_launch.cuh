@@ -10,8 +10,9 @@ namespace tree {
 // 8 or 16 rows a warp, then pairs of warps take different rows; above 32 rows
 // bf16 queries go to tcgen05, whose 128 rows cost the same however many are
 // there (8 cache heads, 196122 e4m3 keys of each in two sequences, head_dim
-// 128: 20 rows 162 us against 216 on tcgen05, 32 rows 177 against 231, 60 rows
-// 298 against 277, 244 rows 850 against 485).  f32 queries, whose products need
+// 128: 20 rows 119 us against 192 on tcgen05, 32 rows 123 against 192, 60 rows
+// 216 against 206, 244 rows 784 against 391; 60 rows over 40134 keys of each in
+// 16 sequences 70 against 83, bf16 keys 78 against 67).  f32 queries, whose products need
 // more terms, stay with warps that take different rows.
 template <int kFmt, bool kF32, int D, class F>
 auto with_rows(int R, F f) {

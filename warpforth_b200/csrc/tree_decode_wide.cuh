@@ -23,12 +23,16 @@
 // P V of i.  TMEM columns: twice 64 for S and P, 64 or 128 for O; 256 a CTA, two
 // CTAs an SM.
 //
+// With more than 128 query rows a cache head the tiles are segments of their own,
+// and each reads and converts the keys again.
+//
 // Measured: 61-node trees of 4 query heads a cache head over two e4m3 caches of
-// 65,000 and 131,000 keys, 8 heads of 128: 410 us, 478 TFLOP/s.  A unit takes a
+// 65,000 and 131,000 keys, 8 heads of 128: 412 us, 476 TFLOP/s.  A unit takes a
 // CTA about 4,000 clocks; rows are placed in 1,350, S is there 1,500 after Q K^T
 // begins, weights take 2,400 and P V 840.  No one of them is the bound: without
 // weights it would be 286 us, without conversion 349, with half the products 390.
-// 15-node trees over 37,840 keys of 8 heads: 65 us (bf16), 69 (4 bits).
+// 15-node trees, 16 sequences, 40,134 keys of each of 8 heads: 65 us (bf16), 70 (4
+// bits), 82 (e4m3).
 //
 // Every wait has a limit.  After one that runs out the warps that make weights
 // go on to the end without waiting; the two of a row meet as often as ever.
@@ -51,10 +55,10 @@ struct WideCfg {
   static constexpr bool kScaled = !kBf16Rows;
   static constexpr int kRowBytes = CacheRow<kFmt, D>::kBytes;
   // Threads of a query row.  4-bit rows take two, as their minima make the weights
-  // dearer: 15-node trees, 4 query heads on 8, 69 us against 79 (64 values a row: 52
-  // against 58); 61-node trees over 196,000 keys 417 against 434 (319 against 302).
-  // The others lose more by having 80 registers a thread: bf16 74 against 66, e4m3
-  // 91 against 81.
+  // dearer: 15-node trees, 4 query heads on 8, 70 us against 80 (64 values a row: 55
+  // against 57); 61-node trees over 196,000 keys 398 against 403 (319 against 286).
+  // The others have nothing from it, or lose by 80 registers a thread: bf16 67 us
+  // both ways, e4m3 97 against 83.
   static constexpr int kHalves = kFmt == WFATTN_CACHE_INT4 ? 2 : 1;
   static constexpr int kWeighers = kHalves * kThreads, kWideThreads = kWeighers + kThreads;
   static constexpr int kMine = kKeys / kHalves, kDims = D / kHalves;  // of a thread's row
