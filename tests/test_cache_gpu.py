@@ -830,6 +830,34 @@ def test_trees_over_one_long_sequence(wf, fmt, dtype, d, g, n):
     check(out, ref, tol)
 
 
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+def test_the_smallest_cache(wf, fmt, dtype):
+    for d in (64, 128):
+        cache = make_cache(wf, fmt, 1, 1, 1, d, 39)
+        q = torch.randn(1, 70, 1, d, generator=torch.Generator().manual_seed(39)).to(TYPES[dtype])
+        for g in (1, 12, 70):
+            for length, nodes in ((0, 1), (1, 0), (0, 0)):
+                out = wf.tree_decode(q[:, :g].cuda(), cache, ints([length]), nodes=ints([nodes]))
+                ref, tol = attend(fmt, cache, q[:, :g], [length], [[1]], [nodes])
+                check(out, ref, tol)
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+def test_the_most_query_rows(wf, fmt, dtype):
+    """2^20 of one cache head: 16,384 query heads that are one in memory, of 64 nodes."""
+    d, g, n, length = 64, 1 << 14, 64, 70
+    cache = make_cache(wf, fmt, 1, 1, length + n, d, 40)
+    q = torch.randn(1, 1, n, d, generator=torch.Generator().manual_seed(40)).to(TYPES[dtype])
+    words = wf.tree_words(random_trees(1, n, 40)[0])
+    out = wf.tree_decode(q.cuda().expand(1, g, n, d), cache, ints([length]), tree=words.cuda())
+    ref, tol = attend(fmt, cache, q, [length], [words.tolist()], [n])
+    check(out[:, :1], ref, tol)
+    check(out[:, -1:], ref, tol)
+    low, high = out.amin(1, keepdim=True), out.amax(1, keepdim=True)
+    check(low, ref, tol)
+    check(high, ref, tol)
+
+
 # ---------------------------------------------------------------------- used together
 
 

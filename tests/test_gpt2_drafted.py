@@ -202,6 +202,17 @@ def test_quantised_caches_generate(gpt2, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int4"])
+@pytest.mark.parametrize("nodes", [1, 64])
+def test_bf16_models_generate(gpt2, fmt, nodes):
+    model = gpt2.random_gpt2(seed=4).bfloat16()
+    prompt = gpt2.synthetic_prompt(40, seed=4)
+    got, runs = gpt2.generate_drafted(model, prompt, 12, nodes=nodes, cache=fmt, prompt_chunk=17)
+    assert got.shape == (1, 52) and got[0, :40].tolist() == prompt[0].tolist()
+    assert 1 <= runs <= 11 and (nodes > 1 or runs == 11)
+
+
+@pytest.mark.gpu
 def test_generation_to_the_last_position(gpt2):
     model = gpt2.random_gpt2(seed=3)
     prompt = torch.arange(990).remainder(5)[None]
